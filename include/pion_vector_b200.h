@@ -231,6 +231,8 @@ int pion_v_b200_beam_forget(const uint32_t *l0_compact);
  * recorded for messages only. */
 int pion_v_b200_init(int device, int worker_id, pion_b200_ctx **out_ctx);
 int pion_v_b200_shutdown(pion_b200_ctx *ctx);
+/* The CUDA device the context runs on. */
+int pion_v_b200_ctx_device(const pion_b200_ctx *ctx);
 /* Run this context's work on an existing CUDA stream (cudaStream_t), e.g. a
  * framework's current stream; NULL restores the context's own stream (pass
  * cudaStreamLegacy for the legacy default stream).  Work queued after a switch waits
@@ -451,6 +453,92 @@ int pion_v_b200_flat_i8_knn_sharded(pion_b200_ctx *ctx, const pion_b200_index *i
                                     pion_b200_exchange *ex, const int8_t *q, const float *q_scale,
                                     int64_t nq, int64_t k, uint32_t epoch, int flags,
                                     int32_t *out_ids, float *out_scores);
+
+/* ---------------------------------------- microscaled 4-bit floating point -- */
+/* Rows held in 4 bits an element, quantised as they are written, read back, multiplied with
+ * query batches and searched.  No counterpart in the reference.  Formats:
+ *   MX  blocks of 32: s = 2^(floor(log2 bmax) - 2) as e8m0, code = e2m1(x / s); g = 1
+ *   NV  blocks of 16: g = amax / 2688 (float32, per row), s = e4m3(bmax / f32(6 g)),
+ *       code = e2m1(x / f32(s g))
+ * amax, bmax: the largest magnitude of the row, of the block.  e2m1 holds 0, .5, 1, 1.5, 2,
+ * 3, 4, 6 and their negatives; every rounding is to nearest, ties to even, of the exact
+ * quotient, saturating.  A row of zeros, and in NV one whose amax is below 2^-100, is held
+ * as zeros with g = 0.  A row with a NaN or an infinity cannot be held: its slot becomes
+ * empty (g = NaN).  An empty slot reads as NaN, scores -inf and is never found. */
+#define PION_B200_FP4_MX 0
+#define PION_B200_FP4_NV 1
+
+/* Element types of rows, queries and outputs of the calls below. */
+#define PION_B200_F32 0
+#define PION_B200_BF16 1
+#define PION_B200_F16 2
+
+/* A store of rows: the caller's DEVICE buffers (16-byte aligned), which every call below
+ * reads or writes in place.  dp = dim rounded up to a multiple of 128.  Calls of several
+ * contexts or streams on one store are ordered by the caller: a write runs alone.
+ *
+ * `cuda_stream` (a cudaStream_t; cudaStreamLegacy for the legacy default stream): with `mem`
+ * DEVICE the call runs on that stream, NULL being the context's.  Calls with DEVICE memory
+ * on a stream of their own use no memory of the context's (scores and search then need a
+ * `workspace`) but its status word, and may be captured into a CUDA graph, which keeps
+ * using the pointers it was captured with. */
+typedef struct pion_b200_fp4_rows {
+    int32_t format;      /* PION_B200_FP4_* */
+    int32_t reserved;
+    int64_t n_rows;      /* slots */
+    int64_t dim;         /* 1 <= dim <= 8192 */
+    uint8_t *codes;      /* [n_rows][dp / 2], the lower nibble first */
+    uint8_t *scales;     /* [ceil(n_rows / 128)][atoms][32][4][4], atoms = dp / 128 (MX) or
+                            dp / 64 (NV): block b of row r at tile r / 128, atom b / 4,
+                            [r % 32][r % 128 / 32][b % 4] */
+    float *row_scale;    /* [n_rows]: g; NaN = empty */
+    float *norm_max;     /* [1]: at least every row's norm so far (never lowered) */
+    int32_t *claim;      /* [n_rows], zero between calls; needed by writes with slots, else
+                            may be NULL */
+} pion_b200_fp4_rows;
+
+/* Bytes of a store's codes and scales. */
+int pion_v_b200_fp4_sizes(int format, int64_t n_rows, int64_t dim, int64_t *codes_bytes,
+                          int64_t *scales_bytes);
+/* Empties every slot (norm_max = 0, claim = 0). */
+int pion_v_b200_fp4_clear(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, void *cuda_stream);
+/* Quantises n rows of `type` (row i at src + i * stride elements, stride >= dim) into slots
+ * slots[i], or start + i where slots is NULL.  A negative slot skips its row; of several
+ * rows for one slot the last is kept; other slots stay as they were.  A slot past the store
+ * is PION_B200_EINVAL, nothing written: from the call with `mem` HOST (src and slots in host
+ * memory), from pion_v_b200_sync with DEVICE (there the rows of valid slots are written). */
+int pion_v_b200_fp4_write(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, const void *src,
+                          int type, int64_t stride, int64_t n, const int64_t *slots,
+                          int64_t start, int mem, void *cuda_stream);
+/* Reads n slots back as rows of `type`: f32((code s) g), rounded to the type.  A negative
+ * slot leaves its row of dst as it was (with `mem` DEVICE; HOST refuses it). */
+int pion_v_b200_fp4_read(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows,
+                         const int64_t *slots, int64_t start, int64_t n, void *dst, int type,
+                         int64_t stride, int mem, void *cuda_stream);
+
+/* Workspace of the two calls below for nq queries over `n_rows` rows (k = 0:
+ * pion_v_b200_fp4_scores), in bytes; negative: a status. */
+int64_t pion_v_b200_fp4_workspace(const pion_b200_fp4_rows *rows, int64_t n_rows, int64_t nq,
+                                  int64_t k);
+/* Scores of every query with the rows of slots [0, n_rows): out[t * out_stride + r] =
+ * ((sum_j q_j v_j) g_r) g_t, accumulated in float32.  q: nq rows of q_type, quantised here
+ * in the store's format.  With `mem` DEVICE the scratch is the caller's `workspace`
+ * (16-byte aligned; pion_v_b200_fp4_workspace bytes), or the context's where both it and
+ * cuda_stream are NULL. */
+int pion_v_b200_fp4_scores(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, int64_t n_rows,
+                           const void *q, int q_type, int64_t q_stride, int64_t nq, void *out,
+                           int out_type, int64_t out_stride, void *workspace,
+                           int64_t workspace_bytes, int mem, void *cuda_stream);
+/* The k best of slots [0, n_rows) by (score desc, slot asc) -> out_ids (id_base + slot) and
+ * out_scores [nq x k]; -1 / -inf past the rows that are not empty.  Here a score is
+ * f32(((sum) g_r) g_t) of the sum in float64, so the ids do not depend on an order of
+ * summation.  k <= 256.  A query whose candidates overflow (thousands of rows that tie with
+ * its k-th) is answered by an exact scan of its rows, one CTA per query. */
+int pion_v_b200_flat_fp4_knn(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, int64_t n_rows,
+                             int64_t id_base, const void *q, int q_type, int64_t q_stride,
+                             int64_t nq, int64_t k, int32_t *out_ids, float *out_scores,
+                             void *workspace, int64_t workspace_bytes, int mem,
+                             void *cuda_stream);
 
 /* ------------------------------------------------------------------- HNSW -- */
 

@@ -6,6 +6,7 @@ API (``search``), the build recipe (``build``) and the synthetic workload
 generator (``workloads``).
 """
 from ._lib import PionError, load  # noqa: F401
+from .fp4 import FP4Rows, FlatFP4Index, fp4_scores, quantize_rows_fp4  # noqa: F401
 from .search import (  # noqa: F401
     BQIndex,
     Context,
@@ -23,5 +24,6 @@ from .search import (  # noqa: F401
 )
 
 __all__ = ["Context", "FlatI8Index", "FlatF32Index", "BQIndex", "HNSWGraph", "HNSWIndex",
-           "HNSWQuant", "HNSWQuantIndex", "quantize_rows_i8",
+           "HNSWQuant", "HNSWQuantIndex", "FP4Rows", "FlatFP4Index", "quantize_rows_fp4",
+           "fp4_scores", "quantize_rows_i8",
            "l2_normalize_rows", "merge_topk", "merge_topk_pairs", "rescore_knn", "PionError", "load"]

@@ -32,6 +32,12 @@ MERGE_LISTS_MAJOR = 2
 MERGE_PAIRS = 4
 IPC_HANDLE_BYTES = 64
 
+FP4_MX = 0
+FP4_NV = 1
+F32 = 0
+BF16 = 1
+F16 = 2
+
 ABI_VERSION = 1
 
 _P = ctypes.c_void_p
@@ -115,6 +121,16 @@ SIGNATURES = {
     "pion_v_b200_hnsw_save_quant": (_I, [_P, _P, ctypes.c_char_p, _I64]),
     "pion_v_b200_hnsw_quant_search": (_I, [_P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _I]),
     "pion_v_b200_beam_forget": (_I, [_P]),
+    "pion_v_b200_ctx_device": (_I, [_P]),
+    "pion_v_b200_fp4_sizes": (_I, [_I, _I64, _I64, _P, _P]),
+    "pion_v_b200_fp4_clear": (_I, [_P, _P, _P]),
+    "pion_v_b200_fp4_write": (_I, [_P, _P, _P, _I, _I64, _I64, _P, _I64, _I, _P]),
+    "pion_v_b200_fp4_read": (_I, [_P, _P, _P, _I64, _I64, _P, _I, _I64, _I, _P]),
+    "pion_v_b200_fp4_workspace": (_I64, [_P, _I64, _I64, _I64]),
+    "pion_v_b200_fp4_scores": (_I, [_P, _P, _I64, _P, _I, _I64, _I64, _P, _I, _I64, _P, _I64,
+                                    _I, _P]),
+    "pion_v_b200_flat_fp4_knn": (_I, [_P, _P, _I64, _I64, _P, _I, _I64, _I64, _I64, _P, _P, _P,
+                                      _I64, _I, _P]),
 }
 
 
@@ -135,6 +151,15 @@ class HnswQuantLayout(ctypes.Structure):
                 ("qjl_res_norms", ctypes.c_void_p), ("qjl_random_signs", ctypes.c_void_p),
                 ("qjl_lambda", ctypes.c_float), ("reserved2", ctypes.c_int32),
                 ("rerank", ctypes.c_void_p)]
+
+
+class FP4RowsDesc(ctypes.Structure):
+    """pion_b200_fp4_rows (include/pion_vector_b200.h)."""
+    _fields_ = [("format", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("n_rows", ctypes.c_int64), ("dim", ctypes.c_int64),
+                ("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("row_scale", ctypes.c_void_p), ("norm_max", ctypes.c_void_p),
+                ("claim", ctypes.c_void_p)]
 
 
 class LinearPool(ctypes.Structure):

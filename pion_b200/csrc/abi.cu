@@ -154,7 +154,10 @@ static int sync_words(pion_b200_ctx* ctx, int first, int last) {
             ctx->h_status[w] = 0;
             cudaMemsetAsync(ctx->d_status + w, 0, sizeof(int), ctx->stream);
             cudaStreamSynchronize(ctx->stream);
-            return set_error(ctx, st, "device-side wait gave up (status %d, %s-memory call)",
+            return set_error(ctx, st,
+                             st == PION_B200_ETIMEOUT
+                                 ? "device-side wait gave up (status %d, %s-memory call)"
+                                 : "device-side check failed (status %d, %s-memory call)",
                              st, w == 0 ? "host" : "device");
         }
     }
@@ -169,6 +172,14 @@ int use_device(pion_b200_ctx* ctx) {
     if (cudaSetDevice(ctx->device) != cudaSuccess)
         return set_error(ctx, PION_B200_ENODEV, "cudaSetDevice(%d) failed", ctx->device);
     return 0;
+}
+
+bool stream_capturing(cudaStream_t st) {
+    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+    const cudaError_t e = cudaStreamIsCapturing(st, &s);
+    if (e != cudaSuccess) cudaGetLastError();
+    // the legacy stream cannot be asked while another stream is captured
+    return e == cudaErrorStreamCaptureImplicit || s != cudaStreamCaptureStatusNone;
 }
 
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
@@ -267,6 +278,10 @@ int pion_v_b200_shutdown(pion_b200_ctx* ctx) {
     for (cudaEvent_t e : ctx->ev_end) cudaEventDestroy(e);
     delete ctx;
     return 0;
+}
+
+int pion_v_b200_ctx_device(const pion_b200_ctx* ctx) {
+    return valid_ctx(ctx) ? ctx->device : PION_B200_EINVAL;
 }
 
 int pion_v_b200_set_stream(pion_b200_ctx* ctx, void* cuda_stream) {

@@ -306,6 +306,7 @@ int queue_status_readback(pion_b200_ctx* ctx);
 int* call_status(pion_b200_ctx* ctx, int mem);
 int finish_sync(pion_b200_ctx* ctx);
 bool valid_ctx(const pion_b200_ctx* ctx);
+bool stream_capturing(cudaStream_t st);
 int use_device(pion_b200_ctx* ctx);
 size_t align_up(size_t x, size_t a);
 int prepass_tiles(int k);
@@ -460,6 +461,104 @@ int launch_slot_finish(const float* st_d, const int32_t* st_i, int nq, int k, co
                        const float* rerank, const int32_t* slot_ext, int64_t n, int final_k,
                        int k_out, int32_t* out_ids, float* out_scores, int32_t* out_found,
                        cudaStream_t st);
+
+// ---- fp4_rows.cu
+struct Fp4Write {
+    int format = 0;
+    int dim = 0;
+    const void* src = nullptr;
+    int type = 0;
+    int64_t stride = 0;
+    int64_t n = 0;
+    const int64_t* slots = nullptr;
+    int64_t start = 0;
+    int64_t n_slots = 0;
+    int32_t* claim = nullptr;
+    int tile = 0, tile_pad = 0;  // a query batch: rows in groups of `tile` every `tile_pad` slots
+    uint8_t* codes = nullptr;
+    uint8_t* scales = nullptr;
+    float* row_scale = nullptr;
+    float* norm = nullptr;
+    float* norm_max = nullptr;
+    int* status = nullptr;
+};
+int launch_fp4_write(const Fp4Write& w, cudaStream_t st);
+struct Fp4Read {
+    int format = 0;
+    int dim = 0;
+    const uint8_t* codes = nullptr;
+    const uint8_t* scales = nullptr;
+    const float* row_scale = nullptr;
+    int64_t n_slots = 0;
+    const int64_t* slots = nullptr;
+    int64_t start = 0;
+    int64_t n = 0;
+    void* dst = nullptr;
+    int type = 0;
+    int64_t stride = 0;
+    int* status = nullptr;
+};
+int launch_fp4_read(const Fp4Read& r, cudaStream_t st);
+
+// ---- flat_fp4.cu
+struct Fp4Plan {
+    int nt = 0, nt_pad = 0, n_qt = 0;  // queries per tile, their slots, tiles
+};
+int fp4_max_dim();
+int fp4_cap();
+int fp4_tile_rows();
+bool fp4_plan(int format, int dp, int nq, Fp4Plan* out);
+struct Fp4Product {
+    int format = 0;
+    int dim = 0;
+    const uint8_t* codes = nullptr;
+    const uint8_t* scales = nullptr;
+    const float* row_scale = nullptr;
+    int64_t store_rows = 0;
+    int64_t n_rows = 0;
+    const uint8_t* q_codes = nullptr;
+    const uint8_t* q_scales = nullptr;
+    const float* q_scale = nullptr;
+    int nq = 0;
+    int n_tiles = 0;   // > 0: only that many row tiles, every tile_step-th
+    int tile_step = 1;
+    void* out = nullptr;
+    int out_type = 0;
+    int64_t ld = 0;
+    const float* theta = nullptr;  // collect candidates instead of writing scores
+    int* cand_n = nullptr;
+    uint64_t* cand = nullptr;
+    int* status = nullptr;
+    uint64_t wait_ns = kDefaultWaitNs;
+    int num_sms = 148;
+};
+int launch_fp4_product(const Fp4Product& L, cudaStream_t st);
+// from the sample's scores, or with `cand` from the candidates kept so far
+int launch_fp4_theta(const float* sample, int64_t ld, int m, const uint64_t* cand, int k, int dim,
+                     const float* q_scale, int nt, int nt_pad, const float* q_norm,
+                     const float* norm_max, int nq, float* theta, int* cand_n, cudaStream_t st);
+struct Fp4Finish {
+    int format = 0;
+    int dim = 0;
+    const uint8_t* codes = nullptr;
+    const uint8_t* scales = nullptr;
+    const float* row_scale = nullptr;
+    const float* norm_max = nullptr;
+    int64_t n_rows = 0;
+    int64_t id_base = 0;
+    const uint8_t* q_codes = nullptr;
+    const uint8_t* q_scales = nullptr;
+    const float* q_scale = nullptr;
+    const float* q_norm = nullptr;
+    int nt = 0, nt_pad = 0, nq = 0, k = 0;
+    const float* dense = nullptr;
+    int64_t ld = 0;
+    const int* cand_n = nullptr;
+    const uint64_t* cand = nullptr;
+    int32_t* out_ids = nullptr;
+    float* out_scores = nullptr;
+};
+int launch_fp4_finish(const Fp4Finish& L, cudaStream_t st);
 
 // ---- bq.cu
 int bq_tile_rows();
