@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdlib>
 
 #include "fp4.cuh"
@@ -16,7 +17,9 @@ constexpr int64_t kMaxRows = (int64_t)INT32_MAX - 256;  // slots are 32-bit TMA 
 constexpr int64_t kMaxK = 256;
 constexpr int64_t kMaxQueries = 1 << 24;
 constexpr int64_t kQueryChunk = 4096;  // queries searched at once: bounds the scratch (64 KB each)
-constexpr int kSampleTiles = 64;       // row tiles scored for the first threshold
+// Row tiles scored for the first threshold: more for few queries, where a part of the rows less
+// to score again counts for more than a longer selection.
+int sample_tiles(int64_t nq) { return nq <= 64 ? 64 : 32; }
 
 int elem_bytes(int type) { return type == PION_B200_F32 ? 4 : 2; }
 bool type_ok(int type) { return type >= PION_B200_F32 && type <= PION_B200_F16; }
@@ -77,7 +80,7 @@ struct Scratch {
 bool plan_scratch(int format, int dim, int64_t n_rows, int64_t nq, int64_t k, Scratch* out) {
     const int dp = fp4::pad_dim(dim);
     Scratch s;
-    if (!fp4_plan(format, dp, (int)nq, &s.plan)) return false;
+    if (!fp4_plan(format, dp, (int)nq, n_rows, &s.plan)) return false;
     const size_t slots = (size_t)s.plan.n_qt * s.plan.nt_pad;
     size_t off = 0;
     auto take = [&](size_t bytes) {
@@ -91,7 +94,7 @@ bool plan_scratch(int format, int dim, int64_t n_rows, int64_t nq, int64_t k, Sc
     s.q_norm = take((size_t)nq * 4);
     s.theta = s.cand_n = s.sample = s.cand = 0;
     if (k > 0) {
-        const int64_t most = (int64_t)kSampleTiles * fp4_tile_rows();
+        const int64_t most = (int64_t)sample_tiles(nq) * fp4_tile_rows();
         s.theta = take((size_t)nq * 4);
         s.cand_n = take((size_t)nq * 4);
         s.sample = take((size_t)nq * (n_rows < most ? n_rows : most) * 4);
@@ -224,12 +227,13 @@ int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, i
     if (rc != 0) return rc;
 
     const int64_t n_tiles = (n_rows + fp4_tile_rows() - 1) / fp4_tile_rows();
-    const bool dense = n_tiles <= kSampleTiles;
-    const int64_t m = dense ? n_rows : (int64_t)kSampleTiles * fp4_tile_rows();
+    const int samples = sample_tiles(nq);
+    const bool dense = n_tiles <= samples;
+    const int64_t m = dense ? n_rows : (int64_t)samples * fp4_tile_rows();
     timing_begin(ctx);
     Fp4Product L = product_of(ctx, r, n_rows, nq, s, base, mem);
-    L.n_tiles = (int)(dense ? n_tiles : kSampleTiles);
-    L.tile_step = dense ? 1 : (int)(n_tiles / kSampleTiles);
+    L.n_tiles = (int)(dense ? n_tiles : samples);
+    L.tile_step = dense ? 1 : (int)(n_tiles / samples);
     L.out = sample;
     L.out_type = PION_B200_F32;
     L.ld = m;
@@ -237,19 +241,23 @@ int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, i
     ctx->launches++;
     if (!dense && rc == 0) {
         rc = launch_fp4_theta(sample, m, (int)m, nullptr, (int)k, (int)r->dim, q_scale,
-                              s.plan.nt, s.plan.nt_pad, q_norm, r->norm_max, (int)nq, theta, cand_n, st);
+                              s.plan.nt, s.plan.nt_pad, q_norm, r->norm_max, (int)nq, theta,
+                              cand_n, st);
         ctx->launches++;
         L.theta = theta;
         L.cand_n = cand_n;
         L.cand = cand;
-        // About k * (rows scored) / (rows of the last threshold) rows reach the threshold.
-        const int64_t target = fp4_cap() / 4;
-        int64_t have = kSampleTiles;
+        // About k (rows scored) / (rows of the last threshold) rows reach the threshold, with a
+        // deviation of 1 / sqrt(k) of that: `grow` leaves 13 deviations of room in the lists.
+        const double grow = fp4_cap() / ((double)k + 13.0 * sqrt((double)k));
+        int64_t have = samples;
         while (rc == 0) {
+            const double ratio = (double)n_tiles / (double)have;
             int64_t next = n_tiles;
-            if (k * n_tiles > target * have) {
-                const int64_t grow = target / k > 2 ? target / k : 2;
-                next = have * grow < n_tiles ? have * grow : n_tiles;
+            if (ratio > grow || (nq > 64 && ratio > 16.0)) {
+                const double by = ratio > grow * grow ? grow : sqrt(ratio);
+                next = (int64_t)((double)have * (by > 2.0 ? by : 2.0));
+                if (next > n_tiles) next = n_tiles;
             }
             L.tile_step = (int)(n_tiles / next);
             L.n_tiles = (int)next;

@@ -29,13 +29,21 @@
 namespace pion {
 namespace fp4 {
 
-constexpr int ROWS = 128;                // rows per CTA tile (UMMA M per CTA, TMEM lanes)
+constexpr int HALF = 128;                // rows per CTA (TMEM lanes)
+constexpr int ROWS = 2 * HALF;           // rows per tile: a CTA pair (UMMA M = 256)
 constexpr int KC = 128;                  // code bytes of K per pipeline stage (256 elements)
-constexpr int A_BYTES = ROWS * KC;       // 16 KB
-constexpr int EPI_WARPS = 8;             // two per TMEM lane quarter, alternate column chunks
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int A_BYTES = HALF * KC;       // 16 KB
+// Four warpgroups: the scale warps; the loading and the MMA warp (and two idle ones); two of
+// epilogue warps, two per TMEM lane quarter.  An epilogue thread holds up to 128
+// accumulators, so that one buffer of them is free again as soon as it is read.
+constexpr int EPI_WARPS = 8;
+constexpr int SCALE_WARPS = 4;
+constexpr int THREADS = 512;             // 128 registers a thread at launch ...
+constexpr int REGS_SCALE = 88, REGS_ISSUE = 40, REGS_EPI = 192;  // ... and 4 * 128 in all here
+static_assert(REGS_SCALE + REGS_ISSUE + 2 * REGS_EPI <= 4 * 128, "register split");
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int MAX_STAGES = 8;
+constexpr int MAX_NT = 256;
 constexpr int SMEM_MAX = 232448;         // 227 KB
 constexpr int CAP = 4096;                // candidates kept per query
 constexpr int LIST = 2048;               // of which at most this many are scored exactly
@@ -52,17 +60,25 @@ __host__ __device__ constexpr float rel_eps(int dp) { return (float)(dp / 64 + 8
 
 enum Mode { kScores = 0, kCollect = 1 };
 
+// Shared-memory and TMEM plan of one launch.
+struct Plan {
+    int nt, nt_pad, n_qt;     // queries per tile, their slots (a multiple of 128), tiles
+    int kchunks;              // stages per tile
+    int stages;
+    int bufs;                 // accumulator buffers of nt columns
+    int sets;                 // sets of row-scale columns
+    int resident;             // 1: the queries' scales stay in TMEM, 0: they are in the sets
+    int smem;
+};
+
 struct TcParams {
     const float* row_scale;   // [n_rows]
     const float* q_scale;     // [query slot]
     int64_t n_rows;
     int nq;
-    int nt, nt_pad;           // queries per tile, and their slots (a multiple of 128)
-    int n_qt;
-    int kchunks;              // stages per tile
+    Plan plan;
     int mmas;                 // 64-element steps per tile
-    int atoms;                // scale atoms per row tile
-    int stages;
+    int atoms;                // scale atoms per 128 rows
     int n_tiles;              // row tiles of this launch ...
     int tile_step;            // ... the j-th being tile j * tile_step
     // kScores
@@ -77,21 +93,72 @@ struct TcParams {
     uint64_t wait_ns;
 };
 
-// Shared-memory plan of one launch.
-struct Plan {
-    int nt, nt_pad, n_qt, kchunks, stages;
-    int b_bytes, sfb_bytes, stage_bytes, smem;
-};
-
 // ------------------------------------------------------------- PTX pieces --
-// Scale atoms in shared memory: 32 rows of 16 bytes, no swizzle, 8-row groups 128 B apart.
-__device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
-    d |= static_cast<uint64_t>(128u >> 4) << 16;
-    d |= static_cast<uint64_t>(128u >> 4) << 32;
-    d |= static_cast<uint64_t>(1u) << 46;
-    return d;
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
+                 "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrives on the first CTA's copy of a barrier.
+__device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .b32 remote;\n\tmapa.shared::cluster.u32 remote, %0, 0;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n\t}\n" ::"r"(
+            smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// mbar_wait for phases that the other CTA's threads arrive on.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* status,
+                                                  volatile int* abort_flag, uint64_t budget_ns) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    uint32_t spins = 0;
+    for (;;) {
+        if (mbar_try_wait_cluster(bar, parity)) return true;
+        if ((++spins & 63u) == 0) {
+            if (*abort_flag) return false;
+            if (globaltimer_ns() - t0 > budget_ns) {
+                record_error(status, PION_B200_ETIMEOUT);
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_slot, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(smem_slot)),
+                 "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
+                 : "memory");
+}
+// Arrives on both CTAs' copies of a barrier when the MMAs issued so far are done.
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
 }
 
 // Instruction descriptor of the block-scaled kinds: e2m1 x e2m1 -> f32, both K-major.
@@ -101,11 +168,6 @@ __host__ __device__ constexpr uint32_t make_idesc_fp4(int m, int n) {
            ((FMT == kMX ? 1u : 0u) << 23) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void tc_cp_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
-                 : "memory");
-}
-
 template <int FMT>
 __device__ __forceinline__ void mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                         uint32_t idesc, uint32_t sfa, uint32_t sfb,
@@ -113,17 +175,27 @@ __device__ __forceinline__ void mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64
     if (FMT == kMX)
         asm volatile(
             "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
             " [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
             "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
             : "memory");
     else
         asm volatile(
             "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X"
             " [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
             "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
             : "memory");
+}
+
+// This warp's lanes of four consecutive columns of TMEM.
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint4& r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr),
+                 "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 // Orders floats as unsigned integers; NaN is put below everything by the callers.
@@ -160,105 +232,217 @@ __device__ __forceinline__ void store_chunk(const uint32_t (&r)[32], const TcPar
     }
 }
 
+// One chunk of one row's scores: written, or the row appended to the lists of the queries
+// whose threshold it reaches.
+__device__ __forceinline__ void epilogue_chunk(const uint32_t (&r)[32], const TcParams& p, int mode,
+                                               int t0, int cols, bool row_in, int64_t row,
+                                               int64_t col, const float* gq, const float* th,
+                                               float g) {
+    if (mode == kScores) {
+        if (row_in && cols > 0) {
+            if (p.out_type == PION_B200_F32)
+                store_chunk<float>(r, p, t0, cols, col, gq, g);
+            else if (p.out_type == PION_B200_BF16)
+                store_chunk<__nv_bfloat16>(r, p, t0, cols, col, gq, g);
+            else
+                store_chunk<__half>(r, p, t0, cols, col, gq, g);
+        }
+    } else {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) any |= __uint_as_float(r[i]) * g >= th[i];
+        if (any) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const float v = __uint_as_float(r[i]) * g;
+                if (v >= th[i]) {
+                    const int t = t0 + i;
+                    const int at = atomicAdd(&p.cand_n[t], 1);
+                    if (at < CAP)
+                        p.cand[(int64_t)t * CAP + at] =
+                            ((uint64_t)__float_as_uint(v * gq[i]) << 32) | (uint32_t)row;
+                }
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------ the product --
-// Warp 0 loads, warp 1 issues the MMAs, the others drain TMEM.  Accumulators are double
-// buffered at columns 0 and nt; above them two sets of scale columns, used in turn.  A set is
-// written again only after the MMAs that read it are done (sfree).
+// A CTA pair works on tiles of 256 rows, 128 per CTA, against its tile of queries: each CTA
+// keeps the codes of half of them in shared memory and streams its rows' codes and scales
+// through a ring.  Scale warps move the scales into TMEM -- the rows' per stage into sets of
+// columns used in turn, the queries' once where they fit (tcgen05.cp was tried first: its
+// copies queue with the MMAs, about 90 ns each, and took longer than them) -- and tell the
+// issuing thread of the first CTA, in one arrival, that codes and scales are there.
 template <int FMT>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     fp4_tc_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                   const __grid_constant__ CUtensorMap tmap_row_sf,
                   const __grid_constant__ CUtensorMap tmap_q,
-                  const __grid_constant__ CUtensorMap tmap_q_sf, TcParams p, int mode) {
+                  const __grid_constant__ CUtensorMap tmap_q_sf, const TcParams p, int mode) {
     constexpr int APS = atoms_per_stage(FMT);
     constexpr int STAGE = A_BYTES + APS * 512;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
+    // Both CTAs of a pair have the same shared-memory layout.
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
-    const int nt = p.nt;
-    const int sf_tiles = p.nt_pad / 128;
+    const int nt = p.plan.nt, kchunks = p.plan.kchunks, stages = p.plan.stages;
+    const int bufs = p.plan.bufs, sets = p.plan.sets;
+    const bool resident = p.plan.resident != 0;
+    const int sf_tiles = p.plan.nt_pad / 128;
     uint8_t* ring = smem;                                    // stages x (codes, scale atoms)
-    uint8_t* sB = ring + p.stages * STAGE;                   // [kchunk][query][128 B], swizzled
-    uint8_t* sSF = sB + p.kchunks * nt * KC;                 // [128-query tile][kchunk][APS]
-    float* s_gq = reinterpret_cast<float*>(sSF + sf_tiles * p.kchunks * APS * 512);
-    float* s_th = s_gq + 256;
-    uint64_t* full = reinterpret_cast<uint64_t*>(s_th + 256);
+    uint8_t* sB = ring + stages * STAGE;                     // [kchunk][nt / 2][128 B], swizzled
+    uint8_t* sSF = sB + kchunks * (nt / 2) * KC;             // [128-query tile][kchunk][APS]
+    if (resident) sSF = ring;                                // ... only until it is in TMEM
+    uint8_t* after = sB + kchunks * (nt / 2) * KC + (resident ? 0 : sf_tiles * kchunks * APS * 512);
+    float* s_gq = reinterpret_cast<float*>(after);
+    float* s_th = s_gq + MAX_NT;
+    uint64_t* full = reinterpret_cast<uint64_t*>(s_th + MAX_NT);
     uint64_t* empty = full + MAX_STAGES;
-    uint64_t* tfull = empty + MAX_STAGES;
-    uint64_t* tempty = tfull + 2;
-    uint64_t* sfree = tempty + 2;
-    uint64_t* bfull = sfree + 2;
-    uint64_t* drain = bfull + 1;
+    uint64_t* sready = empty + MAX_STAGES;   // per set, on the first CTA: both CTAs' stage is in
+    uint64_t* sfree = sready + MAX_STAGES;
+    uint64_t* tfull = sfree + MAX_STAGES;
+    uint64_t* tempty = tfull + 2;            // on the first CTA
+    uint64_t* bfull = tempty + 2;
+    uint64_t* qsf_done = bfull + 1;
+    uint64_t* drain = qsf_done + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int qt = blockIdx.x % p.n_qt;
-    const int lanes_of_work = gridDim.x / p.n_qt;  // CTAs per query tile
-    const int first = blockIdx.x / p.n_qt;
+    const uint32_t rank = cluster_rank();
+    const int pair = blockIdx.x >> 1;
+    const int qt = pair % p.plan.n_qt;
+    const int stride = (gridDim.x >> 1) / p.plan.n_qt;  // pairs per query tile
+    const int first = pair / p.plan.n_qt;
+    // TMEM columns: accumulators, query scales (resident), sets of scales
+    const uint32_t col_sfb = bufs * nt;
+    const uint32_t set_cols = APS * 4 * (1 + (resident ? 0 : sf_tiles));
+    const uint32_t col_sets = col_sfb + (resident ? sf_tiles * kchunks * APS * 4 : 0);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < MAX_STAGES; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&empty[s], 1 + SCALE_WARPS);
+            mbar_init(&sready[s], 2 * SCALE_WARPS);
+            mbar_init(&sfree[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&tfull[b], 1);
-            mbar_init(&tempty[b], EPI_WARPS);
-            mbar_init(&sfree[b], 1);
+            mbar_init(&tempty[b], 2 * EPI_WARPS);
         }
         mbar_init(bfull, 1);
+        mbar_init(qsf_done, SCALE_WARPS);
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
-    for (int j = threadIdx.x; j < 256; j += THREADS) {
+    for (int j = threadIdx.x; j < MAX_NT; j += THREADS) {
         const int t = qt * nt + j;
         const bool ok = j < nt && t < p.nq;
-        s_gq[j] = ok ? p.q_scale[(int64_t)qt * p.nt_pad + j] : 0.0f;
+        s_gq[j] = ok ? p.q_scale[(int64_t)qt * p.plan.nt_pad + j] : 0.0f;
         s_th[j] = ok && mode == kCollect ? p.theta[t] : INFINITY;
     }
-    if (warp == 1) {
-        tmem_alloc(tmem_slot, TMEM_COLS);
-        tmem_relinquish();
-    }
+    if (warp == 5) tmem_alloc_pair(tmem_slot, TMEM_COLS);
     tc_fence_before();
-    __syncthreads();
+    cluster_sync();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    if (warp == 0) {
-        // ------------------------------------------------------ TMA producer
-        if (lane == 0) {
+    if (warp < SCALE_WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_SCALE));
+        // -------------------------------------------------------- scale warps
+        const uint32_t lanes = tmem_base + ((uint32_t)(warp * 32) << 16);
+        bool ok = __all_sync(0xffffffffu,
+                             mbar_wait(bfull, 0, p.status, abort_flag, p.wait_ns));
+        if (ok && resident) {
+            for (int a = 0; a < kchunks * APS; ++a)
+                for (int h = 0; h < sf_tiles; ++h)
+                    tmem_st4(lanes + col_sfb + (a * sf_tiles + h) * 4,
+                             *reinterpret_cast<const uint4*>(
+                                 sSF + (h * kchunks * APS + a) * 512 + lane * 16));
+            tmem_st_wait();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qsf_done);
+        int stage = 0, set = 0;
+        uint32_t phase = 0, set_phase = 0;
+        for (int j = first; j < p.n_tiles && ok; j += stride) {
+            for (int kc = 0; kc < kchunks; ++kc) {
+                ok = __all_sync(0xffffffffu,
+                                mbar_wait(&full[stage], phase, p.status, abort_flag, p.wait_ns));
+                if (!ok) break;
+                uint4 v[APS];
+                const uint8_t* atoms = ring + stage * STAGE + A_BYTES;
+#pragma unroll
+                for (int a = 0; a < APS; ++a)
+                    v[a] = *reinterpret_cast<const uint4*>(atoms + a * 512 + lane * 16);
+                ok = __all_sync(0xffffffffu, mbar_wait(&sfree[set], set_phase ^ 1u, p.status,
+                                                       abort_flag, p.wait_ns));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = lanes + col_sets + set * set_cols;
+#pragma unroll
+                for (int a = 0; a < APS; ++a) tmem_st4(at + a * 4, v[a]);
+                if (!resident)
+                    for (int a = 0; a < APS; ++a)
+                        for (int h = 0; h < sf_tiles; ++h)
+                            tmem_st4(at + APS * 4 + (a * sf_tiles + h) * 4,
+                                     *reinterpret_cast<const uint4*>(
+                                         sSF + ((h * kchunks + kc) * APS + a) * 512 + lane * 16));
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive_leader(&sready[set]);
+                    mbar_arrive(&empty[stage]);
+                }
+                if (++stage == stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+                if (++set == sets) {
+                    set = 0;
+                    set_phase ^= 1u;
+                }
+            }
+        }
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
+        if (warp == 4 && lane == 0) {
+            // -------------------------------------------------- TMA producer
             tma_prefetch_desc(&tmap_rows);
             tma_prefetch_desc(&tmap_row_sf);
-            mbar_arrive_expect_tx(bfull, (uint32_t)(p.kchunks * nt * KC +
-                                                    sf_tiles * p.kchunks * APS * 512));
-            for (int kc = 0; kc < p.kchunks; ++kc) {
-                tma_load_2d(sB + kc * nt * KC, &tmap_q, bfull, kc * KC, qt * p.nt_pad);
+            const int half_nt = nt / 2;
+            mbar_arrive_expect_tx(bfull, (uint32_t)(kchunks * half_nt * KC +
+                                                    sf_tiles * kchunks * APS * 512));
+            for (int kc = 0; kc < kchunks; ++kc) {
+                tma_load_2d(sB + kc * half_nt * KC, &tmap_q, bfull, kc * KC,
+                            qt * p.plan.nt_pad + (int)rank * half_nt);
                 for (int h = 0; h < sf_tiles; ++h)
-                    tma_load_2d(sSF + (h * p.kchunks + kc) * APS * 512, &tmap_q_sf, bfull, 0,
+                    tma_load_2d(sSF + (h * kchunks + kc) * APS * 512, &tmap_q_sf, bfull, 0,
                                 (qt * sf_tiles + h) * p.atoms + kc * APS);
             }
+            // The ring holds the queries' scales until they are in TMEM.
+            bool ok = mbar_wait(qsf_done, 0, p.status, abort_flag, p.wait_ns);
             int stage = 0;
             uint32_t phase = 0, issued = 0, parity = 0;  // bits by stage
-            bool ok = true;
-            for (int j = first; j < p.n_tiles && ok; j += lanes_of_work) {
-                const int tile = j * p.tile_step;
-                for (int kc = 0; kc < p.kchunks; ++kc) {
+            for (int j = first; j < p.n_tiles && ok; j += stride) {
+                const int half_tile = j * p.tile_step * 2 + (int)rank;
+                for (int kc = 0; kc < kchunks; ++kc) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, p.status, abort_flag, p.wait_ns)) {
                         ok = false;
                         break;
                     }
                     uint8_t* dst = ring + stage * STAGE;
                     mbar_arrive_expect_tx(&full[stage], STAGE);
-                    tma_load_2d(dst, &tmap_rows, &full[stage], kc * KC, tile * ROWS);
+                    tma_load_2d(dst, &tmap_rows, &full[stage], kc * KC, half_tile * HALF);
                     tma_load_2d(dst + A_BYTES, &tmap_row_sf, &full[stage], 0,
-                                tile * p.atoms + kc * APS);
+                                half_tile * p.atoms + kc * APS);
                     issued |= 1u << stage;
                     parity = (parity & ~(1u << stage)) | (phase << stage);
-                    if (++stage == p.stages) {
+                    if (++stage == stages) {
                         stage = 0;
                         phase ^= 1u;
                     }
@@ -266,47 +450,34 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             // Every copy this thread issued lands before the CTA may exit.
             mbar_wait(bfull, 0, p.status, nullptr, p.wait_ns);
-            for (int s = 0; s < p.stages; ++s)
+            for (int s = 0; s < stages; ++s)
                 if ((issued >> s) & 1u)
                     mbar_wait(&full[s], (parity >> s) & 1u, p.status, nullptr, p.wait_ns);
-        }
-    } else if (warp == 1) {
-        // ------------------------------------------------------- MMA issuer
-        if (lane == 0) {
+        } else if (warp == 5 && lane == 0 && rank == 0) {
+            // --------------------------------------------------- MMA issuer
             const uint32_t idesc = make_idesc_fp4<FMT>(ROWS, nt);
-            const uint32_t sf_set = APS * 4 * (1 + sf_tiles);
-            const uint32_t sf_base = tmem_base + 2 * nt;
-            int stage = 0;
-            uint32_t phase = 0;
-            uint32_t it = 0;
-            bool ok = mbar_wait(bfull, 0, p.status, abort_flag, p.wait_ns);
-            int n = 0;
-            for (int j = first; j < p.n_tiles && ok; j += lanes_of_work, ++n) {
-                const int buf = n & 1;
-                if (!mbar_wait(&tempty[buf], ((n >> 1) & 1) ^ 1, p.status, abort_flag, p.wait_ns))
+            int stage = 0, set = 0, buf = 0;
+            uint32_t set_phase = 0, buf_phase = 0;
+            bool ok = true;
+            for (int j = first; j < p.n_tiles && ok; j += stride) {
+                if (!mbar_wait_cluster(&tempty[buf], buf_phase ^ 1u, p.status, abort_flag,
+                                       p.wait_ns))
                     break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(buf * nt);
-                for (int kc = 0; kc < p.kchunks; ++kc, ++it) {
-                    const uint32_t set = it & 1u;
-                    if (!mbar_wait(&full[stage], phase, p.status, abort_flag, p.wait_ns) ||
-                        !mbar_wait(&sfree[set], ((it >> 1) & 1u) ^ 1u, p.status, abort_flag,
-                                   p.wait_ns)) {
+                for (int kc = 0; kc < kchunks; ++kc) {
+                    if (!mbar_wait_cluster(&sready[set], set_phase, p.status, abort_flag,
+                                           p.wait_ns)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t a0 = smem_u32(ring + stage * STAGE);
-                    const uint32_t b0 = smem_u32(sB + kc * nt * KC);
-                    const uint32_t sfa = sf_base + set * sf_set, sfb = sfa + APS * 4;
-#pragma unroll
-                    for (int a = 0; a < APS; ++a) {
-                        tc_cp_scales(sfa + a * 4, make_scale_desc(a0 + A_BYTES + a * 512));
-                        for (int h = 0; h < sf_tiles; ++h)
-                            tc_cp_scales(sfb + (a * sf_tiles + h) * 4,
-                                         make_scale_desc(smem_u32(
-                                             sSF + ((h * p.kchunks + kc) * APS + a) * 512)));
-                    }
+                    const uint32_t b0 = smem_u32(sB + kc * (nt / 2) * KC);
+                    const uint32_t sfa = tmem_base + col_sets + set * set_cols;
+                    const uint32_t sfb = resident
+                                             ? tmem_base + col_sfb + kc * APS * sf_tiles * 4
+                                             : sfa + APS * 4;
                     const int steps = min(4, p.mmas - kc * 4);
                     for (int kk = 0; kk < steps; ++kk) {
                         // MX: an atom's bytes 0-1 scale one 64-element step, 2-3 the next
@@ -317,145 +488,134 @@ __global__ void __launch_bounds__(THREADS, 1)
                                      idesc | (id << 4) | (id << 29), sfa + a * 4,
                                      sfb + a * sf_tiles * 4, (kc | kk) != 0 ? 1u : 0u);
                     }
-                    tc_commit(&empty[stage]);
-                    tc_commit(&sfree[set]);
-                    if (++stage == p.stages) {
-                        stage = 0;
-                        phase ^= 1u;
+                    tc_commit_pair(&empty[stage]);
+                    tc_commit_pair(&sfree[set]);
+                    if (++stage == stages) stage = 0;
+                    if (++set == sets) {
+                        set = 0;
+                        set_phase ^= 1u;
                     }
                 }
                 if (!ok) break;
-                tc_commit(&tfull[buf]);
+                tc_commit_pair(&tfull[buf]);
+                if (++buf == bufs) {
+                    buf = 0;
+                    buf_phase ^= 1u;
+                }
             }
             // All MMAs issued above complete before TMEM is released.
-            tc_commit(drain);
+            tc_commit_pair(drain);
             mbar_wait(drain, 0, p.status, nullptr, p.wait_ns);
         }
+        __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_EPI));
         // ---------------------------------------------------------- epilogue
         const int quarter = warp & 3;
-        const int half = (warp - 2) >> 2;
-        const int chunks = (nt + 31) / 32;
-        int n = 0;
-        for (int j = first; j < p.n_tiles; j += lanes_of_work, ++n) {
-            const int buf = n & 1;
-            const int in_tile = quarter * 32 + lane;
+        const int half = (warp - 8) >> 2;
+        const int chunks = (nt + 31) / 32;     // of 32 columns; this warp takes every other one
+        const int in_tile = (int)rank * HALF + quarter * 32 + lane;
+        int buf = 0;
+        uint32_t buf_phase = 0;
+        for (int j = first; j < p.n_tiles; j += stride) {
             const int64_t row = (int64_t)j * p.tile_step * ROWS + in_tile;
             const bool row_in = row < p.n_rows;
             const float g = row_in ? __ldg(&p.row_scale[row]) : __int_as_float(0x7fc00000);
-            const bool got = mbar_wait(&tfull[buf], (n >> 1) & 1, p.status, abort_flag, p.wait_ns);
+            const bool got = mbar_wait(&tfull[buf], buf_phase, p.status, abort_flag, p.wait_ns);
             if (!__all_sync(0xffffffffu, got)) break;
             tc_fence_after();
             const uint32_t taddr =
                 tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * nt);
-            for (int c = half; c < chunks; c += 2) {
-                uint32_t r[32];
-                __syncwarp();
-                tmem_ld32(taddr + c * 32, r);
-                tmem_ld_wait_regs(r);
-                const int t0 = qt * nt + c * 32;
-                const int cols = min(32, min(nt - c * 32, p.nq - t0));
-                if (mode == kScores) {
-                    if (row_in && cols > 0) {
-                        const int64_t col = (int64_t)j * ROWS + in_tile;
-                        if (p.out_type == PION_B200_F32)
-                            store_chunk<float>(r, p, t0, cols, col, s_gq + c * 32, g);
-                        else if (p.out_type == PION_B200_BF16)
-                            store_chunk<__nv_bfloat16>(r, p, t0, cols, col, s_gq + c * 32, g);
-                        else
-                            store_chunk<__half>(r, p, t0, cols, col, s_gq + c * 32, g);
-                    }
-                } else {
-                    const float* th = s_th + c * 32;
-                    bool any = false;
+            uint32_t r[4][32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) any |= __uint_as_float(r[i]) * g >= th[i];
-                    if (any) {
+            for (int c = 0; c < 4; ++c)
+                if (2 * c + half < chunks) tmem_ld32(taddr + (2 * c + half) * 32, r[c]);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float v = __uint_as_float(r[i]) * g;
-                            if (v >= th[i]) {
-                                const int t = t0 + i;
-                                const int at = atomicAdd(&p.cand_n[t], 1);
-                                if (at < CAP)
-                                    p.cand[(int64_t)t * CAP + at] =
-                                        ((uint64_t)__float_as_uint(v * s_gq[c * 32 + i]) << 32) |
-                                        (uint32_t)row;
-                            }
-                        }
-                    }
-                }
-            }
+            for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(r[c]);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty[buf]);
+            if (lane == 0) mbar_arrive_leader(&tempty[buf]);
+            const int64_t col = (int64_t)j * ROWS + in_tile;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int at = (2 * c + half) * 32;
+                if (2 * c + half < chunks) {
+                    const int t0 = qt * nt + at;
+                    epilogue_chunk(r[c], p, mode, t0, min(32, min(nt - at, p.nq - t0)), row_in, row,
+                                   col, s_gq + at, s_th + at, g);
+                }
+            }
+            if (++buf == bufs) {
+                buf = 0;
+                buf_phase ^= 1u;
+            }
         }
     }
     tc_fence_before();
-    __syncthreads();
-    if (warp == 1) {
+    cluster_sync();
+    if (warp == 5) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, TMEM_COLS);
+        tmem_dealloc_pair(tmem_base, TMEM_COLS);
     }
 }
 
 // --------------------------------------------------------------- selection --
 constexpr int SEL = 256;  // threads of a selection CTA
-
-// The k-th largest (1-based) of m ordered values, by the CTA: four passes over byte
-// histograms.  `value(i)` is called once per pass for every i.
-template <class F>
-__device__ uint32_t kth_largest(int m, int k, int* hist, F value) {
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_left;
-    uint32_t prefix = 0;
-    int left = k;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int b = threadIdx.x; b < 256; b += SEL) hist[b] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < m; i += SEL) {
-            const uint32_t o = value(i);
-            if (shift == 24 || (o >> (shift + 8)) == (prefix >> (shift + 8)))
-                atomicAdd(&hist[(o >> shift) & 255u], 1);
-        }
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            // warp 0: lane L owns the eight bins 255 - 8 L and below
-            const int lane = threadIdx.x;
-            int c[8], sum = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                c[j] = hist[255 - 8 * lane - j];
-                sum += c[j];
-            }
-            int before = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, before, o);
-                if (lane >= o) before += up;
-            }
-            before -= sum;
-            if (before < left && before + sum >= left) {
-                int b = before;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (b < left && b + c[j] >= left) {
-                        s_prefix = prefix | ((uint32_t)(255 - 8 * lane - j) << shift);
-                        s_left = left - b;
-                    }
-                    b += c[j];
-                }
-            }
-        }
-        __syncthreads();
-        prefix = s_prefix;
-        left = s_left;
-        __syncthreads();
-    }
-    return prefix;
-}
+static_assert(SEL >= 256, "a thread maximum for each of up to 256 results");
 
 __device__ __forceinline__ uint32_t ordered_score(float v) { return v == v ? ordered(v) : 0u; }
+
+// Sorts n <= LIST keys in shared memory, largest first (bitonic over the next power of two;
+// the rest is filled with zeros).
+__device__ void sort_desc(uint64_t* key, int n) {
+    int size = 2;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += SEL) key[i] = 0;
+    __syncthreads();
+    for (int w = 2; w <= size; w <<= 1)
+        for (int s = w >> 1; s; s >>= 1) {
+            for (int i = threadIdx.x; i < size / 2; i += SEL) {
+                const int a = 2 * i - (i & (s - 1));
+                const int b = a + s;
+                const bool desc = (a & w) == 0;
+                const uint64_t x = key[a], y = key[b];
+                if ((x < y) == desc) {
+                    key[a] = y;
+                    key[b] = x;
+                }
+            }
+            __syncthreads();
+        }
+}
+
+// The k-th largest (1-based, k <= SEL, k <= m) of m ordered values, by the CTA, or where more
+// than LIST values reach it a lower bound of it.  The k-th largest of the threads' own
+// maxima is a lower bound that few values reach; those are sorted.  `key` holds LIST keys of
+// scratch, `count` one integer.
+template <class F>
+__device__ uint32_t kth_largest(int m, int k, uint64_t* key, int* count, F value) {
+    uint32_t top = 0;
+    for (int i = threadIdx.x; i < m; i += SEL) top = max(top, value(i));
+    key[threadIdx.x] = (uint64_t)top;
+    sort_desc(key, SEL);
+    const uint64_t low = key[k - 1];
+    if (m <= SEL) return (uint32_t)low;  // a value each
+    __syncthreads();
+    if (threadIdx.x == 0) *count = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < m; i += SEL) {
+        const uint32_t o = value(i);
+        if (o >= low) {
+            const int at = atomicAdd(count, 1);
+            if (at < LIST) key[at] = o;
+        }
+    }
+    __syncthreads();
+    const int n = *count;
+    if (n > LIST) return (uint32_t)low;
+    sort_desc(key, n);
+    return (uint32_t)key[k - 1];
+}
 
 // Infinite where a float32 sum could overflow: nothing is known of an approximate score then.
 // The last term covers products below the least normal float.
@@ -471,7 +631,8 @@ __global__ void __launch_bounds__(SEL)
     theta_kernel(const float* sample, int64_t ld, int m, const uint64_t* cand, int k,
                  int dp, const float* q_scale, int nt, int nt_pad, const float* q_norm,
                  const float* norm_max, float* theta, int* cand_n) {
-    __shared__ int hist[256];
+    __shared__ uint64_t key[LIST];
+    __shared__ int count;
     const int t = blockIdx.x;
     const float* s = sample + (int64_t)t * ld;
     const uint64_t* c = cand + (int64_t)t * CAP;
@@ -482,7 +643,7 @@ __global__ void __launch_bounds__(SEL)
         th = -INFINITY;
         if (cand && m < k) th = theta[t];
         if (m >= k) {
-            const uint32_t o = kth_largest(m, k, hist, [&](int i) {
+            const uint32_t o = kth_largest(m, k, key, &count, [&](int i) {
                 return ordered_score(cand ? __uint_as_float((uint32_t)(c[i] >> 32)) : s[i]);
             });
             const float kth = o ? unordered(o) : -INFINITY;
@@ -569,34 +730,11 @@ __device__ __forceinline__ uint64_t row_key(double dot, float g, float gq, int64
     return ((uint64_t)ordered(s) << 32) | (uint32_t)~(uint32_t)row;
 }
 
-// Sorts n <= LIST keys in shared memory, largest first (bitonic over the next power of two;
-// the rest is filled with zeros).
-__device__ void sort_desc(uint64_t* key, int n) {
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += SEL) key[i] = 0;
-    __syncthreads();
-    for (int w = 2; w <= size; w <<= 1)
-        for (int s = w >> 1; s; s >>= 1) {
-            for (int i = threadIdx.x; i < size / 2; i += SEL) {
-                const int a = 2 * i - (i & (s - 1));
-                const int b = a + s;
-                const bool desc = (a & w) == 0;
-                const uint64_t x = key[a], y = key[b];
-                if ((x < y) == desc) {
-                    key[a] = y;
-                    key[b] = x;
-                }
-            }
-            __syncthreads();
-        }
-}
-
 // The k best rows of one query per CTA.
 template <int FMT>
 __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
     __shared__ __align__(16) uint64_t key[LIST];
-    __shared__ int hist[256];
+    __shared__ int s_warp[SEL / 32];
     __shared__ int s_n;
     extern __shared__ __align__(16) uint8_t dyn[];  // query bytes [dp], scales [dp / block]
     const int t = blockIdx.x;
@@ -630,9 +768,12 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
             float cut = -INFINITY;
             if (m > p.k) {
                 const uint32_t o =
-                    kth_largest(m, p.k, hist, [&](int i) { return ordered_score(approx(i)); });
+                    kth_largest(m, p.k, key, &s_n, [&](int i) { return ordered_score(approx(i)); });
                 cut = o ? unordered(o) - two_eps : -INFINITY;
             }
+            __syncthreads();
+            if (threadIdx.x == 0) s_n = 0;
+            __syncthreads();
             for (int i = threadIdx.x; i < m; i += SEL) {
                 const float a = approx(i);
                 if (a >= cut || !known) {
@@ -691,13 +832,13 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
             const int64_t row = r0 + threadIdx.x;
             const float g = row < p.n_rows ? p.row_scale[row] : __int_as_float(0x7fc00000);
             const unsigned live = __ballot_sync(0xffffffffu, g == g);
-            if (lane == 0) hist[warp] = __popc(live);
+            if (lane == 0) s_warp[warp] = __popc(live);
             __syncthreads();
             int at = found;
             int all = 0;
             for (int w = 0; w < W; ++w) {
-                if (w < warp) at += hist[w];
-                all += hist[w];
+                if (w < warp) at += s_warp[w];
+                all += s_warp[w];
             }
             at += __popc(live & ((1u << lane) - 1u));
             if (g == g && at < p.k) key[at] = ((uint64_t)ordered(0.0f) << 32) | (uint32_t)~(uint32_t)row;
@@ -716,35 +857,58 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
 
 static int round_up(int x, int a) { return (x + a - 1) / a * a; }
 
-// Queries per tile: as many as the accumulators' two buffers and two sets of scale columns
-// leave of the 512 TMEM columns, and shared memory beside at least three stages; spread
-// evenly over the tiles.
-static bool make_plan(int fmt, int dp, int nq, Plan* out) {
-    const int aps = atoms_per_stage(fmt);
-    Plan s;
-    s.kchunks = (dp / 2 + KC - 1) / KC;
-    s.stage_bytes = A_BYTES + aps * 512;
-    const int fixed = 1024 + 2 * 256 * 4 + (2 * MAX_STAGES + 8) * 8 + 64;
-    int most = 0;
-    for (int nt = 16; nt <= 208; nt += 16) {
-        const int pad = round_up(nt, 128);
-        const int cols = 2 * nt + 2 * aps * 4 * (1 + pad / 128);
-        const int bytes = fixed + s.kchunks * (nt * KC + pad / 128 * aps * 512) + 3 * s.stage_bytes;
-        // 16 columns past an odd number of 16s are read with the last chunk
-        if (cols <= (int)TMEM_COLS && bytes <= SMEM_MAX) most = nt;
+// Queries per tile.  A pair's time for a tile of rows is, per 64 elements, nt / 2 cycles of
+// the tensor cores or, where that is more, the bytes that pass through each CTA's shared
+// memory at 128 a cycle: operands, the stage's copy, and the scale warps' reads; about 450
+// cycles more where one accumulator buffer has to be drained before the next tile.  Taken is
+// the nt whose query tiles, spread over the pairs, take the least.
+static bool make_plan(int fmt, int dp, int nq, int64_t n_tiles, Plan* out) {
+    const int aps = atoms_per_stage(fmt), steps = dp / 64;
+    const int kchunks = (dp / 2 + KC - 1) / KC;
+    const int stage = A_BYTES + aps * 512;
+    const int fixed = 1024 + 2 * MAX_NT * 4 + (4 * MAX_STAGES + 8) * 8 + 64;
+    constexpr int64_t pairs = 74;  // of the B200's 148 SMs
+    double best = 0.0;
+    bool any = false;
+    for (int nt = 16; nt <= MAX_NT; nt += 16) {
+        Plan s;
+        s.nt = nt;
+        s.nt_pad = round_up(nt, 128);
+        s.kchunks = kchunks;
+        s.n_qt = (nq + nt - 1) / nt;
+        const int sf_tiles = s.nt_pad / 128, set = aps * 4;
+        // an odd number of 16 columns is read with 16 more
+        const int cols = (int)TMEM_COLS - (nt % 32 ? 16 : 0);
+        const int sfb = kchunks * aps * 4 * sf_tiles;
+        s.resident = nt + sfb + 2 * set <= cols;
+        const int set_cols = s.resident ? set : set * (1 + sf_tiles);
+        const int left = cols - (s.resident ? sfb : 0);
+        if (nt + 2 * set_cols > left) continue;
+        s.bufs = 2 * nt + 2 * set_cols <= left ? 2 : 1;
+        const int held = kchunks * (nt / 2) * KC;
+        const int streamed = s.resident ? 0 : sf_tiles * kchunks * aps * 512;
+        s.stages = (SMEM_MAX - fixed - held - streamed) / stage;
+        // the queries' scales pass through the ring
+        if (s.stages < 3 || (s.resident && s.stages * stage < sf_tiles * kchunks * aps * 512)) continue;
+        if (s.stages > MAX_STAGES) s.stages = MAX_STAGES;
+        s.sets = (left - s.bufs * nt) / set_cols;
+        if (s.sets > s.stages) s.sets = s.stages;
+        s.smem = fixed + held + streamed + s.stages * stage;
+        const double bytes = HALF * 32 + nt / 2 * 32 + stage / 4.0 + 4.0 * aps * 512 / 4 +
+                             (s.resident ? 0.0 : 4.0 * aps * sf_tiles * 512 / 4);
+        const double tensor = nt / 2.0;
+        const double cycles = steps * (tensor > bytes / 128 ? tensor : bytes / 128) +
+                              (s.bufs == 1 ? 450.0 : 0.0);
+        const int64_t per = pairs / s.n_qt > 0 ? pairs / s.n_qt : 1;
+        const int64_t waves = (s.n_qt * per + pairs - 1) / pairs;
+        const double time = cycles * (double)((n_tiles + per - 1) / per) * (double)waves;
+        if (!any || time < best * 0.999) {
+            best = time;
+            *out = s;
+            any = true;
+        }
     }
-    if (most == 0) return false;
-    s.n_qt = (nq + most - 1) / most;
-    s.nt = round_up((nq + s.n_qt - 1) / s.n_qt, 16);
-    s.n_qt = (nq + s.nt - 1) / s.nt;
-    s.nt_pad = round_up(s.nt, 128);
-    s.b_bytes = s.kchunks * s.nt * KC;
-    s.sfb_bytes = s.kchunks * (s.nt_pad / 128) * aps * 512;
-    s.stages = (SMEM_MAX - fixed - s.b_bytes - s.sfb_bytes) / s.stage_bytes;
-    s.stages = s.stages > MAX_STAGES ? MAX_STAGES : s.stages;
-    s.smem = fixed + s.b_bytes + s.sfb_bytes + s.stages * s.stage_bytes;
-    *out = s;
-    return true;
+    return any;
 }
 
 }  // namespace fp4
@@ -753,9 +917,9 @@ int fp4_max_dim() { return fp4::kMaxDim; }
 int fp4_cap() { return fp4::CAP; }
 int fp4_tile_rows() { return fp4::ROWS; }
 
-bool fp4_plan(int format, int dp, int nq, Fp4Plan* out) {
+bool fp4_plan(int format, int dp, int nq, int64_t n_rows, Fp4Plan* out) {
     fp4::Plan s;
-    if (!fp4::make_plan(format, dp, nq, &s)) return false;
+    if (!fp4::make_plan(format, dp, nq, (n_rows + fp4::ROWS - 1) / fp4::ROWS, &s)) return false;
     out->nt = s.nt;
     out->nt_pad = s.nt_pad;
     out->n_qt = s.n_qt;
@@ -766,19 +930,21 @@ int launch_fp4_product(const Fp4Product& L, cudaStream_t st) {
     using namespace fp4;
     Plan s;
     const int dp = pad_dim(L.dim);
-    if (!make_plan(L.format, dp, L.nq, &s)) return PION_B200_ESHAPE;
-    const int atoms = atoms_of(L.format, dp), aps = atoms_per_stage(L.format);
     const int64_t row_tiles = (L.n_rows + ROWS - 1) / ROWS;
+    // the plan of the whole call, whatever part of the rows this launch takes: the queries
+    // are laid out for it
+    if (!make_plan(L.format, dp, L.nq, row_tiles, &s)) return PION_B200_ESHAPE;
+    const int atoms = atoms_of(L.format, dp), aps = atoms_per_stage(L.format);
     const int64_t store_tiles = (L.store_rows + 127) / 128;
     CUtensorMap rows, row_sf, q, q_sf;
     if (make_tmap_2d(&rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, L.codes, (uint64_t)dp / 2,
-                     (uint64_t)L.store_rows, (uint64_t)dp / 2, KC, ROWS,
+                     (uint64_t)L.store_rows, (uint64_t)dp / 2, KC, HALF,
                      CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
         make_tmap_2d(&row_sf, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, L.scales, 128,
                      (uint64_t)store_tiles * atoms, 512, 128, (uint32_t)aps,
                      CU_TENSOR_MAP_SWIZZLE_NONE) != 0 ||
         make_tmap_2d(&q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, L.q_codes, (uint64_t)dp / 2,
-                     (uint64_t)s.n_qt * s.nt_pad, (uint64_t)dp / 2, KC, (uint32_t)s.nt,
+                     (uint64_t)s.n_qt * s.nt_pad, (uint64_t)dp / 2, KC, (uint32_t)s.nt / 2,
                      CU_TENSOR_MAP_SWIZZLE_128B) != 0 ||
         make_tmap_2d(&q_sf, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, L.q_scales, 128,
                      (uint64_t)s.n_qt * (s.nt_pad / 128) * atoms, 512, 128, (uint32_t)aps,
@@ -789,13 +955,9 @@ int launch_fp4_product(const Fp4Product& L, cudaStream_t st) {
     p.q_scale = L.q_scale;
     p.n_rows = L.n_rows;
     p.nq = L.nq;
-    p.nt = s.nt;
-    p.nt_pad = s.nt_pad;
-    p.n_qt = s.n_qt;
-    p.kchunks = s.kchunks;
+    p.plan = s;
     p.mmas = dp / 64;
     p.atoms = atoms;
-    p.stages = s.stages;
     p.n_tiles = L.n_tiles > 0 ? L.n_tiles : (int)row_tiles;
     p.tile_step = L.tile_step;
     p.out = L.out;
@@ -806,10 +968,12 @@ int launch_fp4_product(const Fp4Product& L, cudaStream_t st) {
     p.cand = L.cand;
     p.status = L.status;
     p.wait_ns = L.wait_ns;
-    int64_t per = L.num_sms / s.n_qt;  // CTAs per query tile: one wave where there are enough SMs
+    // Pairs per query tile: one wave where there are enough SMs.  The query tiles of one row
+    // tile run beside each other, so that the rows come from HBM once.
+    int64_t per = L.num_sms / 2 / s.n_qt;
     if (per < 1) per = 1;
     if (per > p.n_tiles) per = p.n_tiles;
-    const dim3 grid((unsigned)(per * s.n_qt));
+    const dim3 grid((unsigned)(2 * per * s.n_qt));
     const int mode = L.theta ? kCollect : kScores;
     const bool mx = L.format == kMX;
     const void* fn = mx ? (const void*)fp4_tc_kernel<kMX> : (const void*)fp4_tc_kernel<kNV>;

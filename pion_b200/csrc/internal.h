@@ -507,7 +507,7 @@ struct Fp4Plan {
 int fp4_max_dim();
 int fp4_cap();
 int fp4_tile_rows();
-bool fp4_plan(int format, int dp, int nq, Fp4Plan* out);
+bool fp4_plan(int format, int dp, int nq, int64_t n_rows, Fp4Plan* out);
 struct Fp4Product {
     int format = 0;
     int dim = 0;
