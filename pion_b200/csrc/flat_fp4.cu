@@ -39,13 +39,14 @@ constexpr int A_BYTES = HALF * KC;       // 16 KB
 constexpr int EPI_WARPS = 8;
 constexpr int SCALE_WARPS = 4;
 constexpr int THREADS = 512;             // 128 registers a thread at launch ...
-constexpr int REGS_SCALE = 88, REGS_ISSUE = 40, REGS_EPI = 192;  // ... and 4 * 128 in all here
+constexpr int REGS_SCALE = 64, REGS_ISSUE = 64, REGS_EPI = 192;  // ... and 4 * 128 in all here
 static_assert(REGS_SCALE + REGS_ISSUE + 2 * REGS_EPI <= 4 * 128, "register split");
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int MAX_STAGES = 8;
 constexpr int MAX_NT = 256;
 constexpr int SMEM_MAX = 232448;         // 227 KB
 constexpr int CAP = 4096;                // candidates kept per query
+constexpr int HITS = 64;                 // appended candidates an epilogue warp holds back
 constexpr int LIST = 2048;               // of which at most this many are scored exactly
 
 // 512-byte scale atoms per stage of 256 elements
@@ -103,42 +104,15 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
                  "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrives on the first CTA's copy of a barrier.
+// Arrives on the first CTA's copy of a barrier.  Relaxed: what the arrival stands for (TMEM
+// stores that were waited for, copies that completed on an mbarrier, TMEM loads) is no memory
+// access of this thread, and a release at cluster scope costs a fence per arrival.
 __device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
     asm volatile(
         "{\n\t.reg .b32 remote;\n\tmapa.shared::cluster.u32 remote, %0, 0;\n\t"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n\t}\n" ::"r"(
+        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [remote];\n\t}\n" ::"r"(
             smem_u32(bar))
         : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// mbar_wait for phases that the other CTA's threads arrive on.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int* status,
-                                                  volatile int* abort_flag, uint64_t budget_ns) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    uint32_t spins = 0;
-    for (;;) {
-        if (mbar_try_wait_cluster(bar, parity)) return true;
-        if ((++spins & 63u) == 0) {
-            if (*abort_flag) return false;
-            if (globaltimer_ns() - t0 > budget_ns) {
-                record_error(status, PION_B200_ETIMEOUT);
-                *abort_flag = 1;
-                return false;
-            }
-        }
-    }
 }
 
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_slot, uint32_t ncols) {
@@ -232,38 +206,64 @@ __device__ __forceinline__ void store_chunk(const uint32_t (&r)[32], const TcPar
     }
 }
 
-// One chunk of one row's scores: written, or the row appended to the lists of the queries
-// whose threshold it reaches.
-__device__ __forceinline__ void epilogue_chunk(const uint32_t (&r)[32], const TcParams& p, int mode,
-                                               int t0, int cols, bool row_in, int64_t row,
-                                               int64_t col, const float* gq, const float* th,
-                                               float g) {
-    if (mode == kScores) {
-        if (row_in && cols > 0) {
-            if (p.out_type == PION_B200_F32)
-                store_chunk<float>(r, p, t0, cols, col, gq, g);
-            else if (p.out_type == PION_B200_BF16)
-                store_chunk<__nv_bfloat16>(r, p, t0, cols, col, gq, g);
-            else
-                store_chunk<__half>(r, p, t0, cols, col, gq, g);
-        }
-    } else {
-        bool any = false;
+// Candidates that an epilogue warp has found and not yet appended: an append waits for its
+// place in the query's list about as long as the MMAs of a third of a tile take, so they are
+// made for up to 64 candidates at once.
+struct Hits {
+    uint64_t* entry;  // [HITS] score bits << 32 | row
+    uint8_t* col;     // [HITS] query's column
+    int n;            // warp-uniform
+};
+
+__device__ __forceinline__ void append_hits(Hits& h, const TcParams& p, int qt_first, int lane) {
+    __syncwarp();
+    for (int i = lane; i < h.n; i += 32) {
+        const int t = qt_first + h.col[i];
+        const int at = atomicAdd(&p.cand_n[t], 1);
+        if (at < CAP) p.cand[(int64_t)t * CAP + at] = h.entry[i];
+    }
+    __syncwarp();
+    h.n = 0;
+}
+
+// r[i] for a warp-uniform i, without an indexed access that would move r to local memory.
+__device__ __forceinline__ float pick(const uint32_t (&r)[32], int i) {
+    uint32_t t[16];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) any |= __uint_as_float(r[i]) * g >= th[i];
-        if (any) {
+    for (int j = 0; j < 16; ++j) t[j] = selp_u32(r[2 * j + 1], r[2 * j], i & 1);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float v = __uint_as_float(r[i]) * g;
-                if (v >= th[i]) {
-                    const int t = t0 + i;
-                    const int at = atomicAdd(&p.cand_n[t], 1);
-                    if (at < CAP)
-                        p.cand[(int64_t)t * CAP + at] =
-                            ((uint64_t)__float_as_uint(v * gq[i]) << 32) | (uint32_t)row;
-                }
-            }
+    for (int w = 8, b = 1; w >= 1; w /= 2, ++b)
+#pragma unroll
+        for (int j = 0; j < w; ++j) t[j] = selp_u32(t[2 * j + 1], t[2 * j], (i >> b) & 1);
+    return __uint_as_float(t[0]);
+}
+
+// One chunk of 32 columns of 32 rows, for the queries from column `at`: the rows that reach a
+// query's threshold are kept.  Most chunks have none.
+__device__ __forceinline__ void collect_chunk(const uint32_t (&r)[32], const TcParams& p, Hits& h,
+                                              int qt_first, int at, int64_t row, const float* gq,
+                                              const float* th, float g, int lane) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) any |= __uint_as_float(r[i]) * g >= th[at + i];
+    if (!__any_sync(0xffffffffu, any)) return;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) mine |= (__uint_as_float(r[i]) * g >= th[at + i] ? 1u : 0u) << i;
+    uint32_t columns = __reduce_or_sync(0xffffffffu, mine);
+    while (columns) {
+        const int i = __ffs(columns) - 1;
+        columns &= columns - 1;
+        const float v = pick(r, i) * g;
+        const bool hit = (mine >> i) & 1u;
+        const unsigned m = __ballot_sync(0xffffffffu, hit);
+        if (h.n > HITS - 32) append_hits(h, p, qt_first, lane);
+        if (hit) {
+            const int slot = h.n + __popc(m & ((1u << lane) - 1u));
+            h.entry[slot] = ((uint64_t)__float_as_uint(v * gq[at + i]) << 32) | (uint32_t)row;
+            h.col[slot] = (uint8_t)(at + i);
         }
+        h.n += __popc(m);
     }
 }
 
@@ -297,7 +297,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint8_t* after = sB + kchunks * (nt / 2) * KC + (resident ? 0 : sf_tiles * kchunks * APS * 512);
     float* s_gq = reinterpret_cast<float*>(after);
     float* s_th = s_gq + MAX_NT;
-    uint64_t* full = reinterpret_cast<uint64_t*>(s_th + MAX_NT);
+    uint64_t* s_hits = reinterpret_cast<uint64_t*>(s_th + MAX_NT);
+    uint8_t* s_hit_col = reinterpret_cast<uint8_t*>(s_hits + EPI_WARPS * HITS);
+    uint64_t* full = reinterpret_cast<uint64_t*>(s_hit_col + EPI_WARPS * HITS);
     uint64_t* empty = full + MAX_STAGES;
     uint64_t* sready = empty + MAX_STAGES;   // per set, on the first CTA: both CTAs' stage is in
     uint64_t* sfree = sready + MAX_STAGES;
@@ -460,13 +462,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             uint32_t set_phase = 0, buf_phase = 0;
             bool ok = true;
             for (int j = first; j < p.n_tiles && ok; j += stride) {
-                if (!mbar_wait_cluster(&tempty[buf], buf_phase ^ 1u, p.status, abort_flag,
+                if (!mbar_wait(&tempty[buf], buf_phase ^ 1u, p.status, abort_flag,
                                        p.wait_ns))
                     break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(buf * nt);
                 for (int kc = 0; kc < kchunks; ++kc) {
-                    if (!mbar_wait_cluster(&sready[set], set_phase, p.status, abort_flag,
+                    if (!mbar_wait(&sready[set], set_phase, p.status, abort_flag,
                                            p.wait_ns)) {
                         ok = false;
                         break;
@@ -515,6 +517,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int half = (warp - 8) >> 2;
         const int chunks = (nt + 31) / 32;     // of 32 columns; this warp takes every other one
         const int in_tile = (int)rank * HALF + quarter * 32 + lane;
+        Hits hits = {s_hits + (warp - 8) * HITS, s_hit_col + (warp - 8) * HITS, 0};
         int buf = 0;
         uint32_t buf_phase = 0;
         for (int j = first; j < p.n_tiles; j += stride) {
@@ -539,17 +542,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int at = (2 * c + half) * 32;
-                if (2 * c + half < chunks) {
-                    const int t0 = qt * nt + at;
-                    epilogue_chunk(r[c], p, mode, t0, min(32, min(nt - at, p.nq - t0)), row_in, row,
-                                   col, s_gq + at, s_th + at, g);
+                if (2 * c + half >= chunks) break;
+                if (mode == kCollect) {
+                    collect_chunk(r[c], p, hits, qt * nt, at, row, s_gq, s_th, g, lane);
+                    continue;
                 }
+                const int t0 = qt * nt + at;
+                const int n = min(32, min(nt - at, p.nq - t0));
+                if (!row_in || n <= 0) continue;
+                if (p.out_type == PION_B200_F32)
+                    store_chunk<float>(r[c], p, t0, n, col, s_gq + at, g);
+                else if (p.out_type == PION_B200_BF16)
+                    store_chunk<__nv_bfloat16>(r[c], p, t0, n, col, s_gq + at, g);
+                else
+                    store_chunk<__half>(r[c], p, t0, n, col, s_gq + at, g);
             }
             if (++buf == bufs) {
                 buf = 0;
                 buf_phase ^= 1u;
             }
         }
+        if (mode == kCollect) append_hits(hits, p, qt * nt, lane);
     }
     tc_fence_before();
     cluster_sync();
@@ -560,21 +573,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 }
 
 // --------------------------------------------------------------- selection --
-constexpr int SEL = 256;  // threads of a selection CTA
-static_assert(SEL >= 256, "a thread maximum for each of up to 256 results");
+constexpr int THETA = 1024;  // threads of a threshold CTA
+constexpr int SEL = 512;     // threads of a finishing CTA
+constexpr int MAX_K = 256;
 
 __device__ __forceinline__ uint32_t ordered_score(float v) { return v == v ? ordered(v) : 0u; }
 
-// Sorts n <= LIST keys in shared memory, largest first (bitonic over the next power of two;
-// the rest is filled with zeros).
+// Rank of key[i] among key[0:n], largest first, equal ones by index (n rounded up to a multiple
+// of 2 must be readable; key 16-byte aligned).
+__device__ __forceinline__ int rank_of(const uint64_t* key, int n, int i) {
+    const uint64_t x = key[i];
+    int rank = 0;
+    for (int j = 0; j < n; j += 2) {
+        const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(key + j);
+        rank += y.x > x || (y.x == x && j < i);
+        if (j + 1 < n) rank += y.y > x || (y.y == x && j + 1 < i);
+    }
+    return rank;
+}
+
+// Sorts n <= LIST keys in shared memory, largest first: few by their ranks, more by a bitonic
+// sort over the next power of two (the rest is filled with zeros).
+template <int NT>
 __device__ void sort_desc(uint64_t* key, int n) {
+    if (n <= NT) {
+        __syncthreads();
+        int at = 0;
+        uint64_t x = 0;
+        if ((int)threadIdx.x < n) {
+            x = key[threadIdx.x];
+            at = rank_of(key, n, threadIdx.x);
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < n) key[at] = x;
+        __syncthreads();
+        return;
+    }
     int size = 2;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += SEL) key[i] = 0;
+    for (int i = n + threadIdx.x; i < size; i += NT) key[i] = 0;
     __syncthreads();
     for (int w = 2; w <= size; w <<= 1)
         for (int s = w >> 1; s; s >>= 1) {
-            for (int i = threadIdx.x; i < size / 2; i += SEL) {
+            for (int i = threadIdx.x; i < size / 2; i += NT) {
                 const int a = 2 * i - (i & (s - 1));
                 const int b = a + s;
                 const bool desc = (a & w) == 0;
@@ -588,22 +629,28 @@ __device__ void sort_desc(uint64_t* key, int n) {
         }
 }
 
-// The k-th largest (1-based, k <= SEL, k <= m) of m ordered values, by the CTA, or where more
-// than LIST values reach it a lower bound of it.  The k-th largest of the threads' own
-// maxima is a lower bound that few values reach; those are sorted.  `key` holds LIST keys of
-// scratch, `count` one integer.
-template <class F>
+// The k-th largest (1-based, k <= MAX_K, k <= m) of m ordered values, by the CTA, or where more
+// than LIST values reach it a lower bound of it.  The k-th largest of the maxima of 256
+// groups of threads is a lower bound that few values reach; those are sorted.  `key` holds
+// LIST keys of scratch, `count` one integer.
+template <int NT, class F>
 __device__ uint32_t kth_largest(int m, int k, uint64_t* key, int* count, F value) {
+    constexpr int G = NT / MAX_K;  // threads per group, neighbours of one warp
     uint32_t top = 0;
-    for (int i = threadIdx.x; i < m; i += SEL) top = max(top, value(i));
-    key[threadIdx.x] = (uint64_t)top;
-    sort_desc(key, SEL);
-    const uint64_t low = key[k - 1];
-    if (m <= SEL) return (uint32_t)low;  // a value each
-    __syncthreads();
+#pragma unroll 8
+    for (int i = threadIdx.x; i < m; i += NT) top = max(top, value(i));
+#pragma unroll
+    for (int o = 1; o < G; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (threadIdx.x % G == 0) key[threadIdx.x / G] = top;
     if (threadIdx.x == 0) *count = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < m; i += SEL) {
+    __shared__ uint32_t s_low;
+    if (threadIdx.x < MAX_K && rank_of(key, MAX_K, threadIdx.x) == k - 1)
+        s_low = (uint32_t)key[threadIdx.x];
+    __syncthreads();
+    const uint32_t low = s_low;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < m; i += NT) {
         const uint32_t o = value(i);
         if (o >= low) {
             const int at = atomicAdd(count, 1);
@@ -612,8 +659,8 @@ __device__ uint32_t kth_largest(int m, int k, uint64_t* key, int* count, F value
     }
     __syncthreads();
     const int n = *count;
-    if (n > LIST) return (uint32_t)low;
-    sort_desc(key, n);
+    if (n > LIST) return low;
+    sort_desc<NT>(key, n);
     return (uint32_t)key[k - 1];
 }
 
@@ -627,11 +674,11 @@ __device__ __forceinline__ float eps_of(int dp, float q_norm, float norm_max) {
 // Threshold of one query per CTA: the k-th best of its approximate scores so far (the sample's,
 // or the candidates of a part of the rows) less 2 eps, in units of the query's g.  Resets the
 // query's candidate count.
-__global__ void __launch_bounds__(SEL)
+__global__ void __launch_bounds__(THETA)
     theta_kernel(const float* sample, int64_t ld, int m, const uint64_t* cand, int k,
                  int dp, const float* q_scale, int nt, int nt_pad, const float* q_norm,
                  const float* norm_max, float* theta, int* cand_n) {
-    __shared__ uint64_t key[LIST];
+    __shared__ __align__(16) uint64_t key[LIST];
     __shared__ int count;
     const int t = blockIdx.x;
     const float* s = sample + (int64_t)t * ld;
@@ -643,7 +690,7 @@ __global__ void __launch_bounds__(SEL)
         th = -INFINITY;
         if (cand && m < k) th = theta[t];
         if (m >= k) {
-            const uint32_t o = kth_largest(m, k, key, &count, [&](int i) {
+            const uint32_t o = kth_largest<THETA>(m, k, key, &count, [&](int i) {
                 return ordered_score(cand ? __uint_as_float((uint32_t)(c[i] >> 32)) : s[i]);
             });
             const float kth = o ? unordered(o) : -INFINITY;
@@ -768,7 +815,7 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
             float cut = -INFINITY;
             if (m > p.k) {
                 const uint32_t o =
-                    kth_largest(m, p.k, key, &s_n, [&](int i) { return ordered_score(approx(i)); });
+                    kth_largest<SEL>(m, p.k, key, &s_n, [&](int i) { return ordered_score(approx(i)); });
                 cut = o ? unordered(o) - two_eps : -INFINITY;
             }
             __syncthreads();
@@ -791,7 +838,7 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
                 }
                 __syncthreads();
                 found = s_n;
-                sort_desc(key, found);
+                sort_desc<SEL>(key, found);
             }
         }
         if (whole) {
@@ -815,7 +862,7 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
                 __syncthreads();
                 const int have = s_n;
                 if (have > LIST - BATCH || r0 + BATCH >= p.n_rows) {
-                    sort_desc(key, have);
+                    sort_desc<SEL>(key, have);
                     found = min(have, p.k);
                     floor_key = found == p.k ? key[p.k - 1] : 0;
                     __syncthreads();
@@ -866,7 +913,7 @@ static bool make_plan(int fmt, int dp, int nq, int64_t n_tiles, Plan* out) {
     const int aps = atoms_per_stage(fmt), steps = dp / 64;
     const int kchunks = (dp / 2 + KC - 1) / KC;
     const int stage = A_BYTES + aps * 512;
-    const int fixed = 1024 + 2 * MAX_NT * 4 + (4 * MAX_STAGES + 8) * 8 + 64;
+    const int fixed = 1024 + 2 * MAX_NT * 4 + EPI_WARPS * HITS * 9 + (4 * MAX_STAGES + 8) * 8 + 64;
     constexpr int64_t pairs = 74;  // of the B200's 148 SMs
     double best = 0.0;
     bool any = false;
@@ -988,7 +1035,7 @@ int launch_fp4_product(const Fp4Product& L, cudaStream_t st) {
 int launch_fp4_theta(const float* sample, int64_t ld, int m, const uint64_t* cand, int k, int dim,
                      const float* q_scale, int nt, int nt_pad, const float* q_norm,
                      const float* norm_max, int nq, float* theta, int* cand_n, cudaStream_t st) {
-    fp4::theta_kernel<<<(unsigned)nq, fp4::SEL, 0, st>>>(sample, ld, m, cand, k,
+    fp4::theta_kernel<<<(unsigned)nq, fp4::THETA, 0, st>>>(sample, ld, m, cand, k,
                                                          fp4::pad_dim(dim), q_scale, nt, nt_pad,
                                                          q_norm, norm_max, theta, cand_n);
     return cudaGetLastError() == cudaSuccess ? 0 : PION_B200_ECUDA;
