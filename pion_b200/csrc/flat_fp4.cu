@@ -135,6 +135,14 @@ __device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
         : "memory");
 }
 
+// One lane of the warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(one));
+    return one != 0;
+}
+
 // Instruction descriptor of the block-scaled kinds: e2m1 x e2m1 -> f32, both K-major.
 template <int FMT>
 __host__ __device__ constexpr uint32_t make_idesc_fp4(int m, int n) {
@@ -311,7 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);  // warp-uniform
     const int lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int pair = blockIdx.x >> 1;
@@ -455,58 +463,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             for (int s = 0; s < stages; ++s)
                 if ((issued >> s) & 1u)
                     mbar_wait(&full[s], (parity >> s) & 1u, p.status, nullptr, p.wait_ns);
-        } else if (warp == 5 && lane == 0 && rank == 0) {
+        } else if (warp == 5 && rank == 0) {
             // --------------------------------------------------- MMA issuer
+            // The whole warp runs the loop, so that every operand is in a uniform register; one
+            // lane issues.  (From a branch of one lane an MMA took 130 ns to issue, whatever
+            // its shape.)
             const uint32_t idesc = make_idesc_fp4<FMT>(ROWS, nt);
+            const uint64_t a_first = make_sw128_kmajor_desc(smem_u32(ring));
+            const uint64_t b_first = make_sw128_kmajor_desc(smem_u32(sB));
+            const uint32_t b_step = (uint32_t)(nt / 2) * KC >> 4;
+            const bool one = elect_one();
             int stage = 0, set = 0, buf = 0;
             uint32_t set_phase = 0, buf_phase = 0;
             bool ok = true;
             for (int j = first; j < p.n_tiles && ok; j += stride) {
-                if (!mbar_wait(&tempty[buf], buf_phase ^ 1u, p.status, abort_flag,
-                                       p.wait_ns))
+                if (!__all_sync(0xffffffffu, mbar_wait(&tempty[buf], buf_phase ^ 1u, p.status,
+                                                       abort_flag, p.wait_ns)))
                     break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(buf * nt);
                 for (int kc = 0; kc < kchunks; ++kc) {
-                    if (!mbar_wait(&sready[set], set_phase, p.status, abort_flag,
-                                           p.wait_ns)) {
-                        ok = false;
-                        break;
-                    }
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sready[set], set_phase, p.status,
+                                                           abort_flag, p.wait_ns));
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t a0 = smem_u32(ring + stage * STAGE);
-                    const uint32_t b0 = smem_u32(sB + kc * (nt / 2) * KC);
+                    const uint64_t a = a_first + (uint32_t)(stage * (STAGE >> 4));
+                    const uint64_t b = b_first + (uint32_t)kc * b_step;
                     const uint32_t sfa = tmem_base + col_sets + set * set_cols;
                     const uint32_t sfb = resident
                                              ? tmem_base + col_sfb + kc * APS * sf_tiles * 4
                                              : sfa + APS * 4;
-                    const int steps = min(4, p.mmas - kc * 4);
-                    for (int kk = 0; kk < steps; ++kk) {
-                        // MX: an atom's bytes 0-1 scale one 64-element step, 2-3 the next
-                        const int a = FMT == kMX ? kk >> 1 : kk;
-                        const uint32_t id = FMT == kMX ? (uint32_t)(kk & 1) * 2u : 0u;
-                        mma_fp4<FMT>(d_tmem, make_sw128_kmajor_desc(a0 + kk * 32),
-                                     make_sw128_kmajor_desc(b0 + kk * 32),
-                                     idesc | (id << 4) | (id << 29), sfa + a * 4,
-                                     sfb + a * sf_tiles * 4, (kc | kk) != 0 ? 1u : 0u);
+                    const bool whole = p.mmas - kc * 4 >= 4;  // else 128 elements, two steps
+                    if (one) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            // MX: an atom's bytes 0-1 scale one 64-element step, 2-3 the next
+                            constexpr bool mx = FMT == kMX;
+                            const int atom = mx ? kk >> 1 : kk;
+                            const uint32_t id = mx ? (uint32_t)(kk & 1) * 2u : 0u;
+                            if (kk < 2 || whole)
+                                mma_fp4<FMT>(d_tmem, a + kk * 2, b + kk * 2,
+                                             idesc | (id << 4) | (id << 29), sfa + atom * 4,
+                                             sfb + atom * sf_tiles * 4,
+                                             kk == 0 ? (kc != 0 ? 1u : 0u) : 1u);
+                        }
+                        tc_commit_pair(&empty[stage]);
+                        tc_commit_pair(&sfree[set]);
+                        if (kc == kchunks - 1) tc_commit_pair(&tfull[buf]);
                     }
-                    tc_commit_pair(&empty[stage]);
-                    tc_commit_pair(&sfree[set]);
+                    __syncwarp();
                     if (++stage == stages) stage = 0;
                     if (++set == sets) {
                         set = 0;
                         set_phase ^= 1u;
                     }
                 }
-                if (!ok) break;
-                tc_commit_pair(&tfull[buf]);
                 if (++buf == bufs) {
                     buf = 0;
                     buf_phase ^= 1u;
                 }
             }
             // All MMAs issued above complete before TMEM is released.
-            tc_commit_pair(drain);
+            if (one) tc_commit_pair(drain);
+            __syncwarp();
             mbar_wait(drain, 0, p.status, nullptr, p.wait_ns);
         }
         __syncwarp();
