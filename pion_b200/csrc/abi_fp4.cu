@@ -17,10 +17,6 @@ constexpr int64_t kMaxRows = (int64_t)INT32_MAX - 256;  // slots are 32-bit TMA 
 constexpr int64_t kMaxK = 256;
 constexpr int64_t kMaxQueries = 1 << 24;
 constexpr int64_t kQueryChunk = 4096;  // queries searched at once: bounds the scratch (64 KB each)
-// Row tiles scored for the first threshold: more for few queries, where a part of the rows less
-// to score again counts for more than a longer selection.
-int sample_tiles(int64_t nq) { return nq <= 64 ? 64 : 32; }
-
 int elem_bytes(int type) { return type == PION_B200_F32 ? 4 : 2; }
 bool type_ok(int type) { return type >= PION_B200_F32 && type <= PION_B200_F16; }
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -94,7 +90,7 @@ bool plan_scratch(int format, int dim, int64_t n_rows, int64_t nq, int64_t k, Sc
     s.q_norm = take((size_t)nq * 4);
     s.theta = s.cand_n = s.sample = s.cand = 0;
     if (k > 0) {
-        const int64_t most = (int64_t)sample_tiles(nq) * fp4_tile_rows();
+        const int64_t most = (int64_t)fp4_sample_tiles((int)nq) * fp4_tile_rows();
         s.theta = take((size_t)nq * 4);
         s.cand_n = take((size_t)nq * 4);
         s.sample = take((size_t)nq * (n_rows < most ? n_rows : most) * 4);
@@ -227,7 +223,7 @@ int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, i
     if (rc != 0) return rc;
 
     const int64_t n_tiles = (n_rows + fp4_tile_rows() - 1) / fp4_tile_rows();
-    const int samples = sample_tiles(nq);
+    const int samples = fp4_sample_tiles((int)nq);
     const bool dense = n_tiles <= samples;
     const int64_t m = dense ? n_rows : (int64_t)samples * fp4_tile_rows();
     timing_begin(ctx);
@@ -240,34 +236,46 @@ int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, i
     rc = launch_fp4_product(L, st);
     ctx->launches++;
     if (!dense && rc == 0) {
-        rc = launch_fp4_theta(sample, m, (int)m, nullptr, (int)k, (int)r->dim, q_scale,
-                              s.plan.nt, s.plan.nt_pad, q_norm, r->norm_max, (int)nq, theta,
-                              cand_n, st);
+        rc = launch_fp4_theta(sample, nullptr, (int)k, (int)r->dim, q_scale, s.plan.nt,
+                              s.plan.nt_pad, q_norm, r->norm_max, (int)nq, theta, cand_n, st);
         ctx->launches++;
         L.theta = theta;
         L.cand_n = cand_n;
         L.cand = cand;
-        // About k (rows scored) / (rows of the last threshold) rows reach the threshold, with a
-        // deviation of 1 / sqrt(k) of that: `grow` leaves 13 deviations of room in the lists.
-        const double grow = fp4_cap() / ((double)k + 13.0 * sqrt((double)k));
-        int64_t have = samples;
-        while (rc == 0) {
-            const double ratio = (double)n_tiles / (double)have;
-            int64_t next = n_tiles;
-            if (ratio > grow || (nq > 64 && ratio > 16.0)) {
-                const double by = ratio > grow * grow ? grow : sqrt(ratio);
-                next = (int64_t)((double)have * (by > 2.0 ? by : 2.0));
-                if (next > n_tiles) next = n_tiles;
+        // Stages over growing parts of the rows, each with the threshold of the rows before it:
+        // every R^(L-1)-th tile, then those of every R^(L-2)-th that are new, and so on.  About
+        // k R rows of the first stage and k (R - 1) of each later one reach their threshold,
+        // with a deviation of 1 / sqrt(k) of that: the lists have room for 13 deviations.  A batch takes more stages, since its
+        // candidates cost the product's epilogue more than a stage costs.
+        const double ratio = (double)n_tiles / (double)samples;
+        const double room = fp4_cap() / ((double)k + 13.0 * sqrt((double)k));
+        int stages = 1;
+        int64_t grow = 0;
+        for (;; ++stages) {
+            grow = (int64_t)ceil(pow(ratio, 1.0 / stages));
+            if (grow < 2) grow = 2;
+            if ((double)(grow + (stages - 1) * (grow - 1)) <= room && (nq <= 64 || grow <= 12)) break;
+            if (grow == 2) break;
+        }
+        int64_t step = 1;
+        for (int i = 1; i < stages; ++i) step *= grow;
+        for (int i = 0; i < stages && rc == 0; ++i) {
+            if (i > 0) {
+                rc = launch_fp4_theta(nullptr, cand, (int)k, (int)r->dim, q_scale, s.plan.nt,
+                                      s.plan.nt_pad, q_norm, r->norm_max, (int)nq, theta, cand_n,
+                                      st);
+                ctx->launches++;
+                if (rc != 0) break;
+                step /= grow;
             }
-            L.tile_step = (int)(n_tiles / next);
-            L.n_tiles = (int)next;
+            const int64_t tiles = (n_tiles + step - 1) / step;
+            const int64_t before = i > 0 ? (n_tiles + step * grow - 1) / (step * grow) : 0;
+            if (tiles == before) continue;
+            L.tile_step = (int)step;
+            L.tile_skip = i > 0 ? (int)grow : 0;
+            L.n_tiles = (int)(tiles - before);
             rc = launch_fp4_product(L, st);
             ctx->launches++;
-            if (next == n_tiles || rc != 0) break;
-            rc = launch_fp4_theta(nullptr, 0, 0, cand, (int)k, (int)r->dim, q_scale, s.plan.nt,
-                                  s.plan.nt_pad, q_norm, r->norm_max, (int)nq, theta, cand_n, st);
-            ctx->launches++;
-            have = next;
         }
     }
     timing_end(ctx);

@@ -81,7 +81,8 @@ struct TcParams {
     int mmas;                 // 64-element steps per tile
     int atoms;                // scale atoms per 128 rows
     int n_tiles;              // row tiles of this launch ...
-    int tile_step;            // ... the j-th being tile j * tile_step
+    int tile_step;            // ... the j-th being tile j * tile_step, or with
+    int tile_skip;            // tile_skip = r > 0 the j-th such tile with j not a multiple of r
     // kScores
     void* out;                // [nq][ld]; column = position of the row in this launch
     int out_type;
@@ -251,13 +252,22 @@ __device__ __forceinline__ float pick(const uint32_t (&r)[32], int i) {
 __device__ __forceinline__ void collect_chunk(const uint32_t (&r)[32], const TcParams& p, Hits& h,
                                               int qt_first, int at, int64_t row, const float* gq,
                                               const float* th, float g, int lane) {
-    bool any = false;
+    const float4* t4 = reinterpret_cast<const float4*>(th + at);
+    // the largest excess over a threshold (a maximum passes over the NaN of an empty row)
+    float most = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) any |= __uint_as_float(r[i]) * g >= th[at + i];
-    if (!__any_sync(0xffffffffu, any)) return;
+    for (int i = 0; i < 8; ++i) {
+        const float4 t = t4[i];
+        most = fmaxf(most, fmaxf(fmaf(__uint_as_float(r[4 * i]), g, -t.x),
+                                 fmaf(__uint_as_float(r[4 * i + 1]), g, -t.y)));
+        most = fmaxf(most, fmaxf(fmaf(__uint_as_float(r[4 * i + 2]), g, -t.z),
+                                 fmaf(__uint_as_float(r[4 * i + 3]), g, -t.w)));
+    }
+    if (!__any_sync(0xffffffffu, most >= 0.0f)) return;
     uint32_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) mine |= (__uint_as_float(r[i]) * g >= th[at + i] ? 1u : 0u) << i;
+    for (int i = 0; i < 32; ++i)
+        mine |= (fmaf(__uint_as_float(r[i]), g, -th[at + i]) >= 0.0f ? 1u : 0u) << i;
     uint32_t columns = __reduce_or_sync(0xffffffffu, mine);
     while (columns) {
         const int i = __ffs(columns) - 1;
@@ -273,6 +283,10 @@ __device__ __forceinline__ void collect_chunk(const uint32_t (&r)[32], const TcP
         }
         h.n += __popc(m);
     }
+}
+
+__device__ __forceinline__ int tile_of(const TcParams& p, int j) {
+    return p.tile_step * (p.tile_skip > 0 ? j + j / (p.tile_skip - 1) + 1 : j);
 }
 
 // ------------------------------------------------------------ the product --
@@ -303,7 +317,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint8_t* sSF = sB + kchunks * (nt / 2) * KC;             // [128-query tile][kchunk][APS]
     if (resident) sSF = ring;                                // ... only until it is in TMEM
     uint8_t* after = sB + kchunks * (nt / 2) * KC + (resident ? 0 : sf_tiles * kchunks * APS * 512);
-    float* s_gq = reinterpret_cast<float*>(after);
+    float* s_gq = reinterpret_cast<float*>(after);           // 16-byte aligned, like s_th
     float* s_th = s_gq + MAX_NT;
     uint64_t* s_hits = reinterpret_cast<uint64_t*>(s_th + MAX_NT);
     uint8_t* s_hit_col = reinterpret_cast<uint8_t*>(s_hits + EPI_WARPS * HITS);
@@ -439,7 +453,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             int stage = 0;
             uint32_t phase = 0, issued = 0, parity = 0;  // bits by stage
             for (int j = first; j < p.n_tiles && ok; j += stride) {
-                const int half_tile = j * p.tile_step * 2 + (int)rank;
+                const int half_tile = tile_of(p, j) * 2 + (int)rank;
                 for (int kc = 0; kc < kchunks; ++kc) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, p.status, abort_flag, p.wait_ns)) {
                         ok = false;
@@ -540,7 +554,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         int buf = 0;
         uint32_t buf_phase = 0;
         for (int j = first; j < p.n_tiles; j += stride) {
-            const int64_t row = (int64_t)j * p.tile_step * ROWS + in_tile;
+            const int64_t row = (int64_t)tile_of(p, j) * ROWS + in_tile;
             const bool row_in = row < p.n_rows;
             const float g = row_in ? __ldg(&p.row_scale[row]) : __int_as_float(0x7fc00000);
             const bool got = mbar_wait(&tfull[buf], buf_phase, p.status, abort_flag, p.wait_ns);
@@ -592,49 +606,131 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 }
 
 // --------------------------------------------------------------- selection --
-constexpr int THETA = 1024;  // threads of a threshold CTA
-constexpr int SEL = 512;     // threads of a finishing CTA
-constexpr int MAX_K = 256;
+constexpr int SEL = 256;  // threads of a selection CTA
+static_assert(LIST == 64 * 32, "a warp holds a list in registers");
 
 __device__ __forceinline__ uint32_t ordered_score(float v) { return v == v ? ordered(v) : 0u; }
 
-// Rank of key[i] among key[0:n], largest first, equal ones by index (n rounded up to a multiple
-// of 2 must be readable; key 16-byte aligned).
-__device__ __forceinline__ int rank_of(const uint64_t* key, int n, int i) {
-    const uint64_t x = key[i];
-    int rank = 0;
-    for (int j = 0; j < n; j += 2) {
-        const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(key + j);
-        rank += y.x > x || (y.x == x && j < i);
-        if (j + 1 < n) rank += y.y > x || (y.y == x && j + 1 < i);
+// The k-th largest of a warp's 32 V values, bit by bit from the highest: a bit is set if k values
+// reach the number with it.  About 50 + V cycles a bit, and no shared memory.
+template <int V>
+__device__ __forceinline__ uint32_t warp_kth(const uint32_t (&v)[V], int k) {
+    uint32_t x = 0;
+#pragma unroll 1
+    for (int b = 31; b >= 0; --b) {
+        const uint32_t y = x | (1u << b);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) c += v[i] >= y;
+        if (__reduce_add_sync(0xffffffffu, c) >= k) x = y;
     }
-    return rank;
+    return x;
 }
 
-// Sorts n <= LIST keys in shared memory, largest first: few by their ranks, more by a bitonic
-// sort over the next power of two (the rest is filled with zeros).
-template <int NT>
-__device__ void sort_desc(uint64_t* key, int n) {
-    if (n <= NT) {
-        __syncthreads();
-        int at = 0;
-        uint64_t x = 0;
-        if ((int)threadIdx.x < n) {
-            x = key[threadIdx.x];
-            at = rank_of(key, n, threadIdx.x);
+template <int V, class F>
+__device__ __forceinline__ uint32_t warp_kth_of(int m, int k, F value) {
+    const int lane = threadIdx.x & 31;
+    uint32_t v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = lane + 32 * i < m ? value(lane + 32 * i) : 0u;
+    return warp_kth<V>(v, k);
+}
+
+// The k-th largest (1-based, k <= MAX_K, k <= m) of m ordered values, by a CTA of SEL threads, or
+// where more than LIST values reach it a lower bound of it.  Few values go through one warp;
+// of more, the k-th largest of the threads' maxima is a lower bound that few values reach,
+// and those go through one warp.  A thread keeps its first HOLD values in registers between
+// the two passes.  `list` holds LIST values of scratch.
+template <int HOLD, class F>
+__device__ uint32_t kth_largest(int m, int k, uint32_t* list, F value) {
+    __shared__ uint32_t s_low;
+    __shared__ int s_count;
+    const bool first = threadIdx.x < 32;
+    if (m <= 512) {
+        if (first) {
+            const uint32_t x = m <= 256 ? warp_kth_of<8>(m, k, value) : warp_kth_of<16>(m, k, value);
+            if (threadIdx.x == 0) s_low = x;
         }
         __syncthreads();
-        if ((int)threadIdx.x < n) key[at] = x;
+        return s_low;
+    }
+    uint32_t held[HOLD];
+    uint32_t top = 0;
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) {
+        const int i = threadIdx.x + h * SEL;
+        held[h] = i < m ? value(i) : 0u;
+    }
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h) top = max(top, held[h]);
+    // four loads in flight at a time
+    auto rest = [&](auto use) {
+        for (int i = threadIdx.x + HOLD * SEL; i < m; i += 4 * SEL) {
+            uint32_t o[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[u] = i + u * SEL < m ? value(i + u * SEL) : 0u;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + u * SEL < m) use(o[u]);
+        }
+    };
+    rest([&](uint32_t o) { top = max(top, o); });
+    list[threadIdx.x] = top;
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+    if (first) {
+        const uint32_t x = warp_kth_of<8>(SEL, k, [&](int i) { return list[i]; });
+        if (threadIdx.x == 0) s_low = x;
+    }
+    __syncthreads();
+    const uint32_t low = s_low;
+    auto keep = [&](uint32_t o) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < LIST) list[at] = o;
+    };
+#pragma unroll
+    for (int h = 0; h < HOLD; ++h)
+        if ((int)threadIdx.x + h * SEL < m && held[h] >= low) keep(held[h]);
+    rest([&](uint32_t o) {
+        if (o >= low) keep(o);
+    });
+    __syncthreads();
+    const int n = s_count;
+    if (n > LIST) return low;
+    if (first) {
+        auto at = [&](int i) { return list[i]; };
+        const uint32_t x = n <= 256 ? warp_kth_of<8>(n, k, at) : warp_kth_of<64>(n, k, at);
+        if (threadIdx.x == 0) s_low = x;
+    }
+    __syncthreads();
+    return s_low;
+}
+
+// Sorts n <= LIST keys in shared memory, largest first: up to a key per thread by their ranks,
+// more by a bitonic sort over the next power of two (the rest is filled with zeros).
+__device__ void sort_desc(uint64_t* key, int n) {
+    __syncthreads();
+    if (n <= SEL) {
+        const int i = threadIdx.x;
+        int at = 0;
+        const uint64_t x = i < n ? key[i] : 0;
+        if (i < n)
+            for (int j = 0; j < n; ++j) {
+                const uint64_t y = key[j];
+                at += y > x || (y == x && j < i);
+            }
+        __syncthreads();
+        if (i < n) key[at] = x;
         __syncthreads();
         return;
     }
     int size = 2;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += NT) key[i] = 0;
+    for (int i = n + threadIdx.x; i < size; i += SEL) key[i] = 0;
     __syncthreads();
     for (int w = 2; w <= size; w <<= 1)
         for (int s = w >> 1; s; s >>= 1) {
-            for (int i = threadIdx.x; i < size / 2; i += NT) {
+            for (int i = threadIdx.x; i < size / 2; i += SEL) {
                 const int a = 2 * i - (i & (s - 1));
                 const int b = a + s;
                 const bool desc = (a & w) == 0;
@@ -648,41 +744,6 @@ __device__ void sort_desc(uint64_t* key, int n) {
         }
 }
 
-// The k-th largest (1-based, k <= MAX_K, k <= m) of m ordered values, by the CTA, or where more
-// than LIST values reach it a lower bound of it.  The k-th largest of the maxima of 256
-// groups of threads is a lower bound that few values reach; those are sorted.  `key` holds
-// LIST keys of scratch, `count` one integer.
-template <int NT, class F>
-__device__ uint32_t kth_largest(int m, int k, uint64_t* key, int* count, F value) {
-    constexpr int G = NT / MAX_K;  // threads per group, neighbours of one warp
-    uint32_t top = 0;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < m; i += NT) top = max(top, value(i));
-#pragma unroll
-    for (int o = 1; o < G; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (threadIdx.x % G == 0) key[threadIdx.x / G] = top;
-    if (threadIdx.x == 0) *count = 0;
-    __syncthreads();
-    __shared__ uint32_t s_low;
-    if (threadIdx.x < MAX_K && rank_of(key, MAX_K, threadIdx.x) == k - 1)
-        s_low = (uint32_t)key[threadIdx.x];
-    __syncthreads();
-    const uint32_t low = s_low;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < m; i += NT) {
-        const uint32_t o = value(i);
-        if (o >= low) {
-            const int at = atomicAdd(count, 1);
-            if (at < LIST) key[at] = o;
-        }
-    }
-    __syncthreads();
-    const int n = *count;
-    if (n > LIST) return low;
-    sort_desc<NT>(key, n);
-    return (uint32_t)key[k - 1];
-}
-
 // Infinite where a float32 sum could overflow: nothing is known of an approximate score then.
 // The last term covers products below the least normal float.
 __device__ __forceinline__ float eps_of(int dp, float q_norm, float norm_max) {
@@ -690,39 +751,92 @@ __device__ __forceinline__ float eps_of(int dp, float q_norm, float norm_max) {
     return size < 0x1p120f ? rel_eps(dp) * size + 0x1p-100f : INFINITY;
 }
 
-// Threshold of one query per CTA: the k-th best of its approximate scores so far (the sample's,
-// or the candidates of a part of the rows) less 2 eps, in units of the query's g.  Resets the
-// query's candidate count.
-__global__ void __launch_bounds__(THETA)
-    theta_kernel(const float* sample, int64_t ld, int m, const uint64_t* cand, int k,
-                 int dp, const float* q_scale, int nt, int nt_pad, const float* q_norm,
-                 const float* norm_max, float* theta, int* cand_n) {
-    __shared__ __align__(16) uint64_t key[LIST];
-    __shared__ int count;
+// A query's threshold: the k-th best (ordered) of its approximate scores so far less 2 eps, in
+// units of the query's g.
+__device__ __forceinline__ float threshold_of(uint32_t kth, float two_eps, float gq) {
+    const float x = ((kth ? unordered(kth) : -INFINITY) - two_eps) / gq;
+    return x > -INFINITY ? x - 0x1p-20f * fabsf(x) : -INFINITY;
+}
+
+// First thresholds, one query per CTA, from the scores of 4 V4 NT sampled rows, which stay in
+// registers: the k-th largest of the maxima of 256 groups of threads bounds the k-th best
+// from below, and the few scores that reach it are searched.  Resets the candidate counts.
+template <int NT, int V4>
+__global__ void __launch_bounds__(NT)
+    theta_sample_kernel(const float* __restrict__ sample, int k, int dp,
+                        const float* __restrict__ q_scale, int nt, int nt_pad,
+                        const float* __restrict__ q_norm, const float* __restrict__ norm_max,
+                        float* theta, int* cand_n) {
+    __shared__ uint32_t list[LIST];
+    __shared__ uint32_t s_low;
+    __shared__ int s_count;
     const int t = blockIdx.x;
-    const float* s = sample + (int64_t)t * ld;
-    const uint64_t* c = cand + (int64_t)t * CAP;
-    if (cand) m = min(cand_n[t], CAP);
-    const float gq = q_scale[query_slot(t, nt, nt_pad)];
-    float th = INFINITY;  // an empty or zero query collects nothing
-    if (gq > 0.0f) {
-        th = -INFINITY;
-        if (cand && m < k) th = theta[t];
-        if (m >= k) {
-            const uint32_t o = kth_largest<THETA>(m, k, key, &count, [&](int i) {
-                return ordered_score(cand ? __uint_as_float((uint32_t)(c[i] >> 32)) : s[i]);
-            });
-            const float kth = o ? unordered(o) : -INFINITY;
-            const float low = kth - 2.0f * eps_of(dp, q_norm[t], *norm_max);
-            th = low / gq;
-            th = th > -INFINITY ? th - 0x1p-20f * fabsf(th) : -INFINITY;
-        }
+    const float4* s = reinterpret_cast<const float4*>(sample) + (int64_t)t * NT * V4;
+    float4 v[V4];
+#pragma unroll
+    for (int i = 0; i < V4; ++i) v[i] = __ldg(s + threadIdx.x + i * NT);
+    const float gq = __ldg(q_scale + query_slot(t, nt, nt_pad));
+    const float two_eps = 2.0f * eps_of(dp, __ldg(q_norm + t), __ldg(norm_max));
+    float most = -INFINITY;  // (passes over NaN)
+#pragma unroll
+    for (int i = 0; i < V4; ++i)
+        most = fmaxf(most, fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w)));
+#pragma unroll
+    for (int o = 1; o < NT / 256; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (threadIdx.x % (NT / 256) == 0) list[threadIdx.x / (NT / 256)] = ordered(most);
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const uint32_t x = warp_kth_of<8>(256, k, [&](int i) { return list[i]; });
+        if (threadIdx.x == 0) s_low = x;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        theta[t] = th;
-        cand_n[t] = 0;
+    const uint32_t low = s_low;
+    const float low_f = unordered(low);
+    auto keep = [&](float x) {
+        if (x >= low_f) {
+            const int at = atomicAdd(&s_count, 1);
+            if (at < LIST) list[at] = ordered(x);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < V4; ++i) {
+        keep(v[i].x);
+        keep(v[i].y);
+        keep(v[i].z);
+        keep(v[i].w);
     }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int n = s_count;
+        auto at = [&](int i) { return list[i]; };
+        const uint32_t x = n > LIST  ? low
+                           : n <= 64 ? warp_kth_of<2>(n, k, at)
+                           : n <= 512 ? warp_kth_of<16>(n, k, at)
+                                      : warp_kth_of<64>(n, k, at);
+        if (threadIdx.x == 0) {
+            // an empty or zero query collects nothing
+            theta[t] = gq > 0.0f ? threshold_of(x, two_eps, gq) : INFINITY;
+            cand_n[t] = 0;
+        }
+    }
+}
+
+// Tighter thresholds, one query per CTA, from the candidates so far.
+__global__ void __launch_bounds__(SEL)
+    theta_kernel(const uint64_t* cand, int k, int dp, const float* q_scale, int nt, int nt_pad,
+                 const float* q_norm, const float* norm_max, float* theta, const int* cand_n) {
+    __shared__ uint32_t list[LIST];
+    const int t = blockIdx.x;
+    const int m = min(__ldg(cand_n + t), CAP);
+    const float gq = __ldg(q_scale + query_slot(t, nt, nt_pad));
+    const float two_eps = 2.0f * eps_of(dp, __ldg(q_norm + t), __ldg(norm_max));
+    if (!(gq > 0.0f) || m < k) return;
+    const uint64_t* c = cand + (int64_t)t * CAP;
+    const uint32_t x = kth_largest<4>(m, k, list, [&](int i) {
+        return ordered_score(__uint_as_float((uint32_t)(__ldg(c + i) >> 32)));
+    });
+    if (threadIdx.x == 0) theta[t] = threshold_of(x, two_eps, gq);
 }
 
 struct FinishParams {
@@ -834,7 +948,8 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
             float cut = -INFINITY;
             if (m > p.k) {
                 const uint32_t o =
-                    kth_largest<SEL>(m, p.k, key, &s_n, [&](int i) { return ordered_score(approx(i)); });
+                    kth_largest<8>(m, p.k, reinterpret_cast<uint32_t*>(key),
+                                   [&](int i) { return ordered_score(approx(i)); });
                 cut = o ? unordered(o) - two_eps : -INFINITY;
             }
             __syncthreads();
@@ -857,7 +972,7 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
                 }
                 __syncthreads();
                 found = s_n;
-                sort_desc<SEL>(key, found);
+                sort_desc(key, found);
             }
         }
         if (whole) {
@@ -881,7 +996,7 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
                 __syncthreads();
                 const int have = s_n;
                 if (have > LIST - BATCH || r0 + BATCH >= p.n_rows) {
-                    sort_desc<SEL>(key, have);
+                    sort_desc(key, have);
                     found = min(have, p.k);
                     floor_key = found == p.k ? key[p.k - 1] : 0;
                     __syncthreads();
@@ -1026,6 +1141,7 @@ int launch_fp4_product(const Fp4Product& L, cudaStream_t st) {
     p.atoms = atoms;
     p.n_tiles = L.n_tiles > 0 ? L.n_tiles : (int)row_tiles;
     p.tile_step = L.tile_step;
+    p.tile_skip = L.tile_skip;
     p.out = L.out;
     p.out_type = L.out_type;
     p.ld = L.ld;
@@ -1051,12 +1167,25 @@ int launch_fp4_product(const Fp4Product& L, cudaStream_t st) {
     return cudaGetLastError() == cudaSuccess ? 0 : PION_B200_ECUDA;
 }
 
-int launch_fp4_theta(const float* sample, int64_t ld, int m, const uint64_t* cand, int k, int dim,
+int fp4_sample_tiles(int nq) { return nq <= 64 ? 64 : 32; }
+
+int launch_fp4_theta(const float* sample, const uint64_t* cand, int k, int dim,
                      const float* q_scale, int nt, int nt_pad, const float* q_norm,
                      const float* norm_max, int nq, float* theta, int* cand_n, cudaStream_t st) {
-    fp4::theta_kernel<<<(unsigned)nq, fp4::THETA, 0, st>>>(sample, ld, m, cand, k,
-                                                         fp4::pad_dim(dim), q_scale, nt, nt_pad,
-                                                         q_norm, norm_max, theta, cand_n);
+    using namespace fp4;
+    const int dp = pad_dim(dim);
+    if (cand) {
+        theta_kernel<<<(unsigned)nq, SEL, 0, st>>>(cand, k, dp, q_scale, nt, nt_pad, q_norm,
+                                                   norm_max, theta, cand_n);
+    } else if (fp4_sample_tiles(nq) == 64) {
+        static_assert(64 * ROWS == 1024 * 4 * 4, "sample");
+        theta_sample_kernel<1024, 4><<<(unsigned)nq, 1024, 0, st>>>(
+            sample, k, dp, q_scale, nt, nt_pad, q_norm, norm_max, theta, cand_n);
+    } else {
+        static_assert(32 * ROWS == 256 * 8 * 4, "sample");
+        theta_sample_kernel<256, 8><<<(unsigned)nq, 256, 0, st>>>(
+            sample, k, dp, q_scale, nt, nt_pad, q_norm, norm_max, theta, cand_n);
+    }
     return cudaGetLastError() == cudaSuccess ? 0 : PION_B200_ECUDA;
 }
 

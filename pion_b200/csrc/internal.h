@@ -520,8 +520,9 @@ struct Fp4Product {
     const uint8_t* q_scales = nullptr;
     const float* q_scale = nullptr;
     int nq = 0;
-    int n_tiles = 0;   // > 0: only that many row tiles, every tile_step-th
-    int tile_step = 1;
+    int n_tiles = 0;   // > 0: only that many row tiles, every tile_step-th, with tile_skip = r
+    int tile_step = 1; // those of them that are not a multiple of r
+    int tile_skip = 0;
     void* out = nullptr;
     int out_type = 0;
     int64_t ld = 0;
@@ -533,8 +534,11 @@ struct Fp4Product {
     int num_sms = 148;
 };
 int launch_fp4_product(const Fp4Product& L, cudaStream_t st);
-// from the sample's scores, or with `cand` from the candidates kept so far
-int launch_fp4_theta(const float* sample, int64_t ld, int m, const uint64_t* cand, int k, int dim,
+// Row tiles scored for the first thresholds: more for few queries, where a part of the rows less
+// to score again counts for more than a longer selection.
+int fp4_sample_tiles(int nq);
+// From the sample's scores [nq][sample rows], or with `cand` from the candidates kept so far.
+int launch_fp4_theta(const float* sample, const uint64_t* cand, int k, int dim,
                      const float* q_scale, int nt, int nt_pad, const float* q_norm,
                      const float* norm_max, int nq, float* theta, int* cand_n, cudaStream_t st);
 struct Fp4Finish {
