@@ -69,7 +69,8 @@ int check_mem(pion_b200_ctx* ctx, const char* who, int mem) {
 
 // The scratch of a scores or knn call of at most `nq` queries at once.
 struct Scratch {
-    size_t q_codes, q_scales, q_scale, q_norm, theta, cand_n, sample, cand, total;
+    size_t q_codes, q_scales, q_scale, q_norm, theta, cand_n, n_flagged, flagged, done, parts, sample,
+        cand, total;
     Fp4Plan plan;
 };
 
@@ -88,11 +89,15 @@ bool plan_scratch(int format, int dim, int64_t n_rows, int64_t nq, int64_t k, Sc
     s.q_scales = take(slots / 128 * fp4::atoms_of(format, dp) * 512);
     s.q_scale = take(slots * 4);
     s.q_norm = take((size_t)nq * 4);
-    s.theta = s.cand_n = s.sample = s.cand = 0;
+    s.theta = s.cand_n = s.n_flagged = s.flagged = s.done = s.parts = s.sample = s.cand = 0;
     if (k > 0) {
         const int64_t most = (int64_t)fp4_sample_tiles((int)nq) * fp4_tile_rows();
         s.theta = take((size_t)nq * 4);
         s.cand_n = take((size_t)nq * 4);
+        s.n_flagged = take(4);
+        s.flagged = take((size_t)nq * 4);
+        s.done = take((size_t)nq * 4);
+        s.parts = take((size_t)fp4_rescue_items(nq) * k * 8);
         s.sample = take((size_t)nq * (n_rows < most ? n_rows : most) * 4);
         if (n_rows > most) s.cand = take((size_t)nq * fp4_cap() * 8);
     }
@@ -169,7 +174,7 @@ int stage_rows(pion_b200_ctx* ctx, const char* who, const void* src, size_t byte
 
 // The call's queries, quantised into its scratch.
 int quantise_queries(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, const void* q, int type,
-                     int64_t stride, int64_t nq, const Scratch& s, char* base) {
+                     int64_t stride, int64_t nq, const Scratch& s, char* base, int64_t k) {
     Fp4Write w;
     w.format = r->format;
     w.dim = (int)r->dim;
@@ -183,6 +188,7 @@ int quantise_queries(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, const void
     w.scales = reinterpret_cast<uint8_t*>(base + s.q_scales);
     w.row_scale = reinterpret_cast<float*>(base + s.q_scale);
     w.norm = reinterpret_cast<float*>(base + s.q_norm);
+    if (k > 0) w.zero = reinterpret_cast<int*>(base + s.n_flagged);
     ctx->launches++;
     return launch_fp4_write(w, ctx->stream);
 }
@@ -219,7 +225,7 @@ int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, i
     uint64_t* cand = reinterpret_cast<uint64_t*>(base + s.cand);
     const float* q_scale = reinterpret_cast<const float*>(base + s.q_scale);
     const float* q_norm = reinterpret_cast<const float*>(base + s.q_norm);
-    int rc = quantise_queries(ctx, r, q, q_type, q_stride, nq, s, base);
+    int rc = quantise_queries(ctx, r, q, q_type, q_stride, nq, s, base, k);
     if (rc != 0) return rc;
 
     const int64_t n_tiles = (n_rows + fp4_tile_rows() - 1) / fp4_tile_rows();
@@ -301,9 +307,13 @@ int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, i
     f.ld = m;
     f.cand_n = cand_n;
     f.cand = cand;
+    f.n_flagged = reinterpret_cast<int*>(base + s.n_flagged);
+    f.flagged = reinterpret_cast<int*>(base + s.flagged);
+    f.done = reinterpret_cast<int*>(base + s.done);
+    f.parts = reinterpret_cast<uint64_t*>(base + s.parts);
     f.out_ids = ids;
     f.out_scores = scores;
-    ctx->launches++;
+    ctx->launches += 2;
     return launch_fp4_finish(f, st);
 }
 
@@ -498,7 +508,7 @@ int pion_v_b200_fp4_scores(pion_b200_ctx* ctx, const pion_b200_fp4_rows* rows, i
         if (ensure(ctx->stage_out, (size_t)nq * n_rows * elem_bytes(out_type)) != 0)
             return set_error(ctx, PION_B200_ENOMEM, "%s: staging", who);
     }
-    int rc = quantise_queries(ctx, rows, dq, q_type, q_stride, nq, s, base);
+    int rc = quantise_queries(ctx, rows, dq, q_type, q_stride, nq, s, base, 0);
     if (rc == 0) {
         Fp4Product L = product_of(ctx, rows, n_rows, nq, s, base, mem);
         L.out = host ? ctx->stage_out.ptr : out;

@@ -12,6 +12,7 @@
 //                     or keep the rows that reach a query's threshold.
 //   theta_kernel      a query's threshold from its scores of a sample of the rows.
 //   finish_kernel     the k best of a query: its candidates scored exactly, sorted.
+//   rescue_kernel     queries with more candidates than are kept: every row, exactly.
 //
 // Exactness: a product of two codes is a multiple of 1/4 up to 36, and a row's scales span a
 // few powers of two, so the sum in float64 is exact; it is rounded once to float32, and rows
@@ -362,11 +363,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         *abort_flag = 0;
         fence_barrier_init();
     }
+    griddep_launch();
+    griddep_wait();
     for (int j = threadIdx.x; j < MAX_NT; j += THREADS) {
         const int t = qt * nt + j;
         const bool ok = j < nt && t < p.nq;
-        s_gq[j] = ok ? p.q_scale[(int64_t)qt * p.plan.nt_pad + j] : 0.0f;
-        s_th[j] = ok && mode == kCollect ? p.theta[t] : INFINITY;
+        s_gq[j] = ok ? __ldcg(p.q_scale + (int64_t)qt * p.plan.nt_pad + j) : 0.0f;
+        s_th[j] = ok && mode == kCollect ? __ldcg(p.theta + t) : INFINITY;
     }
     if (warp == 5) tmem_alloc_pair(tmem_slot, TMEM_COLS);
     tc_fence_before();
@@ -556,7 +559,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         for (int j = first; j < p.n_tiles; j += stride) {
             const int64_t row = (int64_t)tile_of(p, j) * ROWS + in_tile;
             const bool row_in = row < p.n_rows;
-            const float g = row_in ? __ldg(&p.row_scale[row]) : __int_as_float(0x7fc00000);
+            const float g = row_in ? __ldcg(&p.row_scale[row]) : __int_as_float(0x7fc00000);
             const bool got = mbar_wait(&tfull[buf], buf_phase, p.status, abort_flag, p.wait_ns);
             if (!__all_sync(0xffffffffu, got)) break;
             tc_fence_after();
@@ -607,7 +610,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
 // --------------------------------------------------------------- selection --
 constexpr int SEL = 256;  // threads of a selection CTA
-static_assert(LIST == 64 * 32, "a warp holds a list in registers");
 
 __device__ __forceinline__ uint32_t ordered_score(float v) { return v == v ? ordered(v) : 0u; }
 
@@ -636,18 +638,54 @@ __device__ __forceinline__ uint32_t warp_kth_of(int m, int k, F value) {
     return warp_kth<V>(v, k);
 }
 
-// The k-th largest (1-based, k <= MAX_K, k <= m) of m ordered values, by a CTA of SEL threads, or
+// The k-th largest of n <= LIST values in shared memory, by a CTA of NT threads: one warp's
+// search of up to 512, else the same search by all with a barrier a bit.
+template <int NT>
+__device__ uint32_t list_kth(const uint32_t* list, int n, int k) {
+    __shared__ uint32_t s_kth;
+    __shared__ int s_bit[32];
+    if (n <= 512) {
+        if (threadIdx.x < 32) {
+            auto at = [&](int i) { return list[i]; };
+            const uint32_t x = n <= 64 ? warp_kth_of<2>(n, k, at) : warp_kth_of<16>(n, k, at);
+            if (threadIdx.x == 0) s_kth = x;
+        }
+        __syncthreads();
+        return s_kth;
+    }
+    constexpr int V = LIST / NT;
+    uint32_t v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        v[i] = (int)threadIdx.x + i * NT < n ? list[threadIdx.x + i * NT] : 0u;
+    if (threadIdx.x < 32) s_bit[threadIdx.x] = 0;
+    __syncthreads();
+    uint32_t x = 0;
+#pragma unroll 1
+    for (int b = 31; b >= 0; --b) {
+        const uint32_t y = x | (1u << b);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) c += v[i] >= y;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if ((threadIdx.x & 31) == 0 && c) atomicAdd(&s_bit[b], c);
+        __syncthreads();
+        if (s_bit[b] >= k) x = y;
+    }
+    return x;
+}
+
+// The k-th largest (1-based, k <= 256, k <= m) of m ordered values, by a CTA of NT threads, or
 // where more than LIST values reach it a lower bound of it.  Few values go through one warp;
 // of more, the k-th largest of the threads' maxima is a lower bound that few values reach,
-// and those go through one warp.  A thread keeps its first HOLD values in registers between
-// the two passes.  `list` holds LIST values of scratch.
-template <int HOLD, class F>
+// and those are searched.  A thread keeps its first HOLD values in registers between the two
+// passes.  `list` holds LIST values of scratch.
+template <int NT, int HOLD, class F>
 __device__ uint32_t kth_largest(int m, int k, uint32_t* list, F value) {
     __shared__ uint32_t s_low;
     __shared__ int s_count;
-    const bool first = threadIdx.x < 32;
     if (m <= 512) {
-        if (first) {
+        if (threadIdx.x < 32) {
             const uint32_t x = m <= 256 ? warp_kth_of<8>(m, k, value) : warp_kth_of<16>(m, k, value);
             if (threadIdx.x == 0) s_low = x;
         }
@@ -658,28 +696,28 @@ __device__ uint32_t kth_largest(int m, int k, uint32_t* list, F value) {
     uint32_t top = 0;
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) {
-        const int i = threadIdx.x + h * SEL;
+        const int i = threadIdx.x + h * NT;
         held[h] = i < m ? value(i) : 0u;
     }
 #pragma unroll
     for (int h = 0; h < HOLD; ++h) top = max(top, held[h]);
     // four loads in flight at a time
     auto rest = [&](auto use) {
-        for (int i = threadIdx.x + HOLD * SEL; i < m; i += 4 * SEL) {
+        for (int i = threadIdx.x + HOLD * NT; i < m; i += 4 * NT) {
             uint32_t o[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) o[u] = i + u * SEL < m ? value(i + u * SEL) : 0u;
+            for (int u = 0; u < 4; ++u) o[u] = i + u * NT < m ? value(i + u * NT) : 0u;
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (i + u * SEL < m) use(o[u]);
+                if (i + u * NT < m) use(o[u]);
         }
     };
     rest([&](uint32_t o) { top = max(top, o); });
     list[threadIdx.x] = top;
     if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
-    if (first) {
-        const uint32_t x = warp_kth_of<8>(SEL, k, [&](int i) { return list[i]; });
+    if (threadIdx.x < 32) {
+        const uint32_t x = warp_kth_of<NT / 32>(NT, k, [&](int i) { return list[i]; });
         if (threadIdx.x == 0) s_low = x;
     }
     __syncthreads();
@@ -690,27 +728,21 @@ __device__ uint32_t kth_largest(int m, int k, uint32_t* list, F value) {
     };
 #pragma unroll
     for (int h = 0; h < HOLD; ++h)
-        if ((int)threadIdx.x + h * SEL < m && held[h] >= low) keep(held[h]);
+        if ((int)threadIdx.x + h * NT < m && held[h] >= low) keep(held[h]);
     rest([&](uint32_t o) {
         if (o >= low) keep(o);
     });
     __syncthreads();
     const int n = s_count;
-    if (n > LIST) return low;
-    if (first) {
-        auto at = [&](int i) { return list[i]; };
-        const uint32_t x = n <= 256 ? warp_kth_of<8>(n, k, at) : warp_kth_of<64>(n, k, at);
-        if (threadIdx.x == 0) s_low = x;
-    }
-    __syncthreads();
-    return s_low;
+    return n > LIST ? low : list_kth<NT>(list, n, k);
 }
 
 // Sorts n <= LIST keys in shared memory, largest first: up to a key per thread by their ranks,
 // more by a bitonic sort over the next power of two (the rest is filled with zeros).
+template <int NT>
 __device__ void sort_desc(uint64_t* key, int n) {
     __syncthreads();
-    if (n <= SEL) {
+    if (n <= NT && n <= 512) {
         const int i = threadIdx.x;
         int at = 0;
         const uint64_t x = i < n ? key[i] : 0;
@@ -726,11 +758,11 @@ __device__ void sort_desc(uint64_t* key, int n) {
     }
     int size = 2;
     while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += SEL) key[i] = 0;
+    for (int i = n + threadIdx.x; i < size; i += NT) key[i] = 0;
     __syncthreads();
     for (int w = 2; w <= size; w <<= 1)
         for (int s = w >> 1; s; s >>= 1) {
-            for (int i = threadIdx.x; i < size / 2; i += SEL) {
+            for (int i = threadIdx.x; i < size / 2; i += NT) {
                 const int a = 2 * i - (i & (s - 1));
                 const int b = a + s;
                 const bool desc = (a & w) == 0;
@@ -763,20 +795,22 @@ __device__ __forceinline__ float threshold_of(uint32_t kth, float two_eps, float
 // from below, and the few scores that reach it are searched.  Resets the candidate counts.
 template <int NT, int V4>
 __global__ void __launch_bounds__(NT)
-    theta_sample_kernel(const float* __restrict__ sample, int k, int dp,
-                        const float* __restrict__ q_scale, int nt, int nt_pad,
-                        const float* __restrict__ q_norm, const float* __restrict__ norm_max,
+    theta_sample_kernel(const float* sample, int k, int dp,
+                        const float* q_scale, int nt, int nt_pad,
+                        const float* q_norm, const float* norm_max,
                         float* theta, int* cand_n) {
     __shared__ uint32_t list[LIST];
     __shared__ uint32_t s_low;
     __shared__ int s_count;
+    griddep_launch();
+    griddep_wait();
     const int t = blockIdx.x;
     const float4* s = reinterpret_cast<const float4*>(sample) + (int64_t)t * NT * V4;
     float4 v[V4];
 #pragma unroll
-    for (int i = 0; i < V4; ++i) v[i] = __ldg(s + threadIdx.x + i * NT);
-    const float gq = __ldg(q_scale + query_slot(t, nt, nt_pad));
-    const float two_eps = 2.0f * eps_of(dp, __ldg(q_norm + t), __ldg(norm_max));
+    for (int i = 0; i < V4; ++i) v[i] = __ldcg(s + threadIdx.x + i * NT);
+    const float gq = __ldcg(q_scale + query_slot(t, nt, nt_pad));
+    const float two_eps = 2.0f * eps_of(dp, __ldcg(q_norm + t), __ldcg(norm_max));
     float most = -INFINITY;  // (passes over NaN)
 #pragma unroll
     for (int i = 0; i < V4; ++i)
@@ -807,18 +841,12 @@ __global__ void __launch_bounds__(NT)
         keep(v[i].w);
     }
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const int n = s_count;
-        auto at = [&](int i) { return list[i]; };
-        const uint32_t x = n > LIST  ? low
-                           : n <= 64 ? warp_kth_of<2>(n, k, at)
-                           : n <= 512 ? warp_kth_of<16>(n, k, at)
-                                      : warp_kth_of<64>(n, k, at);
-        if (threadIdx.x == 0) {
-            // an empty or zero query collects nothing
-            theta[t] = gq > 0.0f ? threshold_of(x, two_eps, gq) : INFINITY;
-            cand_n[t] = 0;
-        }
+    const int n = s_count;
+    const uint32_t x = n > LIST ? low : list_kth<NT>(list, n, k);
+    if (threadIdx.x == 0) {
+        // an empty or zero query collects nothing
+        theta[t] = gq > 0.0f ? threshold_of(x, two_eps, gq) : INFINITY;
+        cand_n[t] = 0;
     }
 }
 
@@ -827,14 +855,16 @@ __global__ void __launch_bounds__(SEL)
     theta_kernel(const uint64_t* cand, int k, int dp, const float* q_scale, int nt, int nt_pad,
                  const float* q_norm, const float* norm_max, float* theta, const int* cand_n) {
     __shared__ uint32_t list[LIST];
+    griddep_launch();
+    griddep_wait();
     const int t = blockIdx.x;
-    const int m = min(__ldg(cand_n + t), CAP);
-    const float gq = __ldg(q_scale + query_slot(t, nt, nt_pad));
-    const float two_eps = 2.0f * eps_of(dp, __ldg(q_norm + t), __ldg(norm_max));
+    const int m = min(__ldcg(cand_n + t), CAP);
+    const float gq = __ldcg(q_scale + query_slot(t, nt, nt_pad));
+    const float two_eps = 2.0f * eps_of(dp, __ldcg(q_norm + t), __ldcg(norm_max));
     if (!(gq > 0.0f) || m < k) return;
     const uint64_t* c = cand + (int64_t)t * CAP;
-    const uint32_t x = kth_largest<4>(m, k, list, [&](int i) {
-        return ordered_score(__uint_as_float((uint32_t)(__ldg(c + i) >> 32)));
+    const uint32_t x = kth_largest<SEL, 4>(m, k, list, [&](int i) {
+        return ordered_score(__uint_as_float((uint32_t)(__ldcg(c + i) >> 32)));
     });
     if (threadIdx.x == 0) theta[t] = threshold_of(x, two_eps, gq);
 }
@@ -857,6 +887,11 @@ struct FinishParams {
     int64_t ld;
     const int* cand_n;       // else the candidates
     const uint64_t* cand;
+    int nq;
+    int* n_flagged;          // queries left to rescue_kernel, their number
+    int* flagged;            // ... which [nq]
+    int* done;               // ... their finished parts [nq]
+    uint64_t* parts;         // ... the parts' best keys [items][k]
     int32_t* out_ids;        // [nq][k]
     float* out_scores;
 };
@@ -875,7 +910,7 @@ __device__ __forceinline__ double warp_dot(const FinishParams& p, const QuerySha
     const uint4* codes = reinterpret_cast<const uint4*>(p.codes + row * (p.dp / 2));
     double acc = 0.0;
     for (int b = lane; b < p.dp / 32; b += 32) {  // 32 elements per lane
-        const uint4 w = __ldg(codes + b);
+        const uint4 w = __ldcg(codes + b);
         const uint32_t raw[4] = {w.x, w.y, w.z, w.w};
         const int4* qb = reinterpret_cast<const int4*>(q.codes + b * 32);
         int dot[2] = {0, 0};
@@ -889,11 +924,11 @@ __device__ __forceinline__ double warp_dot(const FinishParams& p, const QuerySha
         }
         if (FMT == kMX) {
             const float s =
-                e8m0_value(__ldg(p.scales + scale_word(row, b >> 2, p.atoms) + (b & 3)));
+                e8m0_value(__ldcg(p.scales + scale_word(row, b >> 2, p.atoms) + (b & 3)));
             acc += (double)(dot[0] + dot[1]) * ((double)q.scales[b] * (double)s);
         } else {
             const uint8_t* at = p.scales + scale_word(row, b >> 1, p.atoms) + (b & 1) * 2;
-            const uint32_t two = __ldg(reinterpret_cast<const uint16_t*>(at));
+            const uint32_t two = __ldcg(reinterpret_cast<const uint16_t*>(at));
             acc += (double)dot[0] * ((double)q.scales[2 * b] * (double)e4m3_value(two & 255u));
             acc += (double)dot[1] * ((double)q.scales[2 * b + 1] * (double)e4m3_value(two >> 8));
         }
@@ -910,56 +945,81 @@ __device__ __forceinline__ uint64_t row_key(double dot, float g, float gq, int64
     return ((uint64_t)ordered(s) << 32) | (uint32_t)~(uint32_t)row;
 }
 
-// The k best rows of one query per CTA.
-template <int FMT>
-__global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
+template <int FMT, int NT>
+__device__ __forceinline__ void load_query(const FinishParams& p, const QueryShared& q, int64_t qs) {
+    const uint16_t* codes = reinterpret_cast<const uint16_t*>(p.q_codes + qs * (p.dp / 2));
+    for (int i = threadIdx.x; i < p.dp / 4; i += NT)
+        reinterpret_cast<uint32_t*>(q.codes)[i] = e2m1x4_bytes(__ldcg(codes + i));
+    for (int b = threadIdx.x; b < p.dp / block_of(FMT); b += NT)
+        q.scales[b] = scale_value<FMT>(__ldcg(p.q_scales + scale_word(qs, b >> 2, p.atoms) + (b & 3)));
+}
+
+template <int NT>
+__device__ __forceinline__ void write_best(const FinishParams& p, int t, const uint64_t* key,
+                                           int found) {
+    for (int j = threadIdx.x; j < p.k; j += NT) {
+        const uint64_t x = j < found ? key[j] : 0;
+        p.out_ids[(int64_t)t * p.k + j] =
+            x ? (int32_t)(p.id_base + (int64_t)(uint32_t)~(uint32_t)x) : -1;
+        p.out_scores[(int64_t)t * p.k + j] = x ? unordered((uint32_t)(x >> 32)) : -INFINITY;
+    }
+}
+
+// The k best rows of one query per CTA: its candidates whose approximate score can be among
+// the k best are scored exactly and sorted.  A query with more than LIST of those, or whose
+// candidates overflowed, is left to rescue_kernel.
+template <int FMT, int NT>
+__global__ void __launch_bounds__(NT) finish_kernel(const FinishParams p) {
     __shared__ __align__(16) uint64_t key[LIST];
-    __shared__ int s_warp[SEL / 32];
+    __shared__ int s_warp[NT / 32];
     __shared__ int s_n;
     extern __shared__ __align__(16) uint8_t dyn[];  // query bytes [dp], scales [dp / block]
+    griddep_launch();
+    griddep_wait();
     const int t = blockIdx.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int W = SEL / 32;
+    constexpr int W = NT / 32;
     const int64_t qs = query_slot(t, p.nt, p.nt_pad);
-    const float gq = p.q_scale[qs];
+    const float gq = __ldcg(p.q_scale + qs);
+    const int m = p.dense ? (int)p.n_rows : __ldcg(p.cand_n + t);
+    const float two_eps = 2.0f * eps_of(p.dp, __ldcg(p.q_norm + t), __ldcg(p.norm_max));
     QueryShared q;
     q.codes = reinterpret_cast<int8_t*>(dyn);
     q.scales = reinterpret_cast<float*>(dyn + p.dp);
+    if (threadIdx.x == 0) s_n = 0;
 
     int found = 0;
     if (gq > 0.0f) {
-        for (int i = threadIdx.x; i < p.dp / 4; i += SEL)
-            reinterpret_cast<uint32_t*>(q.codes)[i] = e2m1x4_bytes(
-                reinterpret_cast<const uint16_t*>(p.q_codes + qs * (p.dp / 2))[i]);
-        for (int b = threadIdx.x; b < p.dp / block_of(FMT); b += SEL)
-            q.scales[b] = scale_value<FMT>(p.q_scales[scale_word(qs, b >> 2, p.atoms) + (b & 3)]);
-        if (threadIdx.x == 0) s_n = 0;
-        __syncthreads();
-        const float two_eps = 2.0f * eps_of(p.dp, p.q_norm[t], *p.norm_max);
-        const float* dense = p.dense ? p.dense + (int64_t)t * p.ld : nullptr;
-        const uint64_t* cand = p.dense ? nullptr : p.cand + (int64_t)t * CAP;
-        const int m = p.dense ? (int)p.n_rows : p.cand_n[t];
         const bool known = two_eps < INFINITY;  // else any row may be among the best
         bool whole = !p.dense && (m > CAP || !known);
         if (!whole) {
+            const float* dense = p.dense + (int64_t)t * p.ld;
+            const uint64_t* cand = p.cand + (int64_t)t * CAP;
             auto approx = [&](int i) {
-                return dense ? dense[i] : __uint_as_float((uint32_t)(cand[i] >> 32));
+                return p.dense ? __ldcg(dense + i)
+                               : __uint_as_float((uint32_t)(__ldcg(cand + i) >> 32));
             };
             float cut = -INFINITY;
             if (m > p.k) {
                 const uint32_t o =
-                    kth_largest<8>(m, p.k, reinterpret_cast<uint32_t*>(key),
-                                   [&](int i) { return ordered_score(approx(i)); });
+                    kth_largest<NT, 8>(m, p.k, reinterpret_cast<uint32_t*>(key),
+                                       [&](int i) { return ordered_score(approx(i)); });
                 cut = o ? unordered(o) - two_eps : -INFINITY;
             }
+            load_query<FMT, NT>(p, q, qs);
             __syncthreads();
-            if (threadIdx.x == 0) s_n = 0;
-            __syncthreads();
-            for (int i = threadIdx.x; i < m; i += SEL) {
-                const float a = approx(i);
-                if (a >= cut || !known) {
-                    const int at = atomicAdd(&s_n, 1);
-                    if (at < LIST) key[at] = dense ? (uint64_t)i : (cand[i] & 0xFFFFFFFFu);
+            for (int i0 = threadIdx.x; i0 < m; i0 += 4 * NT) {
+                float a[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) a[u] = i0 + u * NT < m ? approx(i0 + u * NT) : -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int i = i0 + u * NT;
+                    if (i < m && (a[u] >= cut || !known)) {
+                        const int at = atomicAdd(&s_n, 1);
+                        if (at < LIST)
+                            key[at] = p.dense ? (uint64_t)i : (__ldcg(cand + i) & 0xFFFFFFFFu);
+                    }
                 }
             }
             __syncthreads();
@@ -967,51 +1027,27 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
             if (!whole) {
                 for (int i = warp; i < s_n; i += W) {
                     const int64_t row = (int64_t)key[i];
+                    const float g = __ldcg(p.row_scale + row);
                     const double dot = warp_dot<FMT>(p, q, row, lane);
-                    if (lane == 0) key[i] = row_key(dot, p.row_scale[row], gq, row);
+                    if (lane == 0) key[i] = row_key(dot, g, gq, row);
                 }
                 __syncthreads();
                 found = s_n;
-                sort_desc(key, found);
+                sort_desc<NT>(key, found);
             }
         }
         if (whole) {
-            // More rows than fit reach the threshold (many equal rows, a sample that missed
-            // the best ones, or norms past float32): every row exactly, keeping the rows that
-            // beat the k-th best so far.
-            if (threadIdx.x == 0) s_n = 0;
-            __syncthreads();
-            uint64_t floor_key = 0;
-            constexpr int BATCH = 512;
-            for (int64_t r0 = 0; r0 < p.n_rows; r0 += BATCH) {
-                for (int i = warp; i < BATCH; i += W) {
-                    const int64_t row = r0 + i;
-                    if (row >= p.n_rows) break;
-                    const float g = __ldg(&p.row_scale[row]);
-                    if (!(g == g)) continue;
-                    const double dot = warp_dot<FMT>(p, q, row, lane);
-                    const uint64_t x = row_key(dot, g, gq, row);
-                    if (lane == 0 && x > floor_key) key[atomicAdd(&s_n, 1)] = x;
-                }
-                __syncthreads();
-                const int have = s_n;
-                if (have > LIST - BATCH || r0 + BATCH >= p.n_rows) {
-                    sort_desc(key, have);
-                    found = min(have, p.k);
-                    floor_key = found == p.k ? key[p.k - 1] : 0;
-                    __syncthreads();
-                    if (threadIdx.x == 0) s_n = found;
-                }
-                __syncthreads();
+            if (threadIdx.x == 0) {
+                p.done[t] = 0;
+                p.flagged[atomicAdd(p.n_flagged, 1)] = t;
             }
+            return;
         }
     } else if (gq == 0.0f) {
         // Every row that holds anything scores 0: the first k of them.
-        if (threadIdx.x == 0) s_n = 0;
-        __syncthreads();
-        for (int64_t r0 = 0; r0 < p.n_rows && found < p.k; r0 += SEL) {
+        for (int64_t r0 = 0; r0 < p.n_rows && found < p.k; r0 += NT) {
             const int64_t row = r0 + threadIdx.x;
-            const float g = row < p.n_rows ? p.row_scale[row] : __int_as_float(0x7fc00000);
+            const float g = row < p.n_rows ? __ldcg(p.row_scale + row) : __int_as_float(0x7fc00000);
             const unsigned live = __ballot_sync(0xffffffffu, g == g);
             if (lane == 0) s_warp[warp] = __popc(live);
             __syncthreads();
@@ -1028,11 +1064,97 @@ __global__ void __launch_bounds__(SEL) finish_kernel(FinishParams p) {
         }
     }
     __syncthreads();
-    for (int j = threadIdx.x; j < p.k; j += SEL) {
-        const uint64_t x = j < found ? key[j] : 0;
-        p.out_ids[(int64_t)t * p.k + j] =
-            x ? (int32_t)(p.id_base + (int64_t)(uint32_t)~(uint32_t)x) : -1;
-        p.out_scores[(int64_t)t * p.k + j] = x ? unordered((uint32_t)(x >> 32)) : -INFINITY;
+    write_best<NT>(p, t, key, found);
+}
+
+// The k best of a stream of keys, by a CTA: offered keys above the k-th best so far are kept
+// until the list is nearly full, then the k best of them.
+template <int NT>
+struct BestKeys {
+    static constexpr int BATCH = 512;  // offered at most between two calls of settle()
+    uint64_t* key;                     // [LIST], shared
+    int* n;                            // shared, 0 at first
+    uint64_t floor;
+    __device__ __forceinline__ void offer(uint64_t x) {  // by any thread
+        if (x > floor) key[atomicAdd(n, 1)] = x;
+    }
+    __device__ __forceinline__ int settle(int k, bool last) {  // by all threads
+        __syncthreads();
+        int have = *n;
+        if (have > LIST - BATCH || last) {
+            sort_desc<NT>(key, have);
+            have = min(have, k);
+            floor = have == k ? key[k - 1] : 0;
+            __syncthreads();
+            if (threadIdx.x == 0) *n = have;
+        }
+        __syncthreads();
+        return have;
+    }
+};
+
+// Flagged queries (many rows that tie with the k-th best, a sample that missed the best rows, or
+// norms whose products leave float32): every row, exactly.  Each query's rows are split
+// between as many CTAs as the grid has to spare; the last one to finish merges the parts.
+constexpr int RESCUE_CTAS = 296;
+template <int FMT>
+__global__ void __launch_bounds__(SEL) rescue_kernel(const FinishParams p) {
+    __shared__ __align__(16) uint64_t key[LIST];
+    __shared__ int s_n;
+    __shared__ int s_last;
+    extern __shared__ __align__(16) uint8_t dyn[];
+    griddep_launch();
+    griddep_wait();
+    const int flagged = __ldcg(p.n_flagged);
+    if (flagged == 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int W = SEL / 32;
+    QueryShared q;
+    q.codes = reinterpret_cast<int8_t*>(dyn);
+    q.scales = reinterpret_cast<float*>(dyn + p.dp);
+    const int splits = max(1, RESCUE_CTAS / flagged);
+    for (int item = blockIdx.x; item < flagged * splits; item += gridDim.x) {
+        const int t = p.flagged[item / splits];
+        const int part = item % splits;
+        const int64_t qs = query_slot(t, p.nt, p.nt_pad);
+        const float gq = __ldcg(p.q_scale + qs);
+        const int64_t begin = p.n_rows * part / splits, end = p.n_rows * (part + 1) / splits;
+        load_query<FMT, SEL>(p, q, qs);
+        if (threadIdx.x == 0) s_n = 0;
+        __syncthreads();
+        BestKeys<SEL> best = {key, &s_n, 0};
+        int found = begin < end ? 0 : best.settle(p.k, true);
+        for (int64_t r0 = begin; r0 < end; r0 += BestKeys<SEL>::BATCH) {
+            for (int i = warp; i < BestKeys<SEL>::BATCH && r0 + i < end; i += W) {
+                const int64_t row = r0 + i;
+                const float g = __ldcg(p.row_scale + row);
+                if (!(g == g)) continue;
+                const double dot = warp_dot<FMT>(p, q, row, lane);
+                if (lane == 0) best.offer(row_key(dot, g, gq, row));
+            }
+            found = best.settle(p.k, r0 + BestKeys<SEL>::BATCH >= end);
+        }
+        uint64_t* out = p.parts + (int64_t)item * p.k;
+        for (int j = threadIdx.x; j < p.k; j += SEL) out[j] = j < found ? key[j] : 0;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) s_last = atomicAdd(&p.done[t], 1) == splits - 1;
+        __syncthreads();
+        if (s_last) {
+            __threadfence();
+            if (threadIdx.x == 0) s_n = 0;
+            __syncthreads();
+            BestKeys<SEL> all = {key, &s_n, 0};
+            const int64_t n = (int64_t)splits * p.k;
+            const uint64_t* in = p.parts + (int64_t)(item - part) * p.k;
+            for (int64_t r0 = 0; r0 < n; r0 += BestKeys<SEL>::BATCH) {
+                for (int64_t i = r0 + threadIdx.x; i < r0 + BestKeys<SEL>::BATCH && i < n; i += SEL)
+                    all.offer(__ldcg(in + i));
+                found = all.settle(p.k, r0 + BestKeys<SEL>::BATCH >= n);
+            }
+            write_best<SEL>(p, t, key, found);
+        }
+        __syncthreads();
     }
 }
 
@@ -1160,11 +1282,8 @@ int launch_fp4_product(const Fp4Product& L, cudaStream_t st) {
     const bool mx = L.format == kMX;
     const void* fn = mx ? (const void*)fp4_tc_kernel<kMX> : (const void*)fp4_tc_kernel<kNV>;
     if (set_smem_limit(fn, s.smem) != 0) return PION_B200_ECUDA;
-    if (mx)
-        fp4_tc_kernel<kMX><<<grid, THREADS, s.smem, st>>>(rows, row_sf, q, q_sf, p, mode);
-    else
-        fp4_tc_kernel<kNV><<<grid, THREADS, s.smem, st>>>(rows, row_sf, q, q_sf, p, mode);
-    return cudaGetLastError() == cudaSuccess ? 0 : PION_B200_ECUDA;
+    return mx ? launch_pdl(fp4_tc_kernel<kMX>, grid, THREADS, s.smem, st, rows, row_sf, q, q_sf, p, mode)
+              : launch_pdl(fp4_tc_kernel<kNV>, grid, THREADS, s.smem, st, rows, row_sf, q, q_sf, p, mode);
 }
 
 int fp4_sample_tiles(int nq) { return nq <= 64 ? 64 : 32; }
@@ -1174,20 +1293,20 @@ int launch_fp4_theta(const float* sample, const uint64_t* cand, int k, int dim,
                      const float* norm_max, int nq, float* theta, int* cand_n, cudaStream_t st) {
     using namespace fp4;
     const int dp = pad_dim(dim);
-    if (cand) {
-        theta_kernel<<<(unsigned)nq, SEL, 0, st>>>(cand, k, dp, q_scale, nt, nt_pad, q_norm,
-                                                   norm_max, theta, cand_n);
-    } else if (fp4_sample_tiles(nq) == 64) {
+    if (cand)
+        return launch_pdl(theta_kernel, dim3((unsigned)nq), SEL, 0, st, cand, k, dp, q_scale, nt,
+                          nt_pad, q_norm, norm_max, theta, cand_n);
+    if (fp4_sample_tiles(nq) == 64) {
         static_assert(64 * ROWS == 1024 * 4 * 4, "sample");
-        theta_sample_kernel<1024, 4><<<(unsigned)nq, 1024, 0, st>>>(
-            sample, k, dp, q_scale, nt, nt_pad, q_norm, norm_max, theta, cand_n);
-    } else {
-        static_assert(32 * ROWS == 256 * 8 * 4, "sample");
-        theta_sample_kernel<256, 8><<<(unsigned)nq, 256, 0, st>>>(
-            sample, k, dp, q_scale, nt, nt_pad, q_norm, norm_max, theta, cand_n);
+        return launch_pdl(theta_sample_kernel<1024, 4>, dim3((unsigned)nq), 1024, 0, st, sample, k, dp,
+                          q_scale, nt, nt_pad, q_norm, norm_max, theta, cand_n);
     }
-    return cudaGetLastError() == cudaSuccess ? 0 : PION_B200_ECUDA;
+    static_assert(32 * ROWS == 256 * 8 * 4, "sample");
+    return launch_pdl(theta_sample_kernel<256, 8>, dim3((unsigned)nq), 256, 0, st, sample, k, dp,
+                      q_scale, nt, nt_pad, q_norm, norm_max, theta, cand_n);
 }
+
+int64_t fp4_rescue_items(int64_t nq) { return nq > fp4::RESCUE_CTAS ? nq : fp4::RESCUE_CTAS; }
 
 int launch_fp4_finish(const Fp4Finish& L, cudaStream_t st) {
     using namespace fp4;
@@ -1213,12 +1332,25 @@ int launch_fp4_finish(const Fp4Finish& L, cudaStream_t st) {
     p.cand = L.cand;
     p.out_ids = L.out_ids;
     p.out_scores = L.out_scores;
+    p.nq = L.nq;
+    p.n_flagged = L.n_flagged;
+    p.flagged = L.flagged;
+    p.done = L.done;
+    p.parts = L.parts;
     const int smem = p.dp + p.dp / block_of(L.format) * 4;
-    if (L.format == kMX)
-        finish_kernel<kMX><<<(unsigned)L.nq, SEL, smem, st>>>(p);
+    const dim3 grid((unsigned)L.nq);
+    // Few queries: a CTA of 32 warps each, so that the dozen rows scored exactly are one round.
+    const bool mx = L.format == kMX, few = L.nq <= 148;
+    int rc;
+    if (few)
+        rc = mx ? launch_pdl(finish_kernel<kMX, 1024>, grid, 1024, smem, st, p)
+                : launch_pdl(finish_kernel<kNV, 1024>, grid, 1024, smem, st, p);
     else
-        finish_kernel<kNV><<<(unsigned)L.nq, SEL, smem, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? 0 : PION_B200_ECUDA;
+        rc = mx ? launch_pdl(finish_kernel<kMX, SEL>, grid, SEL, smem, st, p)
+                : launch_pdl(finish_kernel<kNV, SEL>, grid, SEL, smem, st, p);
+    if (rc != 0) return rc;
+    return mx ? launch_pdl(rescue_kernel<kMX>, dim3(RESCUE_CTAS), SEL, smem, st, p)
+              : launch_pdl(rescue_kernel<kNV>, dim3(RESCUE_CTAS), SEL, smem, st, p);
 }
 
 }  // namespace pion

@@ -39,6 +39,34 @@ __host__ __device__ __forceinline__ int64_t query_slot(int64_t t, int tile, int 
     return t / tile * tile_pad + t % tile;
 }
 
+// -------------------------------------------------- overlapped launches --
+// The kernels of a call are launched with programmatic stream serialisation: a kernel may
+// start while the one before it still runs, and waits for it, and for its memory, before it
+// reads or writes anything.  What they read they read through L2 (never ld.global.nc): lines
+// that an earlier kernel left in an SM's L1 may be older than what is waited for.
+__device__ __forceinline__ void griddep_wait() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void griddep_launch() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <class... P, class... A>
+inline int launch_pdl(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st,
+                      const A&... args) {
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess ? 0 : PION_B200_ECUDA;
+}
+
 // ------------------------------------------------------------ conversions --
 // Eight floats -> eight e2m1 codes (nearest, ties to even, saturating), element 0 lowest.
 __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {

@@ -21,10 +21,10 @@
 namespace pion {
 namespace fp4 {
 
-constexpr int WARPS = 8;  // rows in flight per CTA, a warp each
-constexpr int STEP = 256; // elements per warp step, eight consecutive ones per lane
+constexpr int WARPS = 8;   // per CTA
+constexpr int STEP = 256;  // elements per warp step, eight consecutive ones per lane
 
-// amax below this is stored as a row of zeros: g = amax / 2688 and its multiples then stay
+// In NV an amax below this is stored as a row of zeros: g = amax / 2688 and its multiples then stay
 // normal numbers.
 __device__ constexpr float kTiny = 0x1p-100f;
 
@@ -46,37 +46,70 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// Eight consecutive elements from column c of a row, zeros past dim.  VEC: the row starts at
-// a 16-byte boundary.
+// Eight consecutive elements from column c = c0 + 8 * lane of a row, zeros past dim.  VEC: rows
+// start at 16-byte boundaries; else the warp's 256 elements come in one by one, side by side,
+// and pass through shared memory.
 template <class T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int c, int dim, float (&v)[8]) {
-    if (VEC && c + 8 <= dim) {
-        constexpr int N = 8 * sizeof(T) / 16;
-        alignas(16) uint4 raw[N];
+__device__ __forceinline__ void load8(const T* row, int c0, int dim, int lane, T* stage,
+                                      float (&v)[8]) {
+    const int c = c0 + 8 * lane;
+    if constexpr (VEC) {
+        if (c + 8 <= dim) {
+            constexpr int N = 8 * sizeof(T) / 16;
+            alignas(16) uint4 raw[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) raw[j] = __ldg(reinterpret_cast<const uint4*>(row + c) + j);
-        const T* t = reinterpret_cast<const T*>(raw);
+            for (int j = 0; j < N; ++j) raw[j] = __ldcg(reinterpret_cast<const uint4*>(row + c) + j);
+            const T* t = reinterpret_cast<const T*>(raw);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(t[j]);
+            for (int j = 0; j < 8; ++j) v[j] = to_float<T>(t[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = c + j < dim ? to_float<T>(row[c + j]) : 0.0f;
+        }
     } else {
+        T x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < dim ? to_float<T>(row[c + j]) : 0.0f;
+        for (int j = 0; j < 8; ++j) {
+            const int e = c0 + 32 * j + lane;
+            x[j] = e < dim ? row[e] : from_float<T>(0.0f);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) stage[32 * j + lane] = x[j];
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(stage[8 * lane + j]);
     }
 }
 
-__device__ __forceinline__ float max8(const float (&v)[8]) {
-    float m = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+// The larger magnitude, NaN if either is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)));
     return m;
 }
+__device__ __forceinline__ float max8(const float (&v)[8]) {
+    return max_abs(max_abs(max_abs(v[0], v[1]), max_abs(v[2], v[3])),
+                   max_abs(max_abs(v[4], v[5]), max_abs(v[6], v[7])));
+}
 
-// The e4m3 byte nearest to top / h (top >= 0, h > 0, quotient at most 448 (1 + 2^-22)).
-__device__ __forceinline__ uint32_t e4m3_quotient(float top, float h) {
-    const float t = __fdividef(top, h);
-    const uint32_t lo = e4m3_byte(t * (1.0f - 0x1p-20f)), hi = e4m3_byte(t * (1.0f + 0x1p-20f));
+__device__ __forceinline__ float rcp_approx(float x) {  // within an ulp, x normal
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// The e4m3 byte nearest to top / h (top >= 0, h > 0, quotient at most 448 (1 + 2^-22)); rh is
+// 1 / h within 2^-22.
+__device__ __forceinline__ uint32_t e4m3_quotient(float top, float h, float rh) {
+    const float t = top * rh;
+    uint32_t two;  // the neighbours' bytes, the lower one first
+    asm("{\n\t.reg .b16 t;\n\tcvt.rn.satfinite.e4m3x2.f32 t, %2, %1;\n\tcvt.u32.u16 %0, t;\n\t}"
+        : "=r"(two)
+        : "f"(t * (1.0f - 0x1p-20f)), "f"(t * (1.0f + 0x1p-20f)));
+    const uint32_t lo = two & 0xFFu, hi = two >> 8;
     if (lo == hi) return lo;
-    // neighbours: compare top with the exact border (5 significant bits) times h
+    // compare top with the exact border (5 significant bits) times h
     const double mid = 0.5 * ((double)e4m3_value(lo) + (double)e4m3_value(hi)) * (double)h;
     if ((double)top == mid) return (lo & 1u) ? hi : lo;
     return (double)top > mid ? hi : lo;
@@ -97,7 +130,7 @@ __device__ __noinline__ uint32_t e2m1_exact(float x, float d) {
     return c | (x < 0.0f ? 8u : 0u);
 }
 
-// Eight codes of v / d; rd = 1 / d rounded (0 for d = 0).
+// Eight codes of v / d; rd is 1 / d, in MX exactly, in NV within 2^-22 (0 for d = 0).
 template <int FMT>
 __device__ __forceinline__ uint32_t codes8(const float (&v)[8], float d, float rd) {
     float a[8];
@@ -136,13 +169,15 @@ struct WriteParams {
     float* row_scale;
     float* norm;           // per row (queries), or null
     float* norm_max;       // the store's bound, or null
-    int* status;
+    int* zero;             // set to 0, or null
 };
 
 // A slot named by several rows of one write keeps the last of them: every row raises the
 // slot's claim to its index, and the write kernel takes only the row that holds it.
-__global__ void claim_kernel(const int64_t* __restrict__ slots, int64_t n, int64_t n_slots,
+__global__ void claim_kernel(const int64_t* slots, int64_t n, int64_t n_slots,
                              int32_t* claim, int* status) {
+    griddep_launch();
+    griddep_wait();
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
     const int64_t s = slots[i];
@@ -150,78 +185,74 @@ __global__ void claim_kernel(const int64_t* __restrict__ slots, int64_t n, int64
     if (s >= 0 && s < n_slots) atomicMax(&claim[s], (int32_t)(i + 1));
 }
 
-// One warp per row.  Bound by HBM: the row once (the NV format's second pass finds it in L1),
-// its codes, scales and g once.
-template <int FMT, class T, bool VEC>
-__global__ void __launch_bounds__(WARPS * 32) write_kernel(WriteParams p) {
-    const int lane = threadIdx.x & 31;
-    const int64_t i = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+// WPR warps per row: one where rows are many, the CTA's eight where they are few and a row's
+// own latency counts.  An MX row is one pass.  NV needs the row's largest magnitude first; its
+// elements stay in registers between the two passes where a warp's share is at most HOLD
+// steps (HOLD = 0: they are read again).  Bound by HBM: the row, its codes, scales and g once.
+template <int FMT, class T, bool VEC, int WPR, int HOLD>
+__global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) {
+    __shared__ __align__(16) T stage_all[VEC ? 1 : WARPS * STEP];
+    __shared__ float s_max[WARPS];
+    __shared__ float s_s2[WARPS];
+    griddep_launch();
+    griddep_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T* stage = stage_all + (VEC ? 0 : warp * STEP);
+    const int64_t i = WPR == 1 ? (int64_t)blockIdx.x * WARPS + warp : blockIdx.x;
     if (i >= p.n) return;
+    if (p.zero && i == 0 && threadIdx.x == 0) *p.zero = 0;
     int64_t slot;
     if (p.tile > 0) {
         slot = query_slot(i, p.tile, p.tile_pad);
     } else if (p.slots) {
-        slot = p.slots[i];
+        slot = __ldcg(p.slots + i);
         if (slot < 0 || slot >= p.n_slots) return;
-        if (*(volatile int32_t*)&p.claim[slot] != (int32_t)(i + 1)) return;
+        if (__ldcg(p.claim + slot) != (int32_t)(i + 1)) return;
     } else {
         slot = p.start + i;
     }
     const T* row = static_cast<const T*>(p.src) + i * p.stride;
     const int atoms = atoms_of(FMT, p.dp);
     constexpr int BL = block_of(FMT) / 8;  // lanes per block
-
-    float amax = 0.0f;
-    bool fine = true;  // no NaN or infinity in the row
-    for (int c = lane * 8; c < p.dp; c += STEP) {
-        float v[8];
-        load8<T, VEC>(row, c, p.dim, v);
-        float z = 0.0f;  // 0 * NaN and 0 * inf are NaN
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z = fmaf(v[j], 0.0f, z);
-        fine = fine && z == 0.0f;
-        amax = fmaxf(amax, max8(v));
-    }
-    fine = __all_sync(0xffffffffu, fine);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const bool live = fine && (FMT == kMX ? amax > 0.0f : amax >= kTiny);
-    float g = 0.0f, h = 1.0f;
-    if (live) {
-        g = FMT == kMX ? 1.0f : __fdiv_rn(amax, 2688.0f);
-        h = __fmul_rn(6.0f, g);
-    }
-
-    float s2 = 0.0f;  // sum of the blocks' squared scales
     const int steps = (p.dp + STEP - 1) / STEP;
-    for (int k = 0; k < steps; ++k) {
+    const int first = WPR == 1 ? 0 : warp;
+    uint32_t* codes_out = reinterpret_cast<uint32_t*>(p.codes + slot * (p.dp / 2));
+
+    float amax = 0.0f;  // of this warp's elements, then of the row: NaN and infinities show
+    float s2 = 0.0f;    // sum of the blocks' squared scales, BL times over
+    float g = 1.0f, h = 1.0f, rh = 1.0f;
+    bool live = true;
+    auto row_max = [&]() {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) amax = max_abs(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if constexpr (WPR > 1) {
+            if (lane == 0) s_max[warp] = amax;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < WPR; ++w) amax = max_abs(amax, s_max[w]);
+        }
+    };
+    auto quantise = [&](int k, const float(&v)[8], float top) {
         const int c = k * STEP + lane * 8;
-        float v[8];
-        load8<T, VEC>(row, c, p.dim, v);
-        float top = max8(v);
 #pragma unroll
         for (int o = 1; o < BL; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         uint32_t bits = 0, codes = 0;
-        if (live) {
-            float d, rd;
-            if (FMT == kMX) {
-                // floor(log2 top) - 2 as a biased exponent, at least the format's least
-                const int e = (int)(__float_as_uint(top) >> 23) - 2;
-                bits = (uint32_t)(e < 0 ? 0 : e);
-                d = e8m0_value(bits);
-                rd = __uint_as_float((254u - bits) << 23);  // 2^(127 - bits), bits <= 252
-                s2 = fmaf(d, d, s2);
-            } else {
-                bits = e4m3_quotient(top, h);
-                const float s = e4m3_value(bits);
-                d = __fmul_rn(s, g);
-                rd = bits ? __frcp_rn(d) : 0.0f;
-                s2 = fmaf(s, s, s2);
-            }
-            codes = codes8<FMT>(v, d, rd);
+        if (FMT == kMX) {
+            // floor(log2 top) - 2 as a biased exponent, at least the format's least (at most
+            // 252, infinities aside)
+            const int e = (int)(__float_as_uint(top) >> 23) - 2;
+            bits = (uint32_t)min(max(e, 0), 252);
+            const float d = e8m0_value(bits);
+            s2 = fmaf(d, d, s2);
+            codes = codes8<FMT>(v, d, __uint_as_float((254u - bits) << 23));  // 2^(127 - bits)
+        } else if (live) {
+            bits = e4m3_quotient(top, h, rh);
+            const float s = e4m3_value(bits);
+            const float d = __fmul_rn(s, g);
+            s2 = fmaf(s, s, s2);
+            codes = codes8<FMT>(v, d, bits ? rcp_approx(d) : 0.0f);
         }
-        if (c < p.dp)
-            reinterpret_cast<uint32_t*>(p.codes + slot * (p.dp / 2))[c >> 3] = codes;
+        if (c < p.dp) codes_out[c >> 3] = codes;
         // four blocks' bytes to the first lane of their atom
         uint32_t word = bits << (8 * ((lane / BL) & 3));
 #pragma unroll
@@ -229,17 +260,76 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(WriteParams p) {
         if (c < p.dp && lane % (4 * BL) == 0)
             *reinterpret_cast<uint32_t*>(p.scales +
                                          scale_word(slot, c / (32 * BL), atoms)) = word;
+    };
+    if constexpr (FMT == kMX) {
+        // four steps' loads in flight
+        for (int k0 = first; k0 < steps; k0 += 4 * WPR) {
+            float v[4][8];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (k0 + u * WPR < steps)
+                    load8<T, VEC>(row, (k0 + u * WPR) * STEP, p.dim, lane, stage, v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (k0 + u * WPR < steps) {
+                    const float top = max8(v[u]);
+                    amax = max_abs(amax, top);
+                    quantise(k0 + u * WPR, v[u], top);
+                }
+        }
+        row_max();
+        if (amax == 0.0f) g = 0.0f;
+    } else {
+        constexpr int H = HOLD > 0 ? HOLD : 1;
+        float v[H][8], top[H];
+        if constexpr (HOLD > 0) {
+#pragma unroll
+            for (int u = 0; u < H; ++u)
+                if (first + u * WPR < steps)
+                    load8<T, VEC>(row, (first + u * WPR) * STEP, p.dim, lane, stage, v[u]);
+#pragma unroll
+            for (int u = 0; u < H; ++u)
+                if (first + u * WPR < steps) amax = max_abs(amax, top[u] = max8(v[u]));
+        } else {
+            for (int k = first; k < steps; k += WPR) {
+                load8<T, VEC>(row, k * STEP, p.dim, lane, stage, v[0]);
+                amax = max_abs(amax, max8(v[0]));
+            }
+        }
+        row_max();
+        live = amax >= kTiny && amax < INFINITY;
+        g = live ? __fdiv_rn(amax, 2688.0f) : 0.0f;
+        h = live ? __fmul_rn(6.0f, g) : 1.0f;
+        rh = rcp_approx(h);
+        if constexpr (HOLD > 0) {
+#pragma unroll
+            for (int u = 0; u < H; ++u)
+                if (first + u * WPR < steps) quantise(first + u * WPR, v[u], top[u]);
+        } else {
+            for (int k = first; k < steps; k += WPR) {
+                load8<T, VEC>(row, k * STEP, p.dim, lane, stage, v[0]);
+                quantise(k, v[0], max8(v[0]));
+            }
+        }
     }
+    const bool fine = amax < INFINITY;
 #pragma unroll
     for (int o = 16; o; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+    if constexpr (WPR > 1) {
+        if (lane == 0) s_s2[warp] = s2;
+        __syncthreads();
+        if (warp != 0) return;
+        s2 = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) s2 += s_s2[w];
+    }
     if (lane == 0) {
         p.row_scale[slot] = fine ? g : __int_as_float(0x7fc00000);
-        // every element is at most 6 s g: |row| <= 6 g sqrt(block * sum s^2).  Every lane of
-        // a block added its scale, BL times in all.
+        // every element is at most 6 s g: |row| <= 6 g sqrt(block * sum s^2)
         const float bound =
             fine ? 6.02f * g * sqrtf((float)(block_of(FMT) / BL) * s2) : 0.0f;
         if (p.norm) p.norm[i] = bound;
-        if (p.norm_max && bound > *(volatile float*)p.norm_max)
+        if (p.norm_max && bound > __ldcg(p.norm_max))
             atomicMax(reinterpret_cast<int*>(p.norm_max), __float_as_int(bound));
         if (p.slots) p.claim[slot] = 0;
     }
@@ -259,64 +349,96 @@ struct ReadParams {
     int* status;
 };
 
+// One warp per row.  Bound by HBM: the output once.
 template <int FMT, class T, bool VEC>
-__global__ void __launch_bounds__(WARPS * 32) read_kernel(ReadParams p) {
-    const int lane = threadIdx.x & 31;
-    const int64_t i = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(WARPS * 32) read_kernel(const ReadParams p) {
+    __shared__ __align__(16) T stage_all[VEC ? 1 : WARPS * STEP];
+    griddep_launch();
+    griddep_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    T* stage = stage_all + (VEC ? 0 : warp * STEP);
+    const int64_t i = (int64_t)blockIdx.x * WARPS + warp;
     if (i >= p.n) return;
-    const int64_t slot = p.slots ? p.slots[i] : p.start + i;
+    const int64_t slot = p.slots ? __ldcg(p.slots + i) : p.start + i;
     if (slot < 0) return;
     if (slot >= p.n_slots) {
         if (lane == 0) record_error(p.status, PION_B200_EINVAL);
         return;
     }
-    const float g = __ldg(&p.row_scale[slot]);
+    const float g = __ldcg(&p.row_scale[slot]);
     const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.codes + slot * (p.dp / 2));
     const int atoms = atoms_of(FMT, p.dp);
     T* out = static_cast<T*>(p.dst) + i * p.stride;
-    for (int c = lane * 8; c < p.dim; c += STEP) {
-        float v[8];
-        e2m1x8_values(__ldg(codes + (c >> 3)), v);
+#pragma unroll 4
+    for (int c0 = 0; c0 < p.dim; c0 += STEP) {
+        const int c = c0 + 8 * lane;
+        const bool in = c < p.dp;
         const int b = c / block_of(FMT);
-        const float s = scale_value<FMT>(__ldg(p.scales + scale_word(slot, b >> 2, atoms) + (b & 3)));
+        const uint32_t packed = in ? __ldcg(codes + (c >> 3)) : 0u;
+        const uint32_t byte =
+            in ? __ldcg(p.scales + scale_word(slot, b >> 2, atoms) + (b & 3)) : 0u;
+        float v[8];
+        e2m1x8_values(packed, v);
+        const float s = scale_value<FMT>(byte);
         // code * s has at most six significant bits: one rounding in the product with g (and
         // one to a 16-bit output, from a value already within 2^-24)
         alignas(16) T t[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) t[j] = from_float<T>(__fmul_rn(__fmul_rn(v[j], s), g));
-        if (VEC && c + 8 <= p.dim) {
-            constexpr int N = 8 * sizeof(T) / 16;
+        if constexpr (VEC) {
+            if (c + 8 <= p.dim) {
+                constexpr int N = 8 * sizeof(T) / 16;
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                reinterpret_cast<uint4*>(out + c)[j] = reinterpret_cast<const uint4*>(t)[j];
+                for (int j = 0; j < N; ++j)
+                    reinterpret_cast<uint4*>(out + c)[j] = reinterpret_cast<const uint4*>(t)[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (c + j < p.dim) out[c + j] = t[j];
+            }
         } else {
+            // side by side through shared memory: eight strided elements a lane took 3.5 times
+            // as long
+            __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c + j < p.dim) out[c + j] = t[j];
+            for (int j = 0; j < 8; ++j) stage[8 * lane + j] = t[j];
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int e = 32 * j + lane;
+                if (c0 + e < p.dim) out[c0 + e] = stage[e];
+            }
         }
     }
 }
 
+template <int FMT, class T, bool VEC>
+static int write_v(const WriteParams& p, cudaStream_t st) {
+    // Few rows: a CTA each; many: a warp each.
+    if (p.n <= 1024)
+        return launch_pdl(write_kernel<FMT, T, VEC, WARPS, 4>, dim3((unsigned)p.n), WARPS * 32, 0,
+                          st, p);
+    const dim3 grid((unsigned)((p.n + WARPS - 1) / WARPS));
+    if constexpr (FMT == kNV) {
+        if (p.dp <= 4 * STEP) return launch_pdl(write_kernel<FMT, T, VEC, 1, 4>, grid, WARPS * 32, 0, st, p);
+        if (p.dp <= 8 * STEP) return launch_pdl(write_kernel<FMT, T, VEC, 1, 8>, grid, WARPS * 32, 0, st, p);
+    }
+    return launch_pdl(write_kernel<FMT, T, VEC, 1, 0>, grid, WARPS * 32, 0, st, p);
+}
+
 template <int FMT, class T>
 static int write_t(const WriteParams& p, cudaStream_t st) {
+    static_assert(kMaxDim <= WARPS * 4 * STEP, "a CTA holds a row");
     const bool vec = reinterpret_cast<uintptr_t>(p.src) % 16 == 0 && p.stride * sizeof(T) % 16 == 0;
-    const dim3 grid((unsigned)((p.n + WARPS - 1) / WARPS));
-    if (vec)
-        write_kernel<FMT, T, true><<<grid, WARPS * 32, 0, st>>>(p);
-    else
-        write_kernel<FMT, T, false><<<grid, WARPS * 32, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? 0 : PION_B200_ECUDA;
+    return vec ? write_v<FMT, T, true>(p, st) : write_v<FMT, T, false>(p, st);
 }
 
 template <int FMT, class T>
 static int read_t(const ReadParams& p, cudaStream_t st) {
     const bool vec = reinterpret_cast<uintptr_t>(p.dst) % 16 == 0 && p.stride * sizeof(T) % 16 == 0;
     const dim3 grid((unsigned)((p.n + WARPS - 1) / WARPS));
-    if (vec)
-        read_kernel<FMT, T, true><<<grid, WARPS * 32, 0, st>>>(p);
-    else
-        read_kernel<FMT, T, false><<<grid, WARPS * 32, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? 0 : PION_B200_ECUDA;
+    return vec ? launch_pdl(read_kernel<FMT, T, true>, grid, WARPS * 32, 0, st, p)
+               : launch_pdl(read_kernel<FMT, T, false>, grid, WARPS * 32, 0, st, p);
 }
 
 }  // namespace fp4
@@ -325,9 +447,9 @@ int launch_fp4_write(const Fp4Write& w, cudaStream_t st) {
     using namespace fp4;
     if (w.n <= 0) return 0;
     if (w.slots) {
-        claim_kernel<<<(unsigned)((w.n + 255) / 256), 256, 0, st>>>(w.slots, w.n, w.n_slots,
-                                                                    w.claim, w.status);
-        if (cudaGetLastError() != cudaSuccess) return PION_B200_ECUDA;
+        if (launch_pdl(claim_kernel, dim3((unsigned)((w.n + 255) / 256)), 256, 0, st, w.slots, w.n,
+                       w.n_slots, w.claim, w.status) != 0)
+            return PION_B200_ECUDA;
     }
     WriteParams p;
     p.src = w.src;
@@ -346,7 +468,7 @@ int launch_fp4_write(const Fp4Write& w, cudaStream_t st) {
     p.row_scale = w.row_scale;
     p.norm = w.norm;
     p.norm_max = w.norm_max;
-    p.status = w.status;
+    p.zero = w.zero;
     const bool mx = w.format == kMX;
     switch (w.type) {
         case PION_B200_F32: return mx ? write_t<kMX, float>(p, st) : write_t<kNV, float>(p, st);

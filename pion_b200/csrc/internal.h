@@ -480,6 +480,7 @@ struct Fp4Write {
     float* row_scale = nullptr;
     float* norm = nullptr;
     float* norm_max = nullptr;
+    int* zero = nullptr;         // an integer that the first kernel sets to 0
     int* status = nullptr;
 };
 int launch_fp4_write(const Fp4Write& w, cudaStream_t st);
@@ -559,9 +560,14 @@ struct Fp4Finish {
     int64_t ld = 0;
     const int* cand_n = nullptr;
     const uint64_t* cand = nullptr;
+    int* n_flagged = nullptr;  // 0 before the call; queries that take the exact scan
+    int* flagged = nullptr;    // [nq]
+    int* done = nullptr;       // [nq]
+    uint64_t* parts = nullptr; // [fp4_rescue_items(nq)][k]
     int32_t* out_ids = nullptr;
     float* out_scores = nullptr;
 };
+int64_t fp4_rescue_items(int64_t nq);
 int launch_fp4_finish(const Fp4Finish& L, cudaStream_t st);
 
 // ---- bq.cu
