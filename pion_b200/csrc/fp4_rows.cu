@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "fp4.cuh"
 #include "internal.h"
@@ -46,51 +47,88 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// Eight consecutive elements from column c = c0 + 8 * lane of a row, zeros past dim.  VEC: rows
-// start at 16-byte boundaries; else the warp's 256 elements come in one by one, side by side,
-// and pass through shared memory.
-template <class T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int c0, int dim, int lane, T* stage,
-                                      float (&v)[8]) {
-    const int c = c0 + 8 * lane;
-    if constexpr (VEC) {
-        if (c + 8 <= dim) {
-            constexpr int N = 8 * sizeof(T) / 16;
-            alignas(16) uint4 raw[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) raw[j] = __ldcg(reinterpret_cast<const uint4*>(row + c) + j);
-            const T* t = reinterpret_cast<const T*>(raw);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = to_float<T>(t[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c + j < dim ? to_float<T>(row[c + j]) : 0.0f;
-        }
-    } else {
-        T x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int e = c0 + 32 * j + lane;
-            x[j] = e < dim ? row[e] : from_float<T>(0.0f);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) stage[32 * j + lane] = x[j];
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(stage[8 * lane + j]);
-    }
-}
-
 // The larger magnitude, NaN if either is.
 __device__ __forceinline__ float max_abs(float a, float b) {
     float m;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)));
     return m;
 }
-__device__ __forceinline__ float max8(const float (&v)[8]) {
-    return max_abs(max_abs(max_abs(v[0], v[1]), max_abs(v[2], v[3])),
-                   max_abs(max_abs(v[4], v[5]), max_abs(v[6], v[7])));
+
+// Eight consecutive elements as they are in memory, their values and their largest magnitude
+// (NaN if one is).
+template <class T>
+struct alignas(16) Eight {
+    T x[8];
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) {
+                v[2 * j] = (float)x[2 * j];
+                v[2 * j + 1] = (float)x[2 * j + 1];
+            } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(w + j));
+                v[2 * j] = f.x;
+                v[2 * j + 1] = f.y;
+            }
+        }
+    }
+    __device__ __forceinline__ float top() const {
+        if constexpr (sizeof(T) == 4) {
+            return max_abs(max_abs(max_abs(x[0], x[1]), max_abs(x[2], x[3])),
+                           max_abs(max_abs(x[4], x[5]), max_abs(x[6], x[7])));
+        } else {  // two at a time; a NaN stays one
+            const uint4 w = *reinterpret_cast<const uint4*>(x);
+            const uint32_t m = 0x7FFF7FFFu;
+            uint32_t a = max16(w.x & m, w.y & m), b = max16(w.z & m, w.w & m);
+            a = max16(a, b);
+            a = max16(a, a >> 16) & 0xFFFFu;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value)
+                return __uint_as_float(a << 16);
+            else
+                return __half2float(__ushort_as_half((unsigned short)a));
+        }
+    }
+    // magnitudes order as integers, infinity and then NaN above all
+    static __device__ __forceinline__ uint32_t max16(uint32_t a, uint32_t b) {
+        return __vmaxu2(a, b);
+    }
+};
+
+// The eight elements from column c0 + 8 * lane of a row, zeros past dim.  VEC: rows start at
+// 16-byte boundaries; else the warp's 256 elements come in one by one, side by side, and pass
+// through shared memory.
+template <class T, bool VEC>
+__device__ __forceinline__ Eight<T> load8(const T* row, int c0, int dim, int lane, T* stage) {
+    const int c = c0 + 8 * lane;
+    Eight<T> e;
+    if constexpr (VEC) {
+        if (c + 8 <= dim) {
+            constexpr int N = sizeof(Eight<T>) / 16;
+            uint4* raw = reinterpret_cast<uint4*>(&e);
+#pragma unroll
+            for (int j = 0; j < N; ++j) raw[j] = __ldcg(reinterpret_cast<const uint4*>(row + c) + j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e.x[j] = c + j < dim ? row[c + j] : from_float<T>(0.0f);
+        }
+    } else {
+        T x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int at = c0 + 32 * j + lane;
+            x[j] = at < dim ? row[at] : from_float<T>(0.0f);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) stage[32 * j + lane] = x[j];
+        __syncwarp();
+        e = *reinterpret_cast<const Eight<T>*>(stage + 8 * lane);
+    }
+    return e;
 }
 
 __device__ __forceinline__ float rcp_approx(float x) {  // within an ulp, x normal
@@ -109,25 +147,30 @@ __device__ __forceinline__ uint32_t e4m3_quotient(float top, float h, float rh) 
         : "f"(t * (1.0f - 0x1p-20f)), "f"(t * (1.0f + 0x1p-20f)));
     const uint32_t lo = two & 0xFFu, hi = two >> 8;
     if (lo == hi) return lo;
-    // compare top with the exact border (5 significant bits) times h
-    const double mid = 0.5 * ((double)e4m3_value(lo) + (double)e4m3_value(hi)) * (double)h;
-    if ((double)top == mid) return (lo & 1u) ? hi : lo;
-    return (double)top > mid ? hi : lo;
+    // the neighbours' border has five significant bits: the fused multiply-add's sign is that
+    // of the exact top - border h
+    const float over = fmaf(-0.5f * (e4m3_value(lo) + e4m3_value(hi)), h, top);
+    return over > 0.0f || (over == 0.0f && (lo & 1u)) ? hi : lo;
 }
 
-// The e2m1 code of |x| / d by the borders themselves; the fused multiply-add's sign is that
-// of the exact x - border d.
-__device__ __noinline__ uint32_t e2m1_exact(float x, float d) {
-    const float a = fabsf(x);
-    uint32_t c = 0;
-    c += fmaf(-0.25f, d, a) > 0.0f;
-    c += fmaf(-0.75f, d, a) >= 0.0f;
-    c += fmaf(-1.25f, d, a) > 0.0f;
-    c += fmaf(-1.75f, d, a) >= 0.0f;
-    c += fmaf(-2.5f, d, a) > 0.0f;
-    c += fmaf(-3.5f, d, a) >= 0.0f;
-    c += fmaf(-5.0f, d, a) > 0.0f;
-    return c | (x < 0.0f ? 8u : 0u);
+// Where the codes of a value's two neighbours differ, the one that is nearest to v / d: the
+// border between two codes c and c + 1 has three significant bits, so the fused multiply-add's
+// sign is that of the exact |v| - border d.  `lo` holds the codes nearer to zero.
+__device__ __forceinline__ uint32_t settle_borders(uint32_t lo, uint32_t hi, const float (&v)[8],
+                                                   float d) {
+    uint32_t open = lo ^ hi;
+    while (open) {
+        const int j = (__ffs(open) - 1) >> 2;
+        float x = v[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) x = j == i ? v[i] : x;
+        const uint32_t c = (lo >> (4 * j)) & 7u;
+        const float border = c < 4 ? 0.25f + 0.5f * (float)c : c == 4 ? 2.5f : c == 5 ? 3.5f : 5.0f;
+        const float over = fmaf(-border, d, fabsf(x));
+        if (over > 0.0f || (over == 0.0f && (c & 1u))) lo += 1u << (4 * j);
+        open &= ~(15u << (4 * j));
+    }
+    return lo;
 }
 
 // Eight codes of v / d; rd is 1 / d, in MX exactly, in NV within 2^-22 (0 for d = 0).
@@ -147,11 +190,7 @@ __device__ __forceinline__ uint32_t codes8(const float (&v)[8], float d, float r
         b[j] = v[j] * r1;
     }
     const uint32_t lo = e2m1x8(a), hi = e2m1x8(b);
-    if (lo == hi) return lo;
-    uint32_t c = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c |= e2m1_exact(v[j], d) << (4 * j);
-    return c;
+    return lo == hi ? lo : settle_borders(lo, hi, v, d);
 }
 
 struct WriteParams {
@@ -216,7 +255,8 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
     constexpr int BL = block_of(FMT) / 8;  // lanes per block
     const int steps = (p.dp + STEP - 1) / STEP;
     const int first = WPR == 1 ? 0 : warp;
-    uint32_t* codes_out = reinterpret_cast<uint32_t*>(p.codes + slot * (p.dp / 2));
+    uint32_t* codes_out = reinterpret_cast<uint32_t*>(p.codes + slot * (p.dp / 2)) + lane;
+    uint8_t* scales_out = p.scales + scale_word(slot, lane / (4 * BL), atoms);
 
     float amax = 0.0f;  // of this warp's elements, then of the row: NaN and infinities show
     float s2 = 0.0f;    // sum of the blocks' squared scales, BL times over
@@ -252,48 +292,49 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
             s2 = fmaf(s, s, s2);
             codes = codes8<FMT>(v, d, bits ? rcp_approx(d) : 0.0f);
         }
-        if (c < p.dp) codes_out[c >> 3] = codes;
+        if (c < p.dp) codes_out[k * 32] = codes;
         // four blocks' bytes to the first lane of their atom
         uint32_t word = bits << (8 * ((lane / BL) & 3));
 #pragma unroll
         for (int o = BL; o < 4 * BL; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
         if (c < p.dp && lane % (4 * BL) == 0)
-            *reinterpret_cast<uint32_t*>(p.scales +
-                                         scale_word(slot, c / (32 * BL), atoms)) = word;
+            *reinterpret_cast<uint32_t*>(scales_out + k * (STEP / (32 * BL)) * 512) = word;
     };
     if constexpr (FMT == kMX) {
         // four steps' loads in flight
         for (int k0 = first; k0 < steps; k0 += 4 * WPR) {
-            float v[4][8];
+            Eight<T> e[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (k0 + u * WPR < steps)
-                    load8<T, VEC>(row, (k0 + u * WPR) * STEP, p.dim, lane, stage, v[u]);
+                    e[u] = load8<T, VEC>(row, (k0 + u * WPR) * STEP, p.dim, lane, stage);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (k0 + u * WPR < steps) {
-                    const float top = max8(v[u]);
+                    float v[8];
+                    e[u].values(v);
+                    const float top = e[u].top();
                     amax = max_abs(amax, top);
-                    quantise(k0 + u * WPR, v[u], top);
+                    quantise(k0 + u * WPR, v, top);
                 }
         }
         row_max();
         if (amax == 0.0f) g = 0.0f;
     } else {
         constexpr int H = HOLD > 0 ? HOLD : 1;
-        float v[H][8], top[H];
+        Eight<T> e[H];
+        float v[8], top[H];
         if constexpr (HOLD > 0) {
 #pragma unroll
             for (int u = 0; u < H; ++u)
                 if (first + u * WPR < steps)
-                    load8<T, VEC>(row, (first + u * WPR) * STEP, p.dim, lane, stage, v[u]);
+                    e[u] = load8<T, VEC>(row, (first + u * WPR) * STEP, p.dim, lane, stage);
 #pragma unroll
             for (int u = 0; u < H; ++u)
-                if (first + u * WPR < steps) amax = max_abs(amax, top[u] = max8(v[u]));
+                if (first + u * WPR < steps) amax = max_abs(amax, top[u] = e[u].top());
         } else {
             for (int k = first; k < steps; k += WPR) {
-                load8<T, VEC>(row, k * STEP, p.dim, lane, stage, v[0]);
-                amax = max_abs(amax, max8(v[0]));
+                amax = max_abs(amax, load8<T, VEC>(row, k * STEP, p.dim, lane, stage).top());
             }
         }
         row_max();
@@ -304,11 +345,15 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
         if constexpr (HOLD > 0) {
 #pragma unroll
             for (int u = 0; u < H; ++u)
-                if (first + u * WPR < steps) quantise(first + u * WPR, v[u], top[u]);
+                if (first + u * WPR < steps) {
+                    e[u].values(v);
+                    quantise(first + u * WPR, v, top[u]);
+                }
         } else {
             for (int k = first; k < steps; k += WPR) {
-                load8<T, VEC>(row, k * STEP, p.dim, lane, stage, v[0]);
-                quantise(k, v[0], max8(v[0]));
+                e[0] = load8<T, VEC>(row, k * STEP, p.dim, lane, stage);
+                e[0].values(v);
+                quantise(k, v, e[0].top());
             }
         }
     }
@@ -349,6 +394,16 @@ struct ReadParams {
     int* status;
 };
 
+__device__ __forceinline__ void store8(float* to, const float (&t)[8]) {  // a whole sector a lane
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "f"(t[0]),
+                 "f"(t[1]), "f"(t[2]), "f"(t[3]), "f"(t[4]), "f"(t[5]), "f"(t[6]), "f"(t[7])
+                 : "memory");
+}
+template <class T>
+__device__ __forceinline__ void store8(T* to, const T (&t)[8]) {
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(t);
+}
+
 // One warp per row.  Bound by HBM: the output once.
 template <int FMT, class T, bool VEC>
 __global__ void __launch_bounds__(WARPS * 32) read_kernel(const ReadParams p) {
@@ -366,47 +421,59 @@ __global__ void __launch_bounds__(WARPS * 32) read_kernel(const ReadParams p) {
         return;
     }
     const float g = __ldcg(&p.row_scale[slot]);
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.codes + slot * (p.dp / 2));
     const int atoms = atoms_of(FMT, p.dp);
+    constexpr int BL = block_of(FMT) / 8;              // lanes per block
+    constexpr int APB = 8 * STEP / (4 * block_of(FMT));  // atoms of eight steps, at most a warp's
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(p.codes + slot * (p.dp / 2)) + lane;
+    const uint8_t* scales = p.scales + scale_word(slot, 0, atoms);
     T* out = static_cast<T*>(p.dst) + i * p.stride;
-#pragma unroll 4
-    for (int c0 = 0; c0 < p.dim; c0 += STEP) {
-        const int c = c0 + 8 * lane;
-        const bool in = c < p.dp;
-        const int b = c / block_of(FMT);
-        const uint32_t packed = in ? __ldcg(codes + (c >> 3)) : 0u;
-        const uint32_t byte =
-            in ? __ldcg(p.scales + scale_word(slot, b >> 2, atoms) + (b & 3)) : 0u;
-        float v[8];
-        e2m1x8_values(packed, v);
-        const float s = scale_value<FMT>(byte);
-        // code * s has at most six significant bits: one rounding in the product with g (and
-        // one to a 16-bit output, from a value already within 2^-24)
-        alignas(16) T t[8];
+    // Eight steps' loads in flight: a word of codes a lane and step, and the scale bytes of an
+    // atom a lane, handed round by shuffles.
+    for (int c00 = 0; c00 < p.dim; c00 += 8 * STEP) {
+        const int atom0 = c00 / (4 * block_of(FMT));
+        const uint32_t bytes = lane < APB && atom0 + lane < atoms
+                                   ? __ldcg(reinterpret_cast<const uint32_t*>(
+                                         scales + (int64_t)(atom0 + lane) * 512))
+                                   : 0u;
+        uint32_t packed[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = from_float<T>(__fmul_rn(__fmul_rn(v[j], s), g));
-        if constexpr (VEC) {
-            if (c + 8 <= p.dim) {
-                constexpr int N = 8 * sizeof(T) / 16;
+        for (int u = 0; u < 8; ++u)
+            packed[u] = c00 + u * STEP + 8 * lane < p.dp ? __ldcg(codes + c00 / 8 + u * 32) : 0u;
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    reinterpret_cast<uint4*>(out + c)[j] = reinterpret_cast<const uint4*>(t)[j];
+        for (int u = 0; u < 8; ++u) {
+            const int c0 = c00 + u * STEP;
+            if (c0 >= p.dim) break;
+            const int c = c0 + 8 * lane;
+            const uint32_t word =
+                __shfl_sync(0xffffffffu, bytes, u * (STEP / (4 * block_of(FMT))) + lane / (4 * BL));
+            const float s = scale_value<FMT>((word >> (8 * ((lane / BL) & 3))) & 255u);
+            float v[8];
+            e2m1x8_values(packed[u], v);
+            // code * s has at most six significant bits: one rounding in the product with g
+            // (and one to a 16-bit output, from a value already within 2^-24)
+            alignas(16) T t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = from_float<T>(__fmul_rn(__fmul_rn(v[j], s), g));
+            if constexpr (VEC) {
+                if (c + 8 <= p.dim) {
+                    store8(out + c, t);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (c + j < p.dim) out[c + j] = t[j];
+                }
             } else {
+                // side by side through shared memory: eight strided elements a lane took 3.5
+                // times as long
+                __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (c + j < p.dim) out[c + j] = t[j];
-            }
-        } else {
-            // side by side through shared memory: eight strided elements a lane took 3.5 times
-            // as long
-            __syncwarp();
+                for (int j = 0; j < 8; ++j) stage[8 * lane + j] = t[j];
+                __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) stage[8 * lane + j] = t[j];
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int e = 32 * j + lane;
-                if (c0 + e < p.dim) out[c0 + e] = stage[e];
+                for (int j = 0; j < 8; ++j) {
+                    const int e = 32 * j + lane;
+                    if (c0 + e < p.dim) out[c0 + e] = stage[e];
+                }
             }
         }
     }
@@ -421,6 +488,7 @@ static int write_v(const WriteParams& p, cudaStream_t st) {
     const dim3 grid((unsigned)((p.n + WARPS - 1) / WARPS));
     if constexpr (FMT == kNV) {
         if (p.dp <= 4 * STEP) return launch_pdl(write_kernel<FMT, T, VEC, 1, 4>, grid, WARPS * 32, 0, st, p);
+        if (p.dp <= 6 * STEP) return launch_pdl(write_kernel<FMT, T, VEC, 1, 6>, grid, WARPS * 32, 0, st, p);
         if (p.dp <= 8 * STEP) return launch_pdl(write_kernel<FMT, T, VEC, 1, 8>, grid, WARPS * 32, 0, st, p);
     }
     return launch_pdl(write_kernel<FMT, T, VEC, 1, 0>, grid, WARPS * 32, 0, st, p);
@@ -435,7 +503,8 @@ static int write_t(const WriteParams& p, cudaStream_t st) {
 
 template <int FMT, class T>
 static int read_t(const ReadParams& p, cudaStream_t st) {
-    const bool vec = reinterpret_cast<uintptr_t>(p.dst) % 16 == 0 && p.stride * sizeof(T) % 16 == 0;
+    constexpr size_t A = 8 * sizeof(T);
+    const bool vec = reinterpret_cast<uintptr_t>(p.dst) % A == 0 && p.stride * sizeof(T) % A == 0;
     const dim3 grid((unsigned)((p.n + WARPS - 1) / WARPS));
     return vec ? launch_pdl(read_kernel<FMT, T, true>, grid, WARPS * 32, 0, st, p)
                : launch_pdl(read_kernel<FMT, T, false>, grid, WARPS * 32, 0, st, p);
