@@ -236,53 +236,69 @@ __device__ __forceinline__ void append_hits(Hits& h, const TcParams& p, int qt_f
     h.n = 0;
 }
 
-// r[i] for a warp-uniform i, without an indexed access that would move r to local memory.
+// r[i], without an indexed access that would move r to local memory: a tree of selects.
 __device__ __forceinline__ float pick(const uint32_t (&r)[32], int i) {
     uint32_t t[16];
+    asm("{\n\t.reg .pred p;\n\t.reg .b32 x;\n\tand.b32 x, %48, 1;\n\tsetp.ne.u32 p, x, 0;\n\t"
+        "selp.b32 %0, %17, %16, p;\n\t"
+        "selp.b32 %1, %19, %18, p;\n\t"
+        "selp.b32 %2, %21, %20, p;\n\t"
+        "selp.b32 %3, %23, %22, p;\n\t"
+        "selp.b32 %4, %25, %24, p;\n\t"
+        "selp.b32 %5, %27, %26, p;\n\t"
+        "selp.b32 %6, %29, %28, p;\n\t"
+        "selp.b32 %7, %31, %30, p;\n\t"
+        "selp.b32 %8, %33, %32, p;\n\t"
+        "selp.b32 %9, %35, %34, p;\n\t"
+        "selp.b32 %10, %37, %36, p;\n\t"
+        "selp.b32 %11, %39, %38, p;\n\t"
+        "selp.b32 %12, %41, %40, p;\n\t"
+        "selp.b32 %13, %43, %42, p;\n\t"
+        "selp.b32 %14, %45, %44, p;\n\t"
+        "selp.b32 %15, %47, %46, p;\n\t}"
+        : "=&r"(t[0]), "=&r"(t[1]), "=&r"(t[2]), "=&r"(t[3]), "=&r"(t[4]), "=&r"(t[5]), "=&r"(t[6]), "=&r"(t[7]), "=&r"(t[8]), "=&r"(t[9]), "=&r"(t[10]), "=&r"(t[11]), "=&r"(t[12]), "=&r"(t[13]), "=&r"(t[14]), "=&r"(t[15])
+        : "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(i));
 #pragma unroll
-    for (int j = 0; j < 16; ++j) t[j] = selp_u32(r[2 * j + 1], r[2 * j], i & 1);
+    for (int w = 8, b = 1; w >= 1; w /= 2, ++b) {
+        const bool odd = (i >> b) & 1;
 #pragma unroll
-    for (int w = 8, b = 1; w >= 1; w /= 2, ++b)
-#pragma unroll
-        for (int j = 0; j < w; ++j) t[j] = selp_u32(t[2 * j + 1], t[2 * j], (i >> b) & 1);
+        for (int j = 0; j < w; ++j) t[j] = odd ? t[2 * j + 1] : t[2 * j];
+    }
     return __uint_as_float(t[0]);
 }
 
 // One chunk of 32 columns of 32 rows, for the queries from column `at`: the rows that reach a
-// query's threshold are kept.  Most chunks have none.
+// query's threshold are kept.  Most chunks have none.  The sign of threshold - score is shifted
+// into a mask (that of a NaN, an empty row's, is clear); then each lane deals with its own
+// hits, one a round.
 __device__ __forceinline__ void collect_chunk(const uint32_t (&r)[32], const TcParams& p, Hits& h,
                                               int qt_first, int at, int64_t row, const float* gq,
                                               const float* th, float g, int lane) {
     const float4* t4 = reinterpret_cast<const float4*>(th + at);
-    // the largest excess over a threshold (a maximum passes over the NaN of an empty row)
-    float most = -INFINITY;
+    const float minus_g = -g;
+    uint32_t mine = 0;  // column i in bit 31 - i
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float4 t = t4[i];
-        most = fmaxf(most, fmaxf(fmaf(__uint_as_float(r[4 * i]), g, -t.x),
-                                 fmaf(__uint_as_float(r[4 * i + 1]), g, -t.y)));
-        most = fmaxf(most, fmaxf(fmaf(__uint_as_float(r[4 * i + 2]), g, -t.z),
-                                 fmaf(__uint_as_float(r[4 * i + 3]), g, -t.w)));
-    }
-    if (!__any_sync(0xffffffffu, most >= 0.0f)) return;
-    uint32_t mine = 0;
+        const float x[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-        mine |= (fmaf(__uint_as_float(r[i]), g, -th[at + i]) >= 0.0f ? 1u : 0u) << i;
-    uint32_t columns = __reduce_or_sync(0xffffffffu, mine);
-    while (columns) {
-        const int i = __ffs(columns) - 1;
-        columns &= columns - 1;
-        const float v = pick(r, i) * g;
-        const bool hit = (mine >> i) & 1u;
-        const unsigned m = __ballot_sync(0xffffffffu, hit);
+        for (int u = 0; u < 4; ++u)
+            mine = __funnelshift_l(
+                __float_as_uint(fmaf(__uint_as_float(r[4 * i + u]), minus_g, x[u])), mine, 1);
+    }
+    unsigned lanes = __ballot_sync(0xffffffffu, mine != 0);
+    while (lanes) {
         if (h.n > HITS - 32) append_hits(h, p, qt_first, lane);
-        if (hit) {
-            const int slot = h.n + __popc(m & ((1u << lane) - 1u));
+        const int i = __clz((int)mine);
+        const float v = pick(r, i) * g;
+        if (mine) {
+            const int slot = h.n + __popc(lanes & ((1u << lane) - 1u));
             h.entry[slot] = ((uint64_t)__float_as_uint(v * gq[at + i]) << 32) | (uint32_t)row;
             h.col[slot] = (uint8_t)(at + i);
+            mine &= ~(0x80000000u >> i);
         }
-        h.n += __popc(m);
+        h.n += __popc(lanes);
+        lanes = __ballot_sync(0xffffffffu, mine != 0);
     }
 }
 
@@ -1162,9 +1178,11 @@ static int round_up(int x, int a) { return (x + a - 1) / a * a; }
 
 // Queries per tile.  A pair's time for a tile of rows is, per 64 elements, nt / 2 cycles of
 // the tensor cores or, where that is more, the bytes that pass through each CTA's shared
-// memory at 128 a cycle: operands, the stage's copy, and the scale warps' reads; about 450
-// cycles more where one accumulator buffer has to be drained before the next tile.  Taken is
-// the nt whose query tiles, spread over the pairs, take the least.
+// memory -- operands, the stage's copy, and the scale warps' reads -- at the 88 a cycle that
+// fit what was measured (1M x 1536, us a tile: NV nt 128 1.77, 192 2.00, 256 2.40; MX 1.75,
+// 1.83, 2.35); about 450 cycles more where one accumulator buffer has to be drained before
+// the next tile.  Taken is the nt whose query tiles, spread over the pairs, take the least:
+// 256 for a batch of 1024 (search 0.80 ms against 0.96 at 192), 16 for one query.
 static bool make_plan(int fmt, int dp, int nq, int64_t n_tiles, Plan* out) {
     const int aps = atoms_per_stage(fmt), steps = dp / 64;
     const int kchunks = (dp / 2 + KC - 1) / KC;
@@ -1200,7 +1218,7 @@ static bool make_plan(int fmt, int dp, int nq, int64_t n_tiles, Plan* out) {
         const double bytes = HALF * 32 + nt / 2 * 32 + stage / 4.0 + 4.0 * aps * 512 / 4 +
                              (s.resident ? 0.0 : 4.0 * aps * sf_tiles * 512 / 4);
         const double tensor = nt / 2.0;
-        const double cycles = steps * (tensor > bytes / 128 ? tensor : bytes / 128) +
+        const double cycles = steps * (tensor > bytes / 88 ? tensor : bytes / 88) +
                               (s.bufs == 1 ? 450.0 : 0.0);
         const int64_t per = pairs / s.n_qt > 0 ? pairs / s.n_qt : 1;
         const int64_t waves = (s.n_qt * per + pairs - 1) / pairs;
