@@ -630,7 +630,8 @@ constexpr int SEL = 256;  // threads of a selection CTA
 __device__ __forceinline__ uint32_t ordered_score(float v) { return v == v ? ordered(v) : 0u; }
 
 // The k-th largest of a warp's 32 V values, bit by bit from the highest: a bit is set if k values
-// reach the number with it.  About 50 + V cycles a bit, and no shared memory.
+// reach the number with it; once exactly k do, it is the least of those.  About 50 + 2 V
+// cycles a bit, and no shared memory.
 template <int V>
 __device__ __forceinline__ uint32_t warp_kth(const uint32_t (&v)[V], int k) {
     uint32_t x = 0;
@@ -640,9 +641,14 @@ __device__ __forceinline__ uint32_t warp_kth(const uint32_t (&v)[V], int k) {
         int c = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) c += v[i] >= y;
-        if (__reduce_add_sync(0xffffffffu, c) >= k) x = y;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c >= k) x = y;
+        if (c == k) break;
     }
-    return x;
+    uint32_t least = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < V; ++i) least = v[i] >= x ? min(least, v[i]) : least;
+    return __reduce_min_sync(0xffffffffu, least);
 }
 
 template <int V, class F>
@@ -654,16 +660,18 @@ __device__ __forceinline__ uint32_t warp_kth_of(int m, int k, F value) {
     return warp_kth<V>(v, k);
 }
 
-// The k-th largest of n <= LIST values in shared memory, by a CTA of NT threads: one warp's
-// search of up to 512, else the same search by all with a barrier a bit.
+// The k-th largest of n <= LIST values in shared memory, by a CTA of NT threads: one warp's search of up
+// to 1024, else the same search by all with a barrier a bit.
 template <int NT>
 __device__ uint32_t list_kth(const uint32_t* list, int n, int k) {
     __shared__ uint32_t s_kth;
     __shared__ int s_bit[32];
-    if (n <= 512) {
+    if (n <= 1024) {
         if (threadIdx.x < 32) {
             auto at = [&](int i) { return list[i]; };
-            const uint32_t x = n <= 64 ? warp_kth_of<2>(n, k, at) : warp_kth_of<16>(n, k, at);
+            const uint32_t x = n <= 64    ? warp_kth_of<2>(n, k, at)
+                               : n <= 256 ? warp_kth_of<8>(n, k, at)
+                                          : warp_kth_of<32>(n, k, at);
             if (threadIdx.x == 0) s_kth = x;
         }
         __syncthreads();
@@ -961,12 +969,14 @@ __device__ __forceinline__ uint64_t row_key(double dot, float g, float gq, int64
     return ((uint64_t)ordered(s) << 32) | (uint32_t)~(uint32_t)row;
 }
 
+// By NT threads, this one the `at`-th.
 template <int FMT, int NT>
-__device__ __forceinline__ void load_query(const FinishParams& p, const QueryShared& q, int64_t qs) {
+__device__ __forceinline__ void load_query(const FinishParams& p, const QueryShared& q, int64_t qs,
+                                           int at) {
     const uint16_t* codes = reinterpret_cast<const uint16_t*>(p.q_codes + qs * (p.dp / 2));
-    for (int i = threadIdx.x; i < p.dp / 4; i += NT)
+    for (int i = at; i < p.dp / 4; i += NT)
         reinterpret_cast<uint32_t*>(q.codes)[i] = e2m1x4_bytes(__ldcg(codes + i));
-    for (int b = threadIdx.x; b < p.dp / block_of(FMT); b += NT)
+    for (int b = at; b < p.dp / block_of(FMT); b += NT)
         q.scales[b] = scale_value<FMT>(__ldcg(p.q_scales + scale_word(qs, b >> 2, p.atoms) + (b & 3)));
 }
 
@@ -1015,26 +1025,48 @@ __global__ void __launch_bounds__(NT) finish_kernel(const FinishParams p) {
                 return p.dense ? __ldcg(dense + i)
                                : __uint_as_float((uint32_t)(__ldcg(cand + i) >> 32));
             };
-            float cut = -INFINITY;
-            if (m > p.k) {
-                const uint32_t o =
-                    kth_largest<NT, 8>(m, p.k, reinterpret_cast<uint32_t*>(key),
-                                       [&](int i) { return ordered_score(approx(i)); });
-                cut = o ? unordered(o) - two_eps : -INFINITY;
-            }
-            load_query<FMT, NT>(p, q, qs);
-            __syncthreads();
-            for (int i0 = threadIdx.x; i0 < m; i0 += 4 * NT) {
-                float a[4];
+            uint32_t* list = reinterpret_cast<uint32_t*>(key);
+            auto take = [&](float a, float cut, uint64_t row) {
+                if (a >= cut || !known) {
+                    const int at = atomicAdd(&s_n, 1);
+                    if (at < LIST) key[at] = row;
+                }
+            };
+            auto cut_of = [&](uint32_t o) { return o ? unordered(o) - two_eps : -INFINITY; };
+            if (!p.dense && m <= LIST) {
+                // candidates in registers; the first warp searches while the others load the query
+                constexpr int V = LIST / NT;
+                uint64_t c[V];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) a[u] = i0 + u * NT < m ? approx(i0 + u * NT) : -INFINITY;
+                for (int u = 0; u < V; ++u) {
+                    const int i = threadIdx.x + u * NT;
+                    c[u] = i < m ? __ldcg(cand + i) : 0;
+                    if (i < m) list[i] = ordered_score(__uint_as_float((uint32_t)(c[u] >> 32)));
+                }
+                __syncthreads();
+                if (warp > 0) load_query<FMT, NT - 32>(p, q, qs, threadIdx.x - 32);
+                const float cut = m > p.k ? cut_of(list_kth<NT>(list, m, p.k)) : -INFINITY;
+                __syncthreads();
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int i = i0 + u * NT;
-                    if (i < m && (a[u] >= cut || !known)) {
-                        const int at = atomicAdd(&s_n, 1);
-                        if (at < LIST)
-                            key[at] = p.dense ? (uint64_t)i : (__ldcg(cand + i) & 0xFFFFFFFFu);
+                for (int u = 0; u < V; ++u)
+                    if ((int)threadIdx.x + u * NT < m)
+                        take(__uint_as_float((uint32_t)(c[u] >> 32)), cut, c[u] & 0xFFFFFFFFu);
+            } else {
+                load_query<FMT, NT>(p, q, qs, threadIdx.x);
+                float cut = -INFINITY;
+                if (m > p.k)
+                    cut = cut_of(kth_largest<NT, 8>(
+                        m, p.k, list, [&](int i) { return ordered_score(approx(i)); }));
+                __syncthreads();
+                for (int i0 = threadIdx.x; i0 < m; i0 += 4 * NT) {
+                    float a[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) a[u] = i0 + u * NT < m ? approx(i0 + u * NT) : 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int i = i0 + u * NT;
+                        if (i < m)
+                            take(a[u], cut, p.dense ? (uint64_t)i : (__ldcg(cand + i) & 0xFFFFFFFFu));
                     }
                 }
             }
@@ -1135,7 +1167,7 @@ __global__ void __launch_bounds__(SEL) rescue_kernel(const FinishParams p) {
         const int64_t qs = query_slot(t, p.nt, p.nt_pad);
         const float gq = __ldcg(p.q_scale + qs);
         const int64_t begin = p.n_rows * part / splits, end = p.n_rows * (part + 1) / splits;
-        load_query<FMT, SEL>(p, q, qs);
+        load_query<FMT, SEL>(p, q, qs, threadIdx.x);
         if (threadIdx.x == 0) s_n = 0;
         __syncthreads();
         BestKeys<SEL> best = {key, &s_n, 0};
