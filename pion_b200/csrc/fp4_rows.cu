@@ -23,6 +23,7 @@ namespace pion {
 namespace fp4 {
 
 constexpr int WARPS = 8;   // per CTA
+constexpr int FEW = 1024;  // rows written by a CTA each
 constexpr int STEP = 256;  // elements per warp step, eight consecutive ones per lane
 
 // In NV an amax below this is stored as a row of zeros: g = amax / 2688 and its multiples then stay
@@ -209,10 +210,12 @@ struct WriteParams {
     float* norm;           // per row (queries), or null
     float* norm_max;       // the store's bound, or null
     int* zero;             // set to 0, or null
+    int* status;
 };
 
-// A slot named by several rows of one write keeps the last of them: every row raises the
-// slot's claim to its index, and the write kernel takes only the row that holds it.
+// A slot named by several rows of one write keeps the last of them.  Of few rows each CTA looks
+// through the rows after its own; of many, every row first raises the slot's claim to its
+// index, and the write kernel takes only the row that holds it.
 __global__ void claim_kernel(const int64_t* slots, int64_t n, int64_t n_slots,
                              int32_t* claim, int* status) {
     griddep_launch();
@@ -245,8 +248,15 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
         slot = query_slot(i, p.tile, p.tile_pad);
     } else if (p.slots) {
         slot = __ldcg(p.slots + i);
+        if (WPR > 1) {
+            bool later = false;
+            for (int64_t j = i + 1 + threadIdx.x; j < p.n; j += WARPS * 32)
+                later |= __ldcg(p.slots + j) == slot;
+            if (__syncthreads_or(later)) return;
+            if (slot >= p.n_slots && threadIdx.x == 0) record_error(p.status, PION_B200_EINVAL);
+        }
         if (slot < 0 || slot >= p.n_slots) return;
-        if (__ldcg(p.claim + slot) != (int32_t)(i + 1)) return;
+        if (WPR == 1 && __ldcg(p.claim + slot) != (int32_t)(i + 1)) return;
     } else {
         slot = p.start + i;
     }
@@ -376,7 +386,7 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
         if (p.norm) p.norm[i] = bound;
         if (p.norm_max && bound > __ldcg(p.norm_max))
             atomicMax(reinterpret_cast<int*>(p.norm_max), __float_as_int(bound));
-        if (p.slots) p.claim[slot] = 0;
+        if (WPR == 1 && p.slots) p.claim[slot] = 0;
     }
 }
 
@@ -482,7 +492,7 @@ __global__ void __launch_bounds__(WARPS * 32) read_kernel(const ReadParams p) {
 template <int FMT, class T, bool VEC>
 static int write_v(const WriteParams& p, cudaStream_t st) {
     // Few rows: a CTA each; many: a warp each.
-    if (p.n <= 1024)
+    if (p.n <= FEW)
         return launch_pdl(write_kernel<FMT, T, VEC, WARPS, 4>, dim3((unsigned)p.n), WARPS * 32, 0,
                           st, p);
     const dim3 grid((unsigned)((p.n + WARPS - 1) / WARPS));
@@ -515,7 +525,7 @@ static int read_t(const ReadParams& p, cudaStream_t st) {
 int launch_fp4_write(const Fp4Write& w, cudaStream_t st) {
     using namespace fp4;
     if (w.n <= 0) return 0;
-    if (w.slots) {
+    if (w.slots && w.n > FEW) {
         if (launch_pdl(claim_kernel, dim3((unsigned)((w.n + 255) / 256)), 256, 0, st, w.slots, w.n,
                        w.n_slots, w.claim, w.status) != 0)
             return PION_B200_ECUDA;
@@ -538,6 +548,7 @@ int launch_fp4_write(const Fp4Write& w, cudaStream_t st) {
     p.norm = w.norm;
     p.norm_max = w.norm_max;
     p.zero = w.zero;
+    p.status = w.status;
     const bool mx = w.format == kMX;
     switch (w.type) {
         case PION_B200_F32: return mx ? write_t<kMX, float>(p, st) : write_t<kNV, float>(p, st);

@@ -15,6 +15,7 @@ torch's current stream of their device, and calls on them can be captured into C
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 
@@ -48,7 +49,9 @@ def _call(ctx: Context, fn, *args, mem: int = MEM_DEVICE):
     before = torch.cuda.current_device()
     try:
         if mem == MEM_DEVICE:
-            ctx.check(fn(ctx.h, *args, mem, _stream(ctx)))
+            rc = fn(ctx.h, *args, mem, _stream(ctx))
+            if rc != 0:
+                ctx.check(rc)
         else:
             lib = ctx.lib
             ctx.check(lib.pion_v_b200_set_stream(ctx.h, _stream(ctx)))
@@ -116,6 +119,19 @@ def _output(out, shape, dtype, device, make=None):
     return out, typ, (out.stride(0) if shape[0] > 1 else shape[1])
 
 
+@functools.lru_cache(maxsize=256)
+def _sizes(format: str, n_rows: int, dim: int):
+    """Bytes of a store's codes and scales."""
+    if format not in FORMATS:
+        raise ValueError(f"format must be one of {sorted(FORMATS)}, got {format!r}")
+    cb, sb = ctypes.c_int64(), ctypes.c_int64()
+    rc = _lib.load().pion_v_b200_fp4_sizes(FORMATS[format], n_rows, dim, ctypes.byref(cb),
+                                           ctypes.byref(sb))
+    if rc != 0:
+        raise PionError(rc, f"unsupported store: {n_rows} rows of {dim} elements")
+    return cb.value, sb.value
+
+
 class FP4Rows:
     """A store of ``n_rows`` slots of ``dim`` elements in 4 bits (every slot empty at first).
 
@@ -126,15 +142,7 @@ class FP4Rows:
 
     def __init__(self, n_rows: int, dim: int, format: str = "nv", device=None, *, codes=None,
                  scales=None, row_scale=None, norm_max=None, claim=None):
-        if format not in FORMATS:
-            raise ValueError(f"format must be one of {sorted(FORMATS)}, got {format!r}")
-        lib = _lib.load()
-        cb, sb = ctypes.c_int64(), ctypes.c_int64()
-        rc = lib.pion_v_b200_fp4_sizes(FORMATS[format], n_rows, dim, ctypes.byref(cb),
-                                       ctypes.byref(sb))
-        if rc != 0:
-            raise PionError(rc, f"unsupported store: {n_rows} rows of {dim} elements")
-        cb, sb = cb.value, sb.value
+        cb, sb = _sizes(format, n_rows, dim)
         if codes is None and scales is None and row_scale is None and norm_max is None:
             device = torch.device("cuda" if device is None else device)
             codes = torch.zeros((n_rows, cb // max(n_rows, 1)), dtype=torch.uint8, device=device)
@@ -145,7 +153,7 @@ class FP4Rows:
         elif codes is None or scales is None or row_scale is None or norm_max is None:
             raise ValueError("a store of given tensors needs codes, scales, row_scale and norm_max")
         else:
-            at = codes.device
+            at = codes.get_device()
             for name, t, dtype, size in (("codes", codes, torch.uint8, cb),
                                          ("scales", scales, torch.uint8, sb),
                                          ("row_scale", row_scale, torch.float32, n_rows),
@@ -153,9 +161,9 @@ class FP4Rows:
                                          ("claim", claim, torch.int32, n_rows)):
                 if t is None and name == "claim":
                     continue
-                if t.dtype != dtype or t.numel() != size or not t.is_contiguous():
+                if t.dtype is not dtype or t.numel() != size or not t.is_contiguous():
                     raise ValueError(f"{name} must be {size} contiguous {dtype} values")
-                if not t.is_cuda or t.device != at:
+                if at < 0 or t.get_device() != at:
                     raise ValueError(f"{name} must be on the store's CUDA device")
         self.n_rows, self.dim, self.format = n_rows, dim, format
         self.codes, self.scales, self.row_scale = codes, scales, row_scale
