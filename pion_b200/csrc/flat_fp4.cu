@@ -200,20 +200,34 @@ __device__ __forceinline__ __nv_bfloat16 cast_out<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half cast_out<__half>(float v) { return __float2half_rn(v); }
 
-// One 32-column chunk of one row's scores to out[t][col], t from t0.
+// One 32-column chunk of one row's scores, the first n of them, to out[t][col], t from t0.  NaN,
+// which an empty row's or query's scale makes of a score, becomes -inf.
+template <class T, bool FULL>
+__device__ __forceinline__ void store_columns(const uint32_t (&r)[32], T* out, int64_t ld, int n,
+                                              const float* gq, float g) {
+    const float4* g4 = reinterpret_cast<const float4*>(gq);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 s = g4[i];
+        const float x[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int j = 4 * i + u;
+            if (FULL || j < n) {
+                *out = cast_out<T>(fmaxf(__uint_as_float(r[j]) * g * x[u], -INFINITY));
+                out += ld;
+            }
+        }
+    }
+}
 template <class T>
 __device__ __forceinline__ void store_chunk(const uint32_t (&r)[32], const TcParams& p, int t0,
                                             int n, int64_t col, const float* gq, float g) {
     T* out = static_cast<T*>(p.out) + (int64_t)t0 * p.ld + col;
-    const bool row_ok = g == g;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        if (j < n) {
-            const float s = gq[j];
-            const float v = row_ok && s == s ? __uint_as_float(r[j]) * g * s : -INFINITY;
-            out[(int64_t)j * p.ld] = cast_out<T>(v);
-        }
-    }
+    if (n == 32)
+        store_columns<T, true>(r, out, p.ld, n, gq, g);
+    else
+        store_columns<T, false>(r, out, p.ld, n, gq, g);
 }
 
 // Candidates that an epilogue warp has found and not yet appended: an append waits for its
