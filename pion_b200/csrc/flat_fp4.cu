@@ -34,14 +34,17 @@ constexpr int HALF = 128;                // rows per CTA (TMEM lanes)
 constexpr int ROWS = 2 * HALF;           // rows per tile: a CTA pair (UMMA M = 256)
 constexpr int KC = 128;                  // code bytes of K per pipeline stage (256 elements)
 constexpr int A_BYTES = HALF * KC;       // 16 KB
-// Four warpgroups: the scale warps; the loading and the MMA warp (and two idle ones); two of
-// epilogue warps, two per TMEM lane quarter.  An epilogue thread holds up to 128
+// Six warpgroups: the scale warps; the loading and the MMA warp (and two idle ones); four of
+// epilogue warps, four per TMEM lane quarter.  An epilogue thread holds up to 64
 // accumulators, so that one buffer of them is free again as soon as it is read.
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;
+constexpr int PER_QUARTER = EPI_WARPS / 4;
+constexpr int HELD = 8 / PER_QUARTER;    // chunks of 32 columns a warp may have of a tile
 constexpr int SCALE_WARPS = 4;
-constexpr int THREADS = 512;             // 128 registers a thread at launch ...
-constexpr int REGS_SCALE = 64, REGS_ISSUE = 64, REGS_EPI = 192;  // ... and 4 * 128 in all here
-static_assert(REGS_SCALE + REGS_ISSUE + 2 * REGS_EPI <= 4 * 128, "register split");
+constexpr int THREADS = 256 + 32 * EPI_WARPS;  // 80 registers a thread at launch ...
+constexpr int REGS_SCALE = 48, REGS_ISSUE = 48, REGS_EPI = 96;  // ... and 6 * 80 in all here
+static_assert(REGS_SCALE + REGS_ISSUE + (EPI_WARPS / 4) * REGS_EPI <= (THREADS / 128) * 80,
+              "register split");
 constexpr uint32_t TMEM_COLS = 512;
 constexpr int MAX_STAGES = 8;
 constexpr int MAX_NT = 256;
@@ -580,8 +583,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_EPI));
         // ---------------------------------------------------------- epilogue
         const int quarter = warp & 3;
-        const int half = (warp - 8) >> 2;
-        const int chunks = (nt + 31) / 32;     // of 32 columns; this warp takes every other one
+        const int half = (warp - 8) >> 2;      // of PER_QUARTER
+        const int chunks = (nt + 31) / 32;     // of 32 columns; this warp takes every PER_QUARTER-th
         const int in_tile = (int)rank * HALF + quarter * 32 + lane;
         Hits hits = {s_hits + (warp - 8) * HITS, s_hit_col + (warp - 8) * HITS, 0};
         int buf = 0;
@@ -595,20 +598,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             tc_fence_after();
             const uint32_t taddr =
                 tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * nt);
-            uint32_t r[4][32];
+            uint32_t r[HELD][32];
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (2 * c + half < chunks) tmem_ld32(taddr + (2 * c + half) * 32, r[c]);
+            for (int c = 0; c < HELD; ++c)
+                if (PER_QUARTER * c + half < chunks)
+                    tmem_ld32(taddr + (PER_QUARTER * c + half) * 32, r[c]);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld_wait_regs(r[c]);
+            for (int c = 0; c < HELD; ++c) tmem_ld_wait_regs(r[c]);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_leader(&tempty[buf]);
             const int64_t col = (int64_t)j * ROWS + in_tile;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int at = (2 * c + half) * 32;
-                if (2 * c + half >= chunks) break;
+            for (int c = 0; c < HELD; ++c) {
+                const int at = (PER_QUARTER * c + half) * 32;
+                if (at >= nt) break;
                 if (mode == kCollect) {
                     collect_chunk(r[c], p, hits, qt * nt, at, row, s_gq, s_th, g, lane);
                     continue;
