@@ -481,7 +481,8 @@ int pion_v_b200_flat_i8_knn_sharded(pion_b200_ctx *ctx, const pion_b200_index *i
  * DEVICE the call runs on that stream, NULL being the context's.  Calls with DEVICE memory
  * on a stream of their own use no memory of the context's (scores and search then need a
  * `workspace`) but its status word, and may be captured into a CUDA graph, which keeps
- * using the pointers it was captured with. */
+ * using the pointers it was captured with.  pion_v_b200_sync does not wait for such a
+ * stream: after the caller has, it reports what the calls' kernels recorded. */
 typedef struct pion_b200_fp4_rows {
     int32_t format;      /* PION_B200_FP4_* */
     int32_t reserved;

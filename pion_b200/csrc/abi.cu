@@ -184,6 +184,14 @@ bool stream_capturing(cudaStream_t st) {
 
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
+// Test hook (PION_B200_TEST_STALL=1): one CTA of the next main passes waits on a
+// barrier nothing arrives on, so the wait runs out after the context's budget and the
+// call reports PION_B200_ETIMEOUT (no fault, the GPU stays usable).
+int test_stall() {
+    const char* e = getenv("PION_B200_TEST_STALL");
+    return e && atoi(e) == 1 ? 1 : 0;
+}
+
 int timing_begin(pion_b200_ctx* ctx, int tag) {
     if (!ctx->timing) return -1;
     if (ctx->ev_used == ctx->ev_start.size()) {
@@ -500,14 +508,6 @@ int pion_v_b200_register_flat_i8(pion_b200_ctx* ctx, const int8_t* rows, const f
     }
     *out_index = ix;
     return 0;
-}
-
-// Test hook (PION_B200_TEST_STALL=1): one CTA of the next main passes waits on a
-// barrier nothing arrives on, so the wait runs out after the context's budget and the
-// call reports PION_B200_ETIMEOUT (no fault, the GPU stays usable).
-static int test_stall() {
-    const char* e = getenv("PION_B200_TEST_STALL");
-    return e && atoi(e) == 1 ? 1 : 0;
 }
 
 // Forced path selection for tests: 0 auto, 1 one-query scan, 2 tensor-core kernel.

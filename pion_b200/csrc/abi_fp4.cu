@@ -209,6 +209,7 @@ Fp4Product product_of(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n
     L.nq = (int)nq;
     L.status = call_status(ctx, mem);
     L.wait_ns = ctx->wait_ns;
+    L.test_stall = test_stall();
     L.num_sms = ctx->num_sms;
     return L;
 }

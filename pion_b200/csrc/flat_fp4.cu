@@ -97,6 +97,7 @@ struct TcParams {
     uint64_t* cand;           // [nq][CAP]: approximate score bits << 32 | row
     int* status;
     uint64_t wait_ns;
+    int test_stall;           // the first pair's issuer waits on a barrier nothing arrives on
 };
 
 // ------------------------------------------------------------- PTX pieces --
@@ -364,7 +365,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint64_t* bfull = tempty + 2;
     uint64_t* qsf_done = bfull + 1;
     uint64_t* drain = qsf_done + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* stall = drain + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stall + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);  // warp-uniform
@@ -393,6 +395,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         mbar_init(bfull, 1);
         mbar_init(qsf_done, SCALE_WARPS);
         mbar_init(drain, 1);
+        mbar_init(stall, 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -508,11 +511,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     }
                 }
             }
-            // Every copy this thread issued lands before the CTA may exit.
-            mbar_wait(bfull, 0, p.status, nullptr, p.wait_ns);
+            // Every copy this thread issued lands before the CTA may exit (a wait of its own
+            // length: the caller's budget may have run out).
+            mbar_wait(bfull, 0, p.status, nullptr, kWaitBudgetNs);
             for (int s = 0; s < stages; ++s)
                 if ((issued >> s) & 1u)
-                    mbar_wait(&full[s], (parity >> s) & 1u, p.status, nullptr, p.wait_ns);
+                    mbar_wait(&full[s], (parity >> s) & 1u, p.status, nullptr, kWaitBudgetNs);
         } else if (warp == 5 && rank == 0) {
             // --------------------------------------------------- MMA issuer
             // The whole warp runs the loop, so that every operand is in a uniform register; one
@@ -525,7 +529,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const bool one = elect_one();
             int stage = 0, set = 0, buf = 0;
             uint32_t set_phase = 0, buf_phase = 0;
-            bool ok = true;
+            bool ok = !p.test_stall || blockIdx.x != 0;
+            if (!ok) mbar_wait(stall, 0, p.status, abort_flag, p.wait_ns);
             for (int j = first; j < p.n_tiles && ok; j += stride) {
                 if (!__all_sync(0xffffffffu, mbar_wait(&tempty[buf], buf_phase ^ 1u, p.status,
                                                        abort_flag, p.wait_ns)))
@@ -576,7 +581,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             // All MMAs issued above complete before TMEM is released.
             if (one) tc_commit_pair(drain);
             __syncwarp();
-            mbar_wait(drain, 0, p.status, nullptr, p.wait_ns);
+            mbar_wait(drain, 0, p.status, nullptr, kWaitBudgetNs);
+        } else if (warp == 5) {
+            // The other CTA stays until the last arrival on its barriers is in.
+            mbar_wait(drain, 0, p.status, nullptr, kWaitBudgetNs);
         }
         __syncwarp();
     } else {
@@ -678,18 +686,19 @@ __device__ __forceinline__ uint32_t warp_kth_of(int m, int k, F value) {
     return warp_kth<V>(v, k);
 }
 
-// The k-th largest of n <= LIST values in shared memory, by a CTA of NT threads: one warp's search of up
-// to 1024, else the same search by all with a barrier a bit.
+// The k-th largest of n <= LIST values in shared memory, by a CTA of NT threads: one warp's search of few,
+// else the same search by all with a barrier a bit.
 template <int NT>
 __device__ uint32_t list_kth(const uint32_t* list, int n, int k) {
+    constexpr int MOST = NT > 256 ? 32 : 16;  // values a lane holds
     __shared__ uint32_t s_kth;
     __shared__ int s_bit[32];
-    if (n <= 1024) {
+    if (n <= 32 * MOST) {
         if (threadIdx.x < 32) {
             auto at = [&](int i) { return list[i]; };
             const uint32_t x = n <= 64    ? warp_kth_of<2>(n, k, at)
                                : n <= 256 ? warp_kth_of<8>(n, k, at)
-                                          : warp_kth_of<32>(n, k, at);
+                                          : warp_kth_of<MOST>(n, k, at);
             if (threadIdx.x == 0) s_kth = x;
         }
         __syncthreads();
@@ -1013,7 +1022,7 @@ __device__ __forceinline__ void write_best(const FinishParams& p, int t, const u
 // the k best are scored exactly and sorted.  A query with more than LIST of those, or whose
 // candidates overflowed, is left to rescue_kernel.
 template <int FMT, int NT>
-__global__ void __launch_bounds__(NT) finish_kernel(const FinishParams p) {
+__global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const FinishParams p) {
     __shared__ __align__(16) uint64_t key[LIST];
     __shared__ int s_warp[NT / 32];
     __shared__ int s_n;
@@ -1237,7 +1246,7 @@ static bool make_plan(int fmt, int dp, int nq, int64_t n_tiles, Plan* out) {
     const int aps = atoms_per_stage(fmt), steps = dp / 64;
     const int kchunks = (dp / 2 + KC - 1) / KC;
     const int stage = A_BYTES + aps * 512;
-    const int fixed = 1024 + 2 * MAX_NT * 4 + EPI_WARPS * HITS * 9 + (4 * MAX_STAGES + 8) * 8 + 64;
+    const int fixed = 1024 + 2 * MAX_NT * 4 + EPI_WARPS * HITS * 9 + (4 * MAX_STAGES + 9) * 8 + 64;
     constexpr int64_t pairs = 74;  // of the B200's 148 SMs
     double best = 0.0;
     bool any = false;
@@ -1340,6 +1349,7 @@ int launch_fp4_product(const Fp4Product& L, cudaStream_t st) {
     p.cand = L.cand;
     p.status = L.status;
     p.wait_ns = L.wait_ns;
+    p.test_stall = L.test_stall;
     // Pairs per query tile: one wave where there are enough SMs.  The query tiles of one row
     // tile run beside each other, so that the rows come from HBM once.
     int64_t per = L.num_sms / 2 / s.n_qt;

@@ -307,6 +307,7 @@ int* call_status(pion_b200_ctx* ctx, int mem);
 int finish_sync(pion_b200_ctx* ctx);
 bool valid_ctx(const pion_b200_ctx* ctx);
 bool stream_capturing(cudaStream_t st);
+int test_stall();  // PION_B200_TEST_STALL=1
 int use_device(pion_b200_ctx* ctx);
 size_t align_up(size_t x, size_t a);
 int prepass_tiles(int k);
@@ -532,6 +533,7 @@ struct Fp4Product {
     uint64_t* cand = nullptr;
     int* status = nullptr;
     uint64_t wait_ns = kDefaultWaitNs;
+    int test_stall = 0;
     int num_sms = 148;
 };
 int launch_fp4_product(const Fp4Product& L, cudaStream_t st);

@@ -205,7 +205,7 @@ class FP4Rows:
              dtype=None, out=None):
         """Slots ``slots``, or ``count`` slots from ``start`` (default: all), as rows [n, dim] of
         ``dtype`` (default float32) on the store's device, or into ``out``.  An empty slot
-        reads as NaN; a negative one leaves its row of ``out`` as it was."""
+        reads as NaN; a negative one leaves its row of ``out`` as it was (undefined without)."""
         ps = None
         if slots is not None:
             slots = _slots(ctx, slots, MEM_DEVICE)

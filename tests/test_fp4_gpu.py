@@ -34,6 +34,12 @@ def rows_np(n, dim, seed):
     return x * np.exp(rng.standard_normal((n, dim)) * 0.5)
 
 
+def finish(ctx):
+    """Waits for torch's streams, then takes what the calls' kernels have reported."""
+    torch.cuda.synchronize()
+    ctx.sync()
+
+
 def unpack(rows):
     c = rows.codes.cpu().numpy()
     return np.stack((c & 15, c >> 4), 2).reshape(len(c), -1)
@@ -71,7 +77,7 @@ def test_write_and_read(ctx, fmt, dtype, n, dim, pad):
     rows = pion_b200.FP4Rows(n + 5, dim, fmt)
     slots = np.random.default_rng(1).permutation(n + 5)[:n]
     rows.write(ctx, src, slots=torch.from_numpy(slots).cuda())
-    ctx.sync()
+    finish(ctx)
     codes, bits, g = check_store(rows, slots, exact, fmt)
     rest = np.setdiff1d(np.arange(n + 5), slots)
     assert np.isnan(rows.row_scale.cpu().numpy()[rest]).all()
@@ -150,7 +156,7 @@ def test_slots_repeated_skipped_and_out_of_range(ctx):
         slots[::7] = -1
         rows.write(ctx, t if on_gpu else t.cpu(),
                    slots=torch.from_numpy(slots).cuda() if on_gpu else slots)
-        ctx.sync()
+        finish(ctx)
         last = {s: i for i, s in enumerate(slots.tolist()) if s >= 0}
         at = np.array(sorted(last))
         check_store(rows, at, exact[[last[s] for s in at.tolist()]], "nv")
@@ -161,12 +167,12 @@ def test_slots_repeated_skipped_and_out_of_range(ctx):
         rows.write(ctx, x.astype(np.float32), slots=slots)       # host: refused
     rows.write(ctx, t, slots=torch.from_numpy(slots).cuda())      # device: skipped, reported
     with pytest.raises(pion_b200.PionError) as e:
-        ctx.sync()
+        finish(ctx)
     assert e.value.code == -1
     out = torch.full((2, 64), 5.0, device="cuda")
     rows.read(ctx, slots=torch.tensor([-1, 45]).cuda(), out=out)
     with pytest.raises(pion_b200.PionError):
-        ctx.sync()
+        finish(ctx)
     assert (out == 5.0).all()
     for a, b in zip(before, (rows.codes, rows.scales, rows.row_scale)):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
@@ -194,7 +200,7 @@ def test_scores(ctx, fmt, n, dim, nq, types):
     rows.write(ctx, tx)
     want, size = plain.products(eq, ex, fmt)
     got = pion_b200.fp4_scores(ctx, rows, tq_, dtype=TYPES[to])
-    ctx.sync()
+    finish(ctx)
     got = got.double().cpu().numpy()
     assert np.isneginf(got[:, n:]).all()
     got = got[:, :n]
@@ -209,7 +215,7 @@ def test_scores(ctx, fmt, n, dim, nq, types):
     m = max(1, n // 2)
     wide = torch.full((nq, m + 5), 7.0, dtype=TYPES[to], device="cuda")
     pion_b200.fp4_scores(ctx, rows, tq_, n_rows=m, out=wide[:, :m])
-    ctx.sync()
+    finish(ctx)
     full = pion_b200.fp4_scores(ctx, rows, tq_, dtype=TYPES[to])
     assert torch.equal(wide[:, :m], full[:, :m]) and (wide[:, m:] == 7.0).all()
 
@@ -241,7 +247,7 @@ def test_scores_error_bound_of_the_search(ctx):
 def check_knn(ctx, rows, q, exact_q, exact_x, fmt, k, n_rows=None, id_base=0):
     import pion_b200
     ids, sc = pion_b200.FlatFP4Index(ctx, rows, id_base=id_base).search(q, k, n_rows=n_rows)
-    ctx.sync()
+    finish(ctx)
     n = len(exact_x) if n_rows is None else n_rows
     want, _ = plain.products(exact_q, exact_x[:n], fmt)
     wi, wv = plain.best(want, k)
@@ -322,6 +328,111 @@ def test_knn_overflowing_candidates(ctx, fmt):
     check_knn(ctx, rows, tq, eq, ex, fmt, 10)
 
 
+def test_many_overflowing_queries(ctx):
+    """More flagged queries than the rescue's CTAs, and fewer; beside ordinary ones."""
+    import pion_b200
+    rng = np.random.default_rng(16)
+    x = rng.standard_normal((9000, 48))
+    x[::2] = x[0]
+    tx, ex = typed(x, "f32")
+    rows = pion_b200.quantize_rows_fp4(ctx, tx, "nv")
+    for nq, same in ((700, 400), (90, 2)):
+        q = rng.standard_normal((nq, 48))
+        q[nq - same:] = x[0] + 0.01 * rng.standard_normal((same, 48))
+        tq, eq = typed(q, "f32")
+        check_knn(ctx, rows, tq, eq, ex, "nv", 33)
+
+
+def test_wait_that_runs_out(ctx, monkeypatch):
+    """One pair's issuer waits on a barrier that nothing arrives on: the product gives up after
+    the budget, drains and reports it; the next call is right."""
+    import pion_b200
+    x, q = mixture_np(20000, 512, 30, seed=4, n_queries=300)
+    tx, tq = torch.from_numpy(x).cuda(), torch.from_numpy(q).cuda()
+    rows = pion_b200.quantize_rows_fp4(ctx, tx, "nv")
+    ix = pion_b200.FlatFP4Index(ctx, rows)
+    ids, sc = ix.search(tq, 10)
+    full = pion_b200.fp4_scores(ctx, rows, tq)
+    finish(ctx)
+    ctx.set_wait_budget(1_000_000)
+    try:
+        for nq in (300, 1):
+            monkeypatch.setenv("PION_B200_TEST_STALL", "1")
+            pion_b200.fp4_scores(ctx, rows, tq[:nq])
+            with pytest.raises(pion_b200.PionError) as e:
+                finish(ctx)
+            assert e.value.code == -11
+            ix.search(tq[:nq], 10)
+            with pytest.raises(pion_b200.PionError):
+                finish(ctx)
+            with pytest.raises(pion_b200.PionError):
+                ix.search(q[:nq], 10)                    # host memory: reported by the call
+            monkeypatch.delenv("PION_B200_TEST_STALL")
+            again, sc2 = ix.search(tq, 10)
+            assert torch.equal(again, ids) and torch.equal(sc2, sc)
+            assert torch.equal(pion_b200.fp4_scores(ctx, rows, tq), full)
+            finish(ctx)
+    finally:
+        monkeypatch.delenv("PION_B200_TEST_STALL", raising=False)
+        ctx.set_wait_budget(0)
+
+
+def test_refusals(ctx):
+    import pion_b200
+    from pion_b200 import _lib
+    rows = pion_b200.FP4Rows(100, 64, "nv")
+    x = torch.zeros((10, 64), device="cuda")
+    ix = pion_b200.FlatFP4Index(ctx, rows)
+    for bad in (lambda: rows.write(ctx, x, start=91), lambda: rows.write(ctx, x, start=-1),
+                lambda: rows.read(ctx, start=95, count=6), lambda: rows.read(ctx, start=-1, count=2),
+                lambda: pion_b200.fp4_scores(ctx, rows, x, n_rows=101),
+                lambda: ix.search(x, 0), lambda: ix.search(x, 257), lambda: ix.search(x, 5, n_rows=101),
+                lambda: pion_b200.FlatFP4Index(ctx, rows, id_base=-1).search(x, 1),
+                lambda: pion_b200.FlatFP4Index(ctx, rows, id_base=2 ** 31 - 50).search(x, 1)):
+        with pytest.raises(pion_b200.PionError):
+            bad()
+    for bad, err in ((lambda: rows.write(ctx, x[:, :63]), ValueError),
+                     (lambda: rows.write(ctx, x.double()), TypeError),
+                     (lambda: rows.write(ctx, x, slots=[1, 2]), ValueError),
+                     (lambda: rows.write(ctx, x, slots=torch.zeros(10, device="cuda")), TypeError),
+                     (lambda: rows.read(ctx, slots=[1], dtype=torch.float64), TypeError),
+                     (lambda: rows.read(ctx, slots=[1], out=torch.zeros((2, 64), device="cuda")), ValueError),
+                     (lambda: pion_b200.fp4_scores(ctx, rows, x, out=torch.zeros((10, 100))), ValueError),
+                     (lambda: pion_b200.fp4_scores(ctx, rows, x[0]), ValueError)):
+        with pytest.raises(err):
+            bad()
+    # a stream of its own needs a workspace; one that is too small is refused
+    out = torch.empty((10, 100), device="cuda")
+    call = lambda ws, n: ctx.lib.pion_v_b200_fp4_scores(  # noqa: E731
+        ctx.h, rows._ref(ctx), 100, x.data_ptr(), 0, 64, 10, out.data_ptr(), 0, 100, ws, n, 1, 1)
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    assert call(None, 0) == _lib.EINVAL
+    assert call(ws.data_ptr(), 100) == _lib.EINVAL
+    assert call(ws.data_ptr() + 8, 1 << 19) == _lib.EINVAL
+    assert call(ws.data_ptr(), 1 << 20) == 0
+    # the context's own stream and scratch
+    torch.cuda.synchronize()
+    assert ctx.lib.pion_v_b200_fp4_scores(ctx.h, rows._ref(ctx), 100, x.data_ptr(), 0, 64, 10,
+                                          out.data_ptr(), 0, 100, None, 0, 1, None) == 0
+    finish(ctx)
+    assert torch.isneginf(out).all()
+    for bad in (lambda: ctx.lib.pion_v_b200_fp4_write(ctx.h, rows._ref(ctx), x.data_ptr(), 3, 64, 1,
+                                                      None, 0, 1, 1),
+                lambda: ctx.lib.pion_v_b200_fp4_write(ctx.h, rows._ref(ctx), x.data_ptr(), 0, 63, 2,
+                                                      None, 0, 1, 1),
+                lambda: ctx.lib.pion_v_b200_fp4_write(ctx.h, rows._ref(ctx), None, 0, 64, 1, None, 0,
+                                                      1, 1),
+                lambda: ctx.lib.pion_v_b200_fp4_write(ctx.h, rows._ref(ctx), x.data_ptr() + 2, 0, 64,
+                                                      1, None, 0, 1, 1),
+                lambda: ctx.lib.pion_v_b200_fp4_write(ctx.h, rows._ref(ctx), x.data_ptr(), 0, 64, -1,
+                                                      None, 0, 1, 1),
+                lambda: ctx.lib.pion_v_b200_fp4_write(ctx.h, rows._ref(ctx), x.data_ptr(), 0, 64, 1,
+                                                      None, 0, 2, 1),
+                lambda: ctx.lib.pion_v_b200_fp4_write(ctx.h, None, x.data_ptr(), 0, 64, 1, None, 0, 1,
+                                                      1)):
+        assert bad() == _lib.EINVAL
+
+
 def test_host_arrays(ctx):
     import pion_b200
     x, q = mixture_np(9000, 200, 30, seed=1, n_queries=20)
@@ -333,6 +444,8 @@ def test_host_arrays(ctx):
     assert isinstance(s, np.ndarray) and np.array_equal(s, d.cpu().numpy())
     rows.write(ctx, q, slots=np.arange(20) * 3)
     check_store(rows, np.arange(20) * 3, q, "mx")
+    rows.write(ctx, x[::-1][:50, ::1], start=100)          # a view with negative strides
+    check_store(rows, np.arange(100, 150), x[::-1][:50], "mx")
 
 
 def test_large_batches_are_searched_in_chunks(ctx):
@@ -429,7 +542,7 @@ def test_ingest_search_and_rerank_together(ctx):
         short, _ = plain.best(want, 64)
         assert np.array_equal(ids.cpu().numpy(), short)
         got, scores = f32.merge_delta(tq, 30000, ids, sc, 10)
-        ctx.sync()
+        finish(ctx)
         # the ten nearest of the shortlist: float32 distances of unit vectors, 1536 terms
         got, scores = got.cpu().numpy(), scores.cpu().numpy()
         mine = np.take_along_axis(cos, short, 1)
