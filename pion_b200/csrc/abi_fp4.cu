@@ -91,15 +91,17 @@ bool plan_scratch(int format, int dim, int64_t n_rows, int64_t nq, int64_t k, Sc
     s.q_norm = take((size_t)nq * 4);
     s.theta = s.cand_n = s.n_flagged = s.flagged = s.done = s.parts = s.sample = s.cand = 0;
     if (k > 0) {
-        const int64_t most = (int64_t)fp4_sample_tiles((int)nq) * fp4_tile_rows();
+        const bool split = fp4_splits(nq, n_rows, k);
+        const int64_t most = split ? (n_rows + 3) / 4 * 4
+                                   : (int64_t)fp4_sample_tiles((int)nq) * fp4_tile_rows();
         s.theta = take((size_t)nq * 4);
-        s.cand_n = take((size_t)nq * 4);
-        s.n_flagged = take(4);
+        s.n_flagged = take((size_t)(nq + 1) * 4);
+        s.cand_n = s.n_flagged + 4;
         s.flagged = take((size_t)nq * 4);
         s.done = take((size_t)nq * 4);
         s.parts = take((size_t)fp4_rescue_items(nq) * k * 8);
-        s.sample = take((size_t)nq * (n_rows < most ? n_rows : most) * 4);
-        if (n_rows > most) s.cand = take((size_t)nq * fp4_cap() * 8);
+        s.sample = take((size_t)nq * (n_rows < most && !split ? n_rows : most) * 4);
+        if (split || n_rows > most) s.cand = take((size_t)nq * fp4_cap() * 8);
     }
     s.total = off;
     *out = s;
@@ -214,8 +216,9 @@ Fp4Product product_of(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n
     return L;
 }
 
-// One chunk of queries: the threshold of each from a sample of the rows, tightened over
-// growing parts of them, then the rows that reach it, then the k best of those exactly.
+// One chunk of queries: the candidates of each -- from the scores of every row where those are
+// few, else the rows that reach a threshold taken from a sample of them and tightened over
+// growing parts -- then the k best of those exactly.
 int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, int64_t id_base,
               const void* q, int q_type, int64_t q_stride, int64_t nq, int64_t k, int32_t* ids,
               float* scores, const Scratch& s, char* base, int mem) {
@@ -231,18 +234,25 @@ int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, i
 
     const int64_t n_tiles = (n_rows + fp4_tile_rows() - 1) / fp4_tile_rows();
     const int samples = fp4_sample_tiles((int)nq);
-    const bool dense = n_tiles <= samples;
-    const int64_t m = dense ? n_rows : (int64_t)samples * fp4_tile_rows();
+    const bool split = fp4_splits(nq, n_rows, k);
+    const bool dense = !split && n_tiles <= samples;
+    const int64_t m = split   ? (n_rows + 3) / 4 * 4
+                      : dense ? n_rows
+                              : (int64_t)samples * fp4_tile_rows();
     timing_begin(ctx);
     Fp4Product L = product_of(ctx, r, n_rows, nq, s, base, mem);
-    L.n_tiles = (int)(dense ? n_tiles : samples);
-    L.tile_step = dense ? 1 : (int)(n_tiles / samples);
+    L.n_tiles = (int)(split || dense ? n_tiles : samples);
+    L.tile_step = split || dense ? 1 : (int)(n_tiles / samples);
     L.out = sample;
     L.out_type = PION_B200_F32;
     L.ld = m;
     rc = launch_fp4_product(L, st);
     ctx->launches++;
-    if (!dense && rc == 0) {
+    if (split && rc == 0) {
+        rc = launch_fp4_split(sample, m, n_rows, (int)k, (int)r->dim, q_scale, s.plan.nt,
+                              s.plan.nt_pad, q_norm, r->norm_max, (int)nq, cand, cand_n, st);
+        ctx->launches++;
+    } else if (!dense && rc == 0) {
         rc = launch_fp4_theta(sample, nullptr, (int)k, (int)r->dim, q_scale, s.plan.nt,
                               s.plan.nt_pad, q_norm, r->norm_max, (int)nq, theta, cand_n, st);
         ctx->launches++;

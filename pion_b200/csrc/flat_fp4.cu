@@ -399,6 +399,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         *abort_flag = 0;
         fence_barrier_init();
     }
+    if (warp == 5) tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    // Up to here nothing of an earlier kernel's is read.
     griddep_launch();
     griddep_wait();
     for (int j = threadIdx.x; j < MAX_NT; j += THREADS) {
@@ -407,11 +413,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         s_gq[j] = ok ? __ldcg(p.q_scale + (int64_t)qt * p.plan.nt_pad + j) : 0.0f;
         s_th[j] = ok && mode == kCollect ? __ldcg(p.theta + t) : INFINITY;
     }
-    if (warp == 5) tmem_alloc_pair(tmem_slot, TMEM_COLS);
-    tc_fence_before();
-    cluster_sync();
-    tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    __syncthreads();
 
     if (warp < SCALE_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_SCALE));
@@ -920,6 +922,76 @@ __global__ void __launch_bounds__(SEL)
     if (threadIdx.x == 0) theta[t] = threshold_of(x, two_eps, gq);
 }
 
+// Few queries: the candidates straight from the scores of every row, a chunk of SPLIT rows per
+// CTA.  A row among the k best overall is among the k best of its chunk, so its approximate
+// score is at least the chunk's k-th best less 2 eps; for that the k-th largest of the
+// threads' maxima does, a lower bound of it that few scores reach.
+constexpr int SPLIT = 8192;
+__global__ void __launch_bounds__(SEL)
+    split_kernel(const float* scores, int64_t ld, int64_t n_rows, int k, int dp,
+                 const float* q_scale, int nt, int nt_pad, const float* q_norm,
+                 const float* norm_max, uint64_t* cand, int* cand_n) {
+    constexpr int V4 = SPLIT / SEL / 4;
+    __shared__ uint32_t list[SEL];
+    __shared__ float s_cut;
+    __shared__ int s_count, s_base;
+    __shared__ uint64_t s_cand[LIST];
+    griddep_launch();
+    griddep_wait();
+    const int t = blockIdx.y;
+    const int64_t first = (int64_t)blockIdx.x * SPLIT;
+    const float* s = scores + (int64_t)t * ld + first;
+    const int64_t left = n_rows - first;
+    float4 v[V4];
+#pragma unroll
+    for (int i = 0; i < V4; ++i) {  // ld is a multiple of 4: whole vectors lie inside the row
+        const int at = 4 * (int)(threadIdx.x + i * SEL);
+        v[i] = at < left ? __ldcg(reinterpret_cast<const float4*>(s + at))
+                         : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (at + 1 >= left) v[i].y = -INFINITY;
+        if (at + 2 >= left) v[i].z = -INFINITY;
+        if (at + 3 >= left) v[i].w = -INFINITY;
+    }
+    const float gq = __ldcg(q_scale + query_slot(t, nt, nt_pad));
+    const float two_eps = 2.0f * eps_of(dp, __ldcg(q_norm + t), __ldcg(norm_max));
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V4; ++i)
+        most = fmaxf(most, fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w)));
+    list[threadIdx.x] = ordered(most);
+    if (threadIdx.x == 0) s_count = 0;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const uint32_t x = warp_kth_of<8>(SEL, k, [&](int i) { return list[i]; });
+        if (threadIdx.x == 0) s_cut = unordered(x) - two_eps;
+    }
+    __syncthreads();
+    if (!(gq > 0.0f)) return;  // an empty or zero query collects nothing
+    const float cut = s_cut;
+    auto keep = [&](float x, int at) {
+        if (x >= cut && x > -INFINITY) {
+            const int to = atomicAdd(&s_count, 1);
+            if (to < LIST)
+                s_cand[to] = ((uint64_t)__float_as_uint(x) << 32) | (uint32_t)(first + at);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < V4; ++i) {
+        const int at = 4 * (int)(threadIdx.x + i * SEL);
+        keep(v[i].x, at);
+        keep(v[i].y, at + 1);
+        keep(v[i].z, at + 2);
+        keep(v[i].w, at + 3);
+    }
+    __syncthreads();
+    // more than LIST in one chunk overflow the query's list: the rescue's to answer
+    if (threadIdx.x == 0) s_base = atomicAdd(cand_n + t, s_count > LIST ? CAP + 1 : s_count);
+    __syncthreads();
+    const int n = min(s_count, LIST);
+    for (int i = threadIdx.x; i < n; i += SEL)
+        if (s_base + i < CAP) cand[(int64_t)t * CAP + s_base + i] = s_cand[i];
+}
+
 struct FinishParams {
     const uint8_t* codes;
     const uint8_t* scales;
@@ -1033,12 +1105,19 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const Fini
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int W = NT / 32;
     const int64_t qs = query_slot(t, p.nt, p.nt_pad);
+    // Every load that does not wait for another: the candidates' places, however many there are.
+    constexpr int V = LIST / NT;
+    const uint64_t* cand = p.cand + (int64_t)t * CAP;
+    uint64_t c[V];
+#pragma unroll
+    for (int u = 0; u < V; ++u) c[u] = p.dense ? 0 : __ldcg(cand + threadIdx.x + u * NT);
     const float gq = __ldcg(p.q_scale + qs);
     const int m = p.dense ? (int)p.n_rows : __ldcg(p.cand_n + t);
     const float two_eps = 2.0f * eps_of(p.dp, __ldcg(p.q_norm + t), __ldcg(p.norm_max));
     QueryShared q;
     q.codes = reinterpret_cast<int8_t*>(dyn);
     q.scales = reinterpret_cast<float*>(dyn + p.dp);
+    if (warp > 0) load_query<FMT, NT - 32>(p, q, qs, threadIdx.x - 32);
     if (threadIdx.x == 0) s_n = 0;
 
     int found = 0;
@@ -1047,7 +1126,6 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const Fini
         bool whole = !p.dense && (m > CAP || !known);
         if (!whole) {
             const float* dense = p.dense + (int64_t)t * p.ld;
-            const uint64_t* cand = p.cand + (int64_t)t * CAP;
             auto approx = [&](int i) {
                 return p.dense ? __ldcg(dense + i)
                                : __uint_as_float((uint32_t)(__ldcg(cand + i) >> 32));
@@ -1061,25 +1139,24 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const Fini
             };
             auto cut_of = [&](uint32_t o) { return o ? unordered(o) - two_eps : -INFINITY; };
             if (!p.dense && m <= LIST) {
-                // candidates in registers; the first warp searches while the others load the query
-                constexpr int V = LIST / NT;
-                uint64_t c[V];
 #pragma unroll
                 for (int u = 0; u < V; ++u) {
                     const int i = threadIdx.x + u * NT;
-                    c[u] = i < m ? __ldcg(cand + i) : 0;
                     if (i < m) list[i] = ordered_score(__uint_as_float((uint32_t)(c[u] >> 32)));
                 }
                 __syncthreads();
-                if (warp > 0) load_query<FMT, NT - 32>(p, q, qs, threadIdx.x - 32);
-                const float cut = m > p.k ? cut_of(list_kth<NT>(list, m, p.k)) : -INFINITY;
+                // (a thread's values of the list are its own until all are in registers)
+                const float cut =
+                    m <= p.k    ? -INFINITY
+                    : m <= 1024 ? cut_of(list_kth<NT>(list, m, p.k))
+                                : cut_of(kth_largest<NT, V>(m, p.k, list, [&](int i) { return list[i]; }));
                 __syncthreads();
 #pragma unroll
                 for (int u = 0; u < V; ++u)
                     if ((int)threadIdx.x + u * NT < m)
                         take(__uint_as_float((uint32_t)(c[u] >> 32)), cut, c[u] & 0xFFFFFFFFu);
             } else {
-                load_query<FMT, NT>(p, q, qs, threadIdx.x);
+                __syncthreads();
                 float cut = -INFINITY;
                 if (m > p.k)
                     cut = cut_of(kth_largest<NT, 8>(
@@ -1382,6 +1459,22 @@ int launch_fp4_theta(const float* sample, const uint64_t* cand, int k, int dim,
     static_assert(32 * ROWS == 256 * 8 * 4, "sample");
     return launch_pdl(theta_sample_kernel<256, 8>, dim3((unsigned)nq), 256, 0, st, sample, k, dp,
                       q_scale, nt, nt_pad, q_norm, norm_max, theta, cand_n);
+}
+
+// Whether the scores of every row are written and split (they and the second pass over them
+// cost less than a sample's own launch and selection), and the chunks' candidates fit.
+bool fp4_splits(int64_t nq, int64_t n_rows, int64_t k) {
+    const int64_t chunks = (n_rows + fp4::SPLIT - 1) / fp4::SPLIT;
+    return chunks > 2 && nq * n_rows <= (int64_t)1 << 22 && chunks * k <= fp4::CAP / 2;
+}
+
+int launch_fp4_split(const float* scores, int64_t ld, int64_t n_rows, int k, int dim,
+                     const float* q_scale, int nt, int nt_pad, const float* q_norm,
+                     const float* norm_max, int nq, uint64_t* cand, int* cand_n, cudaStream_t st) {
+    using namespace fp4;
+    const dim3 grid((unsigned)((n_rows + SPLIT - 1) / SPLIT), (unsigned)nq);
+    return launch_pdl(split_kernel, grid, SEL, 0, st, scores, ld, n_rows, k, pad_dim(dim), q_scale,
+                      nt, nt_pad, q_norm, norm_max, cand, cand_n);
 }
 
 int64_t fp4_rescue_items(int64_t nq) { return nq > fp4::RESCUE_CTAS ? nq : fp4::RESCUE_CTAS; }

@@ -209,7 +209,7 @@ struct WriteParams {
     float* row_scale;
     float* norm;           // per row (queries), or null
     float* norm_max;       // the store's bound, or null
-    int* zero;             // set to 0, or null
+    int* zero;             // n + 1 integers set to 0, or null
     int* status;
 };
 
@@ -242,7 +242,10 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
     T* stage = stage_all + (VEC ? 0 : warp * STEP);
     const int64_t i = WPR == 1 ? (int64_t)blockIdx.x * WARPS + warp : blockIdx.x;
     if (i >= p.n) return;
-    if (p.zero && i == 0 && threadIdx.x == 0) *p.zero = 0;
+    if (p.zero && lane == 0 && (WPR == 1 || warp == 0)) {
+        p.zero[i + 1] = 0;
+        if (i == 0) p.zero[0] = 0;
+    }
     int64_t slot;
     if (p.tile > 0) {
         slot = query_slot(i, p.tile, p.tile_pad);

@@ -481,7 +481,7 @@ struct Fp4Write {
     float* row_scale = nullptr;
     float* norm = nullptr;
     float* norm_max = nullptr;
-    int* zero = nullptr;         // an integer that the first kernel sets to 0
+    int* zero = nullptr;         // integers that the kernel sets to 0, one for each row and one more
     int* status = nullptr;
 };
 int launch_fp4_write(const Fp4Write& w, cudaStream_t st);
@@ -544,6 +544,10 @@ int fp4_sample_tiles(int nq);
 int launch_fp4_theta(const float* sample, const uint64_t* cand, int k, int dim,
                      const float* q_scale, int nt, int nt_pad, const float* q_norm,
                      const float* norm_max, int nq, float* theta, int* cand_n, cudaStream_t st);
+bool fp4_splits(int64_t nq, int64_t n_rows, int64_t k);
+int launch_fp4_split(const float* scores, int64_t ld, int64_t n_rows, int k, int dim,
+                     const float* q_scale, int nt, int nt_pad, const float* q_norm,
+                     const float* norm_max, int nq, uint64_t* cand, int* cand_n, cudaStream_t st);
 struct Fp4Finish {
     int format = 0;
     int dim = 0;

@@ -262,7 +262,9 @@ def check_knn(ctx, rows, q, exact_q, exact_x, fmt, k, n_rows=None, id_base=0):
 @pytest.mark.parametrize("n,dim,nq,k,dtype", [
     (1, 16, 1, 1, "f32"), (5, 100, 3, 10, "f32"), (1000, 1536, 1, 10, "bf16"),
     (8192, 128, 33, 64, "f32"), (8193, 130, 5, 256, "f16"), (8320, 64, 3, 1, "f32"),
-    (20011, 384, 209, 10, "f32"), (60000, 256, 16, 256, "f32"), (150000, 96, 7, 100, "f32")])
+    (20011, 384, 209, 10, "f32"), (60000, 256, 16, 256, "f32"), (150000, 96, 7, 100, "f32"),
+    (300003, 40, 20, 10, "f32"), (90001, 64, 60, 256, "f32"), (70000, 100, 150, 33, "bf16"),
+    (24577, 200, 1, 10, "f32"), (24576, 200, 4, 1, "f32")])
 def test_knn(ctx, fmt, n, dim, nq, k, dtype):
     import pion_b200
     x, q = mixture_np(n, dim, max(1, n // 200), seed=n + k, n_queries=nq)
@@ -321,6 +323,13 @@ def test_knn_overflowing_candidates(ctx, fmt):
     tx, ex = typed(x, "f32")
     rows = pion_b200.quantize_rows_fp4(ctx, tx, fmt)
     check_knn(ctx, rows, tq, eq, ex, fmt, 10)
+    many = np.repeat(eq, 50, 0)                           # the same with sampled thresholds
+    check_knn(ctx, rows, typed(many, "f32")[0], many, ex, fmt, 10)
+    x[n // 2:] = x[5]                                     # a chunk of equal rows
+    tx, ex = typed(x, "f32")
+    rows = pion_b200.quantize_rows_fp4(ctx, tx, fmt)
+    near = ex[5:6]
+    check_knn(ctx, rows, typed(near, "f32")[0], near, ex, fmt, 10)
     x = rng.standard_normal((10000, 64)) * 2.0 ** 63
     tx, ex = typed(x, "f32")
     tq, eq = typed(q * 2.0 ** 62, "f32")
