@@ -666,9 +666,13 @@ __device__ __forceinline__ uint32_t warp_kth(const uint32_t (&v)[V], int k) {
 #pragma unroll 1
     for (int b = 31; b >= 0; --b) {
         const uint32_t y = x | (1u << b);
-        int c = 0;
+        constexpr int S = V < 4 ? V : 4;  // independent sums
+        int part[S] = {};
 #pragma unroll
-        for (int i = 0; i < V; ++i) c += v[i] >= y;
+        for (int i = 0; i < V; ++i) part[i % S] += v[i] >= y;
+        int c = part[0];
+#pragma unroll
+        for (int i = 1; i < S; ++i) c += part[i];
         c = __reduce_add_sync(0xffffffffu, c);
         if (c >= k) x = y;
         if (c == k) break;
@@ -1025,39 +1029,59 @@ struct QueryShared {
     float* scales;
 };
 
-// sum_j q_j v_j in units of both g, by one warp: exact integer sums per block, float64 over
-// the blocks.
+// sum_j q_j v_j in units of both g, by half a warp (`sub`: the lane's place in it): exact integer
+// sums per block, float64 over the blocks.  A lane's loads of 64 blocks of 32 elements are in
+// flight together.
 template <int FMT>
-__device__ __forceinline__ double warp_dot(const FinishParams& p, const QueryShared& q,
-                                           int64_t row, int lane) {
+__device__ __forceinline__ double half_warp_dot(const FinishParams& p, const QueryShared& q,
+                                                int64_t row, int sub) {
     const uint4* codes = reinterpret_cast<const uint4*>(p.codes + row * (p.dp / 2));
+    const uint8_t* scales = p.scales + scale_word(row, 0, p.atoms);
+    const int blocks = p.dp / 32;
     double acc = 0.0;
-    for (int b = lane; b < p.dp / 32; b += 32) {  // 32 elements per lane
-        const uint4 w = __ldcg(codes + b);
-        const uint32_t raw[4] = {w.x, w.y, w.z, w.w};
-        const int4* qb = reinterpret_cast<const int4*>(q.codes + b * 32);
-        int dot[2] = {0, 0};
+    for (int b0 = sub; b0 < blocks; b0 += 64) {
+        uint4 w[4];
+        uint32_t s[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int4 qq = qb[h];
-            dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h]), qq.x, dot[h]);
-            dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h] >> 16), qq.y, dot[h]);
-            dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h + 1]), qq.z, dot[h]);
-            dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h + 1] >> 16), qq.w, dot[h]);
+        for (int u = 0; u < 4; ++u) {
+            const int b = b0 + 16 * u;
+            const bool in = b < blocks;
+            w[u] = in ? __ldcg(codes + b) : make_uint4(0u, 0u, 0u, 0u);
+            if (FMT == kMX)
+                s[u] = in ? __ldcg(scales + (b >> 2) * 512 + (b & 3)) : 0u;
+            else
+                s[u] = in ? __ldcg(reinterpret_cast<const uint16_t*>(
+                                scales + (b >> 1) * 512 + (b & 1) * 2))
+                          : 0u;
         }
-        if (FMT == kMX) {
-            const float s =
-                e8m0_value(__ldcg(p.scales + scale_word(row, b >> 2, p.atoms) + (b & 3)));
-            acc += (double)(dot[0] + dot[1]) * ((double)q.scales[b] * (double)s);
-        } else {
-            const uint8_t* at = p.scales + scale_word(row, b >> 1, p.atoms) + (b & 1) * 2;
-            const uint32_t two = __ldcg(reinterpret_cast<const uint16_t*>(at));
-            acc += (double)dot[0] * ((double)q.scales[2 * b] * (double)e4m3_value(two & 255u));
-            acc += (double)dot[1] * ((double)q.scales[2 * b + 1] * (double)e4m3_value(two >> 8));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int b = b0 + 16 * u;
+            if (b >= blocks) break;
+            const uint32_t raw[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+            const int4* qb = reinterpret_cast<const int4*>(q.codes + b * 32);
+            int dot[2] = {0, 0};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int4 qq = qb[h];
+                dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h]), qq.x, dot[h]);
+                dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h] >> 16), qq.y, dot[h]);
+                dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h + 1]), qq.z, dot[h]);
+                dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h + 1] >> 16), qq.w, dot[h]);
+            }
+            if (FMT == kMX) {
+                acc += (double)(dot[0] + dot[1]) *
+                       ((double)q.scales[b] * (double)e8m0_value(s[u]));
+            } else {
+                acc += (double)dot[0] *
+                       ((double)q.scales[2 * b] * (double)e4m3_value(s[u] & 255u));
+                acc += (double)dot[1] *
+                       ((double)q.scales[2 * b + 1] * (double)e4m3_value(s[u] >> 8));
+            }
         }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    for (int o = 8; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     return 0.25 * acc;
 }
 
@@ -1177,11 +1201,13 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const Fini
             __syncthreads();
             whole = s_n > LIST;
             if (!whole) {
-                for (int i = warp; i < s_n; i += W) {
+                for (int i0 = 2 * warp; i0 < s_n; i0 += 2 * W) {
+                    const int i = min(i0 + (lane >> 4), s_n - 1);
                     const int64_t row = (int64_t)key[i];
                     const float g = __ldcg(p.row_scale + row);
-                    const double dot = warp_dot<FMT>(p, q, row, lane);
-                    if (lane == 0) key[i] = row_key(dot, g, gq, row);
+                    const double dot = half_warp_dot<FMT>(p, q, row, lane & 15);
+                    // (an odd one out is done by both halves, and written by the first)
+                    if ((lane & 15) == 0 && i == i0 + (lane >> 4)) key[i] = row_key(dot, g, gq, row);
                 }
                 __syncthreads();
                 found = s_n;
@@ -1277,12 +1303,12 @@ __global__ void __launch_bounds__(SEL) rescue_kernel(const FinishParams p) {
         BestKeys<SEL> best = {key, &s_n, 0};
         int found = begin < end ? 0 : best.settle(p.k, true);
         for (int64_t r0 = begin; r0 < end; r0 += BestKeys<SEL>::BATCH) {
-            for (int i = warp; i < BestKeys<SEL>::BATCH && r0 + i < end; i += W) {
-                const int64_t row = r0 + i;
+            for (int i = 2 * warp; i < BestKeys<SEL>::BATCH && r0 + i < end; i += 2 * W) {
+                const int64_t row = min(r0 + i + (lane >> 4), end - 1);
                 const float g = __ldcg(p.row_scale + row);
-                if (!(g == g)) continue;
-                const double dot = warp_dot<FMT>(p, q, row, lane);
-                if (lane == 0) best.offer(row_key(dot, g, gq, row));
+                const double dot = half_warp_dot<FMT>(p, q, row, lane & 15);
+                if ((lane & 15) == 0 && row == r0 + i + (lane >> 4))
+                    best.offer(row_key(dot, g, gq, row));
             }
             found = best.settle(p.k, r0 + BestKeys<SEL>::BATCH >= end);
         }
