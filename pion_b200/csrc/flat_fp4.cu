@@ -176,10 +176,13 @@ __device__ __forceinline__ void mma_fp4(uint32_t d_tmem, uint64_t a_desc, uint64
             : "memory");
 }
 
-// This warp's lanes of four consecutive columns of TMEM.
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint4& r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr),
-                 "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+// This warp's lanes of consecutive columns of TMEM, four to a scale atom.
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint4 (&v)[2]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint4 (&v)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(v[0].x), "r"(v[0].y), "r"(v[0].z), "r"(v[0].w), "r"(v[1].x), "r"(v[1].y), "r"(v[1].z), "r"(v[1].w), "r"(v[2].x), "r"(v[2].y), "r"(v[2].z), "r"(v[2].w), "r"(v[3].x), "r"(v[3].y), "r"(v[3].z), "r"(v[3].w)
                  : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() {
@@ -403,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tc_fence_before();
     cluster_sync();
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;
+    constexpr uint32_t tmem_base = 0;  // all 512 columns are this pair's
     // Up to here nothing of an earlier kernel's is read.
     griddep_launch();
     griddep_wait();
@@ -421,12 +424,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const uint32_t lanes = tmem_base + ((uint32_t)(warp * 32) << 16);
         bool ok = __all_sync(0xffffffffu,
                              mbar_wait(bfull, 0, p.status, abort_flag, p.wait_ns));
+        // A stage's scales of the queries, atom by atom the 128-query tiles side by side.
+        auto put_queries = [&](uint32_t at, int kc) {
+            const uint8_t* from = sSF + kc * APS * 512 + lane * 16;
+            const int tile = kchunks * APS * 512;
+            if (sf_tiles == 1) {
+                uint4 v[APS];
+#pragma unroll
+                for (int a = 0; a < APS; ++a) v[a] = *reinterpret_cast<const uint4*>(from + a * 512);
+                tmem_st(at, v);
+            } else {
+#pragma unroll
+                for (int a = 0; a < APS; a += 2) {
+                    uint4 v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        v[i] = *reinterpret_cast<const uint4*>(from + (i & 1) * tile +
+                                                               (a + (i >> 1)) * 512);
+                    tmem_st(at + a * 8, v);
+                }
+            }
+        };
         if (ok && resident) {
-            for (int a = 0; a < kchunks * APS; ++a)
-                for (int h = 0; h < sf_tiles; ++h)
-                    tmem_st4(lanes + col_sfb + (a * sf_tiles + h) * 4,
-                             *reinterpret_cast<const uint4*>(
-                                 sSF + (h * kchunks * APS + a) * 512 + lane * 16));
+            for (int kc = 0; kc < kchunks; ++kc)
+                put_queries(lanes + col_sfb + kc * APS * sf_tiles * 4, kc);
             tmem_st_wait();
         }
         __syncwarp();
@@ -448,14 +469,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t at = lanes + col_sets + set * set_cols;
-#pragma unroll
-                for (int a = 0; a < APS; ++a) tmem_st4(at + a * 4, v[a]);
-                if (!resident)
-                    for (int a = 0; a < APS; ++a)
-                        for (int h = 0; h < sf_tiles; ++h)
-                            tmem_st4(at + APS * 4 + (a * sf_tiles + h) * 4,
-                                     *reinterpret_cast<const uint4*>(
-                                         sSF + ((h * kchunks + kc) * APS + a) * 512 + lane * 16));
+                tmem_st(at, v);
+                if (!resident) put_queries(at + APS * 4, kc);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
