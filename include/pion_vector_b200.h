@@ -245,8 +245,8 @@ int pion_v_b200_set_stream(pion_b200_ctx *ctx, void *cuda_stream);
  * once its kernels are queued, so its waits are reported here (they are never reported
  * as a later host-buffer call's failure). */
 int pion_v_b200_sync(pion_b200_ctx *ctx);
-/* Budget of each device-side wait in this context's FLAT INT8 tensor-core kernels, in
- * ns (<= 0 restores the default of 2 s).  A wait that runs out records
+/* Budget of each device-side wait in this context's FLAT INT8 and 4-bit tensor-core kernels,
+ * in ns (<= 0 restores the default of 2 s).  A wait that runs out records
  * PION_B200_ETIMEOUT; the kernel then drains its copies and MMAs, frees its tensor
  * memory and returns, so the context stays usable.  (For tests, the environment
  * variable PION_B200_TEST_STALL=1 makes one CTA of each main pass wait on a barrier that

@@ -194,6 +194,8 @@ def test_scores(ctx, fmt, n, dim, nq, types):
     q[nq // 2] = 0
     if n > 4:
         x[3, dim // 2] = np.nan
+    if nq > 2:
+        q[1, dim - 1] = np.inf
     tx, ex = typed(x, "f32")
     tq_, eq = typed(q, tq)
     rows = pion_b200.FP4Rows(n + 3, dim, fmt)
@@ -204,6 +206,10 @@ def test_scores(ctx, fmt, n, dim, nq, types):
     got = got.double().cpu().numpy()
     assert np.isneginf(got[:, n:]).all()
     got = got[:, :n]
+    if nq > 2:
+        assert np.isneginf(got[1]).all()
+        keep = np.arange(nq) != 1
+        got, want, size = got[keep], want[keep], size[keep]
     if n > 4:
         assert np.isneginf(got[:, 3]).all()
         keep = np.arange(n) != 3
@@ -440,6 +446,48 @@ def test_refusals(ctx):
                 lambda: ctx.lib.pion_v_b200_fp4_write(ctx.h, None, x.data_ptr(), 0, 64, 1, None, 0, 1,
                                                       1)):
         assert bad() == _lib.EINVAL
+
+
+def test_rows_past_32_bit_offsets(ctx):
+    """A store of 4.6 GB of codes, almost all of it empty: rows near its end are written, read
+    and found."""
+    import pion_b200
+    n = 6_000_000
+    rows = pion_b200.FP4Rows(n, 1536, "nv")
+    x, q = mixture_np(300, 1536, 4, seed=3, n_queries=5)
+    slots = np.concatenate([np.arange(200) * 7, n - 1 - 5 * np.arange(100)])
+    assert slots[-1] * 768 > 2 ** 32
+    rows.write(ctx, torch.from_numpy(x).cuda(), slots=slots)
+    codes, bits, g = plain.quantise(x, "nv")
+    want = (plain.values(codes, bits, "nv")[:, :1536] * g[:, None].astype(np.float64))
+    got = rows.read(ctx, slots=slots).cpu().numpy()
+    assert np.array_equal(got, want.astype(np.float32))
+    order = np.argsort(slots)
+    s, _ = plain.products(q.astype(np.float64), x[order].astype(np.float64), "nv")
+    wi, wv = plain.best(s, 20)
+    for nq in (1, 5):
+        ids, sc = pion_b200.FlatFP4Index(ctx, rows).search(torch.from_numpy(q[:nq]).cuda(), 20)
+        assert np.array_equal(ids.cpu().numpy(), slots[order][wi[:nq]])
+        assert np.array_equal(sc.cpu().numpy(), wv[:nq])
+    finish(ctx)
+
+
+def test_empty_stores_and_calls(ctx):
+    import pion_b200
+    rows = pion_b200.quantize_rows_fp4(ctx, torch.zeros((0, 40), device="cuda"))
+    q = torch.ones((2, 40), device="cuda")
+    ids, sc = pion_b200.FlatFP4Index(ctx, rows).search(q, 3)
+    assert (ids == -1).all() and torch.isneginf(sc).all()
+    assert pion_b200.fp4_scores(ctx, rows, q).shape == (2, 0)
+    assert rows.read(ctx).shape == (0, 40)
+    rows = pion_b200.FP4Rows(5, 40)
+    rows.write(ctx, q[:0])
+    assert pion_b200.fp4_scores(ctx, rows, q[:0]).shape == (0, 5)
+    ids, sc = pion_b200.FlatFP4Index(ctx, rows).search(q[:0], 3)
+    assert ids.shape == (0, 3)
+    ids, sc = pion_b200.FlatFP4Index(ctx, rows).search(np.ones((2, 40), np.float32), 3)
+    assert (ids == -1).all()
+    finish(ctx)
 
 
 def test_host_arrays(ctx):
