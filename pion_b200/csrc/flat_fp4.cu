@@ -809,6 +809,31 @@ __device__ uint32_t kth_largest(int m, int k, uint32_t* list, F value) {
     return n > LIST ? low : list_kth<NT>(list, n, k);
 }
 
+// A number that at least k, and few more, of n <= LIST values in shared memory reach: their k-th
+// largest where a warp can hold them, else that of the maxima of groups of them.
+template <int NT>
+__device__ uint32_t list_low(const uint32_t* list, int n, int k) {
+    __shared__ uint32_t s_low;
+    if (threadIdx.x < 32) {
+        uint32_t x;
+        if (n <= 256) {
+            x = warp_kth_of<8>(n, k, [&](int i) { return list[i]; });
+        } else {
+            // 16 groups a lane: more than k of them, of at most four values
+            x = warp_kth_of<16>(512, k, [&](int i) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int j = 0; j < LIST / 512; ++j)
+                    top = i + 512 * j < n ? max(top, list[i + 512 * j]) : top;
+                return top;
+            });
+        }
+        if (threadIdx.x == 0) s_low = x;
+    }
+    __syncthreads();
+    return s_low;
+}
+
 // Sorts n <= LIST keys in shared memory, largest first: up to a key per thread by their ranks,
 // more by a bitonic sort over the next power of two (the rest is filled with zeros).
 template <int NT>
@@ -1184,11 +1209,7 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const Fini
                     if (i < m) list[i] = ordered_score(__uint_as_float((uint32_t)(c[u] >> 32)));
                 }
                 __syncthreads();
-                // (a thread's values of the list are its own until all are in registers)
-                const float cut =
-                    m <= p.k    ? -INFINITY
-                    : m <= 1024 ? cut_of(list_kth<NT>(list, m, p.k))
-                                : cut_of(kth_largest<NT, V>(m, p.k, list, [&](int i) { return list[i]; }));
+                const float cut = m <= p.k ? -INFINITY : cut_of(list_low<NT>(list, m, p.k));
                 __syncthreads();
 #pragma unroll
                 for (int u = 0; u < V; ++u)

@@ -476,8 +476,8 @@ __global__ void __launch_bounds__(WARPS * 32) read_kernel(const ReadParams p) {
                         if (c + j < p.dim) out[c + j] = t[j];
                 }
             } else {
-                // side by side through shared memory: eight strided elements a lane took 3.5
-                // times as long
+                // side by side through shared memory: eight strided elements a lane took more
+                // than twice as long
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 8; ++j) stage[8 * lane + j] = t[j];
@@ -494,7 +494,8 @@ __global__ void __launch_bounds__(WARPS * 32) read_kernel(const ReadParams p) {
 
 template <int FMT, class T, bool VEC>
 static int write_v(const WriteParams& p, cudaStream_t st) {
-    // Few rows: a CTA each; many: a warp each.
+    // Few rows: a CTA each; many: a warp each (1536 float32 NV elements a row, us: 148 rows 2.4
+    // and 3.8, 1024 rows 4.9 and 5.8, 2048 rows 8.5 and 6.6).
     if (p.n <= FEW)
         return launch_pdl(write_kernel<FMT, T, VEC, WARPS, 4>, dim3((unsigned)p.n), WARPS * 32, 0,
                           st, p);
