@@ -924,22 +924,27 @@ __global__ void __launch_bounds__(NT)
     __syncthreads();
     const uint32_t low = s_low;
     const float low_f = unordered(low);
+    // For small k hardly two of the k best share a group: the bound does.
+    const bool near = k <= 32;
     auto keep = [&](float x) {
         if (x >= low_f) {
             const int at = atomicAdd(&s_count, 1);
             if (at < LIST) list[at] = ordered(x);
         }
     };
+    uint32_t x = low;
+    if (!near) {
 #pragma unroll
-    for (int i = 0; i < V4; ++i) {
-        keep(v[i].x);
-        keep(v[i].y);
-        keep(v[i].z);
-        keep(v[i].w);
+        for (int i = 0; i < V4; ++i) {
+            keep(v[i].x);
+            keep(v[i].y);
+            keep(v[i].z);
+            keep(v[i].w);
+        }
+        __syncthreads();
+        const int n = s_count;
+        if (n <= LIST) x = list_kth<NT>(list, n, k);
     }
-    __syncthreads();
-    const int n = s_count;
-    const uint32_t x = n > LIST ? low : list_kth<NT>(list, n, k);
     if (threadIdx.x == 0) {
         // an empty or zero query collects nothing
         theta[t] = gq > 0.0f ? threshold_of(x, two_eps, gq) : INFINITY;
