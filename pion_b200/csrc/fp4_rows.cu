@@ -227,8 +227,14 @@ __global__ void claim_kernel(const int64_t* slots, int64_t n, int64_t n_slots,
     if (s >= 0 && s < n_slots) atomicMax(&claim[s], (int32_t)(i + 1));
 }
 
-// WPR warps per row: one where rows are many, the CTA's eight where they are few and a row's
-// own latency counts.  An MX row is one pass.  NV needs the row's largest magnitude first; its
+// A barrier of the row's warps, `base` the first of them.
+template <int WPR>
+__device__ __forceinline__ void row_sync(int base) {
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + base / WPR), "n"(WPR * 32) : "memory");
+}
+
+// WPR warps per row: one or two where rows are many, the CTA's eight where they are few and a
+// row's own latency counts.  An MX row is one pass.  NV needs the row's largest magnitude first; its
 // elements stay in registers between the two passes where a warp's share is at most HOLD
 // steps (HOLD = 0: they are read again).  Bound by HBM: the row, its codes, scales and g once.
 template <int FMT, class T, bool VEC, int WPR, int HOLD>
@@ -240,9 +246,11 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     T* stage = stage_all + (VEC ? 0 : warp * STEP);
-    const int64_t i = WPR == 1 ? (int64_t)blockIdx.x * WARPS + warp : blockIdx.x;
+    const int64_t i = (int64_t)blockIdx.x * (WARPS / WPR) + warp / WPR;
+    const int mine = warp % WPR;               // of the row's warps
+    const int base = warp - mine;
     if (i >= p.n) return;
-    if (p.zero && lane == 0 && (WPR == 1 || warp == 0)) {
+    if (p.zero && lane == 0 && mine == 0) {
         p.zero[i + 1] = 0;
         if (i == 0) p.zero[0] = 0;
     }
@@ -251,7 +259,7 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
         slot = query_slot(i, p.tile, p.tile_pad);
     } else if (p.slots) {
         slot = __ldcg(p.slots + i);
-        if (WPR > 1) {
+        if (WPR == WARPS) {
             bool later = false;
             for (int64_t j = i + 1 + threadIdx.x; j < p.n; j += WARPS * 32)
                 later |= __ldcg(p.slots + j) == slot;
@@ -259,7 +267,7 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
             if (slot >= p.n_slots && threadIdx.x == 0) record_error(p.status, PION_B200_EINVAL);
         }
         if (slot < 0 || slot >= p.n_slots) return;
-        if (WPR == 1 && __ldcg(p.claim + slot) != (int32_t)(i + 1)) return;
+        if (WPR < WARPS && __ldcg(p.claim + slot) != (int32_t)(i + 1)) return;
     } else {
         slot = p.start + i;
     }
@@ -267,7 +275,7 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
     const int atoms = atoms_of(FMT, p.dp);
     constexpr int BL = block_of(FMT) / 8;  // lanes per block
     const int steps = (p.dp + STEP - 1) / STEP;
-    const int first = WPR == 1 ? 0 : warp;
+    const int first = mine;
     uint32_t* codes_out = reinterpret_cast<uint32_t*>(p.codes + slot * (p.dp / 2)) + lane;
     uint8_t* scales_out = p.scales + scale_word(slot, lane / (4 * BL), atoms);
 
@@ -280,9 +288,9 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
         for (int o = 16; o; o >>= 1) amax = max_abs(amax, __shfl_xor_sync(0xffffffffu, amax, o));
         if constexpr (WPR > 1) {
             if (lane == 0) s_max[warp] = amax;
-            __syncthreads();
+            row_sync<WPR>(base);
 #pragma unroll
-            for (int w = 0; w < WPR; ++w) amax = max_abs(amax, s_max[w]);
+            for (int w = 0; w < WPR; ++w) amax = max_abs(amax, s_max[base + w]);
         }
     };
     auto quantise = [&](int k, const float(&v)[8], float top) {
@@ -375,11 +383,11 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
     for (int o = 16; o; o >>= 1) s2 += __shfl_xor_sync(0xffffffffu, s2, o);
     if constexpr (WPR > 1) {
         if (lane == 0) s_s2[warp] = s2;
-        __syncthreads();
-        if (warp != 0) return;
+        row_sync<WPR>(base);
+        if (mine != 0) return;
         s2 = 0.0f;
 #pragma unroll
-        for (int w = 0; w < WPR; ++w) s2 += s_s2[w];
+        for (int w = 0; w < WPR; ++w) s2 += s_s2[base + w];
     }
     if (lane == 0) {
         p.row_scale[slot] = fine ? g : __int_as_float(0x7fc00000);
@@ -389,7 +397,7 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
         if (p.norm) p.norm[i] = bound;
         if (p.norm_max && bound > __ldcg(p.norm_max))
             atomicMax(reinterpret_cast<int*>(p.norm_max), __float_as_int(bound));
-        if (WPR == 1 && p.slots) p.claim[slot] = 0;
+        if (WPR < WARPS && p.slots) p.claim[slot] = 0;
     }
 }
 
@@ -501,9 +509,23 @@ static int write_v(const WriteParams& p, cudaStream_t st) {
                           st, p);
     const dim3 grid((unsigned)((p.n + WARPS - 1) / WARPS));
     if constexpr (FMT == kNV) {
-        if (p.dp <= 4 * STEP) return launch_pdl(write_kernel<FMT, T, VEC, 1, 4>, grid, WARPS * 32, 0, st, p);
-        if (p.dp <= 6 * STEP) return launch_pdl(write_kernel<FMT, T, VEC, 1, 6>, grid, WARPS * 32, 0, st, p);
-        if (p.dp <= 8 * STEP) return launch_pdl(write_kernel<FMT, T, VEC, 1, 8>, grid, WARPS * 32, 0, st, p);
+        // A row stays in one warp's registers while it leaves room for enough warps, then in two
+        // warps' (float32 / bfloat16, us: 262144 x 1536 330 / 285 in one, 365 / 385 in two;
+        // 131072 x 2048 284 / 205 and 216 / 226; 65536 x 4096 348 / 266 read twice, 270 / 226 in
+        // two).
+        const dim3 pairs((unsigned)((p.n + WARPS / 2 - 1) / (WARPS / 2)));
+        if (p.dp <= 4 * STEP)
+            return launch_pdl(write_kernel<FMT, T, VEC, 1, 4>, grid, WARPS * 32, 0, st, p);
+        if (p.dp <= 6 * STEP)
+            return launch_pdl(write_kernel<FMT, T, VEC, 1, 6>, grid, WARPS * 32, 0, st, p);
+        if (p.dp <= 8 * STEP) {
+            if constexpr (sizeof(T) == 4)
+                return launch_pdl(write_kernel<FMT, T, VEC, 2, 4>, pairs, WARPS * 32, 0, st, p);
+            else
+                return launch_pdl(write_kernel<FMT, T, VEC, 1, 8>, grid, WARPS * 32, 0, st, p);
+        }
+        if (p.dp <= 16 * STEP)
+            return launch_pdl(write_kernel<FMT, T, VEC, 2, 8>, pairs, WARPS * 32, 0, st, p);
     }
     return launch_pdl(write_kernel<FMT, T, VEC, 1, 0>, grid, WARPS * 32, 0, st, p);
 }

@@ -67,7 +67,9 @@ def check_store(rows, slots, x, fmt):
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("n,dim,pad", [(1, 1, 0), (3, 15, 1), (9, 16, 0), (130, 33, 3),
                                        (64, 128, 8), (257, 384, 0), (20, 777, 7), (33, 1536, 0),
-                                       (5, 2049, 0), (2, 8192, 0)])
+                                       (5, 2049, 0), (2, 8192, 0), (1100, 1536, 0),
+                                       (1030, 1900, 0), (1027, 4096, 0), (1025, 5000, 3),
+                                       (1051, 600, 1)])
 def test_write_and_read(ctx, fmt, dtype, n, dim, pad):
     import pion_b200
     x = rows_np(n, dim, n * dim + pad)
