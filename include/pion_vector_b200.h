@@ -522,7 +522,7 @@ int pion_v_b200_fp4_read(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows,
 int64_t pion_v_b200_fp4_workspace(const pion_b200_fp4_rows *rows, int64_t n_rows, int64_t nq,
                                   int64_t k);
 /* Scores of every query with the rows of slots [0, n_rows): out[t * out_stride + r] =
- * ((sum_j q_j v_j) g_r) g_t, accumulated in float32.  q: nq rows of q_type, quantised here
+ * ((sum_j q_j v_j) g_r) g_t, accumulated and multiplied in float32.  q: nq rows of q_type, quantised here
  * in the store's format.  With `mem` DEVICE the scratch is the caller's `workspace`
  * (16-byte aligned; pion_v_b200_fp4_workspace bytes), or the context's where both it and
  * cuda_stream are NULL. */
@@ -534,7 +534,8 @@ int pion_v_b200_fp4_scores(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, i
  * out_scores [nq x k]; -1 / -inf past the rows that are not empty.  Here a score is
  * f32(((sum) g_r) g_t) of the sum in float64, so the ids do not depend on an order of
  * summation.  k <= 256.  A query whose candidates overflow (thousands of rows that tie with
- * its k-th) is answered by an exact scan of its rows, one CTA per query. */
+ * its k-th, or are as near to it as float32 sums with the longest row's norm can tell) is
+ * answered by an exact scan of the rows: right, but about 1 ms a query and million rows. */
 int pion_v_b200_flat_fp4_knn(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, int64_t n_rows,
                              int64_t id_base, const void *q, int q_type, int64_t q_stride,
                              int64_t nq, int64_t k, int32_t *out_ids, float *out_scores,

@@ -56,6 +56,9 @@ int check_matrix(pion_b200_ctx* ctx, const char* who, const char* what, const vo
     if (n > 0 && stride < dim)
         return set_error(ctx, PION_B200_EINVAL, "%s: %s rows overlap (stride %lld, %lld elements)", who,
                          what, (long long)stride, (long long)dim);
+    if (n > 1 && stride > INT64_MAX / 8 / n)
+        return set_error(ctx, PION_B200_EINVAL, "%s: %s rows past 64 bits (stride %lld)", who, what,
+                         (long long)stride);
     if (!aligned(p, elem_bytes(type)))
         return set_error(ctx, PION_B200_EINVAL, "%s: misaligned %s", who, what);
     return 0;
@@ -262,8 +265,9 @@ int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, i
         // Stages over growing parts of the rows, each with the threshold of the rows before it:
         // every R^(L-1)-th tile, then those of every R^(L-2)-th that are new, and so on.  About
         // k R rows of the first stage and k (R - 1) of each later one reach their threshold,
-        // with a deviation of 1 / sqrt(k) of that: the lists have room for 13 deviations.  A batch takes more stages, since its
-        // candidates cost the product's epilogue more than a stage costs.
+        // with a deviation of 1 / sqrt(k) of that: the lists have room for 13 deviations.  A
+        // batch takes more stages, since its candidates cost the product's epilogue more than
+        // a stage costs.
         const double ratio = (double)n_tiles / (double)samples;
         const double room = fp4_cap() / ((double)k + 13.0 * sqrt((double)k));
         int stages = 1;

@@ -873,11 +873,12 @@ __device__ void sort_desc(uint64_t* key, int n) {
         }
 }
 
-// Infinite where a float32 sum could overflow: nothing is known of an approximate score then.
-// The last term covers products below the least normal float.
-__device__ __forceinline__ float eps_of(int dp, float q_norm, float norm_max) {
-    const float size = q_norm * norm_max;
-    return size < 0x1p120f ? rel_eps(dp) * size + 0x1p-100f : INFINITY;
+// Infinite where a float32 sum, or its product with the row's g alone (a score in units of the
+// query's g), could overflow: nothing is known of an approximate score then.  The last term
+// covers products below the least normal float.
+__device__ __forceinline__ float eps_of(int dp, float q_norm, float gq, float norm_max) {
+    const float size = q_norm * norm_max, in_units = q_norm / gq * norm_max;
+    return size < 0x1p120f && in_units < 0x1p120f ? rel_eps(dp) * size + 0x1p-100f : INFINITY;
 }
 
 // A query's threshold: the k-th best (ordered) of its approximate scores so far less 2 eps, in
@@ -907,7 +908,7 @@ __global__ void __launch_bounds__(NT)
 #pragma unroll
     for (int i = 0; i < V4; ++i) v[i] = __ldcg(s + threadIdx.x + i * NT);
     const float gq = __ldcg(q_scale + query_slot(t, nt, nt_pad));
-    const float two_eps = 2.0f * eps_of(dp, __ldcg(q_norm + t), __ldcg(norm_max));
+    const float two_eps = 2.0f * eps_of(dp, __ldcg(q_norm + t), gq, __ldcg(norm_max));
     float most = -INFINITY;  // (passes over NaN)
 #pragma unroll
     for (int i = 0; i < V4; ++i)
@@ -962,7 +963,7 @@ __global__ void __launch_bounds__(SEL)
     const int t = blockIdx.x;
     const int m = min(__ldcg(cand_n + t), CAP);
     const float gq = __ldcg(q_scale + query_slot(t, nt, nt_pad));
-    const float two_eps = 2.0f * eps_of(dp, __ldcg(q_norm + t), __ldcg(norm_max));
+    const float two_eps = 2.0f * eps_of(dp, __ldcg(q_norm + t), gq, __ldcg(norm_max));
     if (!(gq > 0.0f) || m < k) return;
     const uint64_t* c = cand + (int64_t)t * CAP;
     const uint32_t x = kth_largest<SEL, 4>(m, k, list, [&](int i) {
@@ -1002,7 +1003,7 @@ __global__ void __launch_bounds__(SEL)
         if (at + 3 >= left) v[i].w = -INFINITY;
     }
     const float gq = __ldcg(q_scale + query_slot(t, nt, nt_pad));
-    const float two_eps = 2.0f * eps_of(dp, __ldcg(q_norm + t), __ldcg(norm_max));
+    const float two_eps = 2.0f * eps_of(dp, __ldcg(q_norm + t), gq, __ldcg(norm_max));
     float most = -INFINITY;
 #pragma unroll
     for (int i = 0; i < V4; ++i)
@@ -1182,7 +1183,7 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const Fini
     for (int u = 0; u < V; ++u) c[u] = p.dense ? 0 : __ldcg(cand + threadIdx.x + u * NT);
     const float gq = __ldcg(p.q_scale + qs);
     const int m = p.dense ? (int)p.n_rows : __ldcg(p.cand_n + t);
-    const float two_eps = 2.0f * eps_of(p.dp, __ldcg(p.q_norm + t), __ldcg(p.norm_max));
+    const float two_eps = 2.0f * eps_of(p.dp, __ldcg(p.q_norm + t), gq, __ldcg(p.norm_max));
     QueryShared q;
     q.codes = reinterpret_cast<int8_t*>(dyn);
     q.scales = reinterpret_cast<float*>(dyn + p.dp);
@@ -1333,7 +1334,7 @@ __global__ void __launch_bounds__(SEL) rescue_kernel(const FinishParams p) {
     q.scales = reinterpret_cast<float*>(dyn + p.dp);
     const int splits = max(1, RESCUE_CTAS / flagged);
     for (int item = blockIdx.x; item < flagged * splits; item += gridDim.x) {
-        const int t = p.flagged[item / splits];
+        const int t = __ldcg(p.flagged + item / splits);
         const int part = item % splits;
         const int64_t qs = query_slot(t, p.nt, p.nt_pad);
         const float gq = __ldcg(p.q_scale + qs);

@@ -345,6 +345,36 @@ def test_knn_overflowing_candidates(ctx, fmt):
     check_knn(ctx, rows, tq, eq, ex, fmt, 10)
 
 
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("n,nq", [(9000, 3), (40000, 3), (40000, 150)])
+@pytest.mark.parametrize("row_exp,q_exp", [(114, -12), (-70, 110), (-95, 0), (100, -99)])
+def test_knn_far_magnitudes(ctx, fmt, n, nq, row_exp, q_exp):
+    """Scores inside float32 whose factors are far apart: the product with the row's g alone
+    may leave it."""
+    import pion_b200
+    rng = np.random.default_rng(n + nq)
+    tx, ex = typed(rng.standard_normal((n, 64)) * 2.0 ** row_exp, "f32")
+    tq, eq = typed(rng.standard_normal((nq, 64)) * 2.0 ** q_exp, "f32")
+    rows = pion_b200.quantize_rows_fp4(ctx, tx, fmt)
+    check_knn(ctx, rows, tq, eq, ex, fmt, 10)
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+def test_knn_beside_a_long_row(ctx, fmt):
+    """One row many times longer than the rest widens every query's margin."""
+    import pion_b200
+    rng = np.random.default_rng(23)
+    x = rng.standard_normal((40000, 64))
+    for factor in (30.0, 1e4, 1e8):
+        y = x.copy()
+        y[777] *= factor
+        tx, ex = typed(y, "f32")
+        rows = pion_b200.quantize_rows_fp4(ctx, tx, fmt)
+        for nq in (3, 150):
+            tq, eq = typed(rng.standard_normal((nq, 64)), "f32")
+            check_knn(ctx, rows, tq, eq, ex, fmt, 10)
+
+
 def test_many_overflowing_queries(ctx):
     """More flagged queries than the rescue's CTAs, and fewer; beside ordinary ones."""
     import pion_b200
@@ -420,6 +450,11 @@ def test_refusals(ctx):
             bad()
     # a stream of its own needs a workspace; one that is too small is refused
     out = torch.empty((10, 100), device="cuda")
+    wide = 2 ** 62                                        # ... and rows that span past 64 bits
+    for dst, q_stride, ld in ((out, wide, 100), (out, 64, wide)):
+        assert ctx.lib.pion_v_b200_fp4_scores(
+            ctx.h, rows._ref(ctx), 100, x.data_ptr(), 0, q_stride, 10, dst.data_ptr(), 0, ld, None,
+            0, 0, None) == _lib.EINVAL
     call = lambda ws, n: ctx.lib.pion_v_b200_fp4_scores(  # noqa: E731
         ctx.h, rows._ref(ctx), 100, x.data_ptr(), 0, 64, 10, out.data_ptr(), 0, 100, ws, n, 1, 1)
     ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
