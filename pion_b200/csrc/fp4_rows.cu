@@ -391,9 +391,12 @@ __global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) 
     }
     if (lane == 0) {
         p.row_scale[slot] = fine ? g : __int_as_float(0x7fc00000);
-        // every element is at most 6 s g: |row| <= 6 g sqrt(block * sum s^2)
-        const float bound =
-            fine ? 6.02f * g * sqrtf((float)(block_of(FMT) / BL) * s2) : 0.0f;
+        // every element is at most 6 s g: |row| <= 6 g sqrt(block * sum s^2); where the squares
+        // of MX scales could leave the normal numbers, no element is more than twice amax
+        float bound = 6.02f * g * sqrtf((float)(block_of(FMT) / BL) * s2);
+        if (FMT == kMX && !(s2 >= 0x1p-100f && s2 < 0x1p100f))
+            bound = 2.01f * amax * sqrtf((float)p.dim);
+        if (!fine) bound = 0.0f;
         if (p.norm) p.norm[i] = bound;
         if (p.norm_max && bound > __ldcg(p.norm_max))
             atomicMax(reinterpret_cast<int*>(p.norm_max), __float_as_int(bound));

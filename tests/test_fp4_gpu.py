@@ -360,6 +360,30 @@ def test_knn_far_magnitudes(ctx, fmt, n, nq, row_exp, q_exp):
 
 
 @pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("row_exp,q_exp", [(0, 0), (-115, 50), (-120, 55), (-120, 100),
+                                           (50, -115), (80, -90)])
+def test_knn_ties_that_float32_sums_tell_apart(ctx, fmt, row_exp, q_exp):
+    """Rows made of the same 16 chunks in another order: equal scores, whose float32 sums
+    differ.  The lowest ids are the best, at every magnitude of rows and queries."""
+    import pion_b200
+    rng = np.random.default_rng(41)
+    n, tied = 17000, 100
+    chunks = rng.standard_normal((16, 64)) * 2.0 ** rng.integers(0, 28, (16, 1))
+    piece = rng.standard_normal(64)
+    chunks *= np.sign(chunks @ piece)[:, None]
+    x = np.zeros((n, 1024), np.float32)
+    x[:, :64] = rng.standard_normal((n, 64))
+    for i in rng.choice(n, tied, replace=False):
+        x[i] = chunks[rng.permutation(16)].reshape(-1)
+    tx, ex = typed(x * 2.0 ** row_exp, "f32")
+    for nq in (2, 130):
+        q = np.tile(piece, (nq, 16)) * 2.0 ** (q_exp + np.arange(nq) % 2)[:, None]
+        tq, eq = typed(q, "f32")
+        rows = pion_b200.quantize_rows_fp4(ctx, tx, fmt)
+        check_knn(ctx, rows, tq, eq, ex, fmt, 10)
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
 def test_knn_beside_a_long_row(ctx, fmt):
     """One row many times longer than the rest widens every query's margin."""
     import pion_b200
