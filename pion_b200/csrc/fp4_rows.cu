@@ -22,7 +22,11 @@
 namespace pion {
 namespace fp4 {
 
-constexpr int WARPS = 8;   // per CTA
+constexpr int WARPS = 8;   // per CTA that writes one row
+constexpr int NW = 2;      // per CTA that writes several: its place is soon free for the next
+                           // (262144 x 1536, us with 8: NV float32 330 -> 313, MX bfloat16
+                           // 246 -> 201)
+constexpr int READ_WARPS = 4;  // (bfloat16 with 8: 173 us -> 165)
 constexpr int FEW = 1024;  // rows written by a CTA each
 constexpr int STEP = 256;  // elements per warp step, eight consecutive ones per lane
 
@@ -174,22 +178,27 @@ __device__ __forceinline__ uint32_t settle_borders(uint32_t lo, uint32_t hi, con
     return lo;
 }
 
+// v r, two products an instruction.
+__device__ __forceinline__ void mul8(float (&out)[8], const float (&v)[8], float r) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+        asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\t"
+            "mul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+            : "=f"(out[j]), "=f"(out[j + 1])
+            : "f"(v[j]), "f"(v[j + 1]), "f"(r));
+}
+
 // Eight codes of v / d; rd is 1 / d, in MX exactly, in NV within 2^-22 (0 for d = 0).
 template <int FMT>
 __device__ __forceinline__ uint32_t codes8(const float (&v)[8], float d, float rd) {
     float a[8];
     if (FMT == kMX) {  // a power of two: the product is the quotient
-#pragma unroll
-        for (int j = 0; j < 8; ++j) a[j] = v[j] * rd;
+        mul8(a, v, rd);
         return e2m1x8(a);
     }
     float b[8];
-    const float r0 = rd * (1.0f - 0x1p-21f), r1 = rd * (1.0f + 0x1p-21f);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        a[j] = v[j] * r0;
-        b[j] = v[j] * r1;
-    }
+    mul8(a, v, rd * (1.0f - 0x1p-21f));
+    mul8(b, v, rd * (1.0f + 0x1p-21f));
     const uint32_t lo = e2m1x8(a), hi = e2m1x8(b);
     return lo == hi ? lo : settle_borders(lo, hi, v, d);
 }
@@ -237,16 +246,16 @@ __device__ __forceinline__ void row_sync(int base) {
 // row's own latency counts.  An MX row is one pass.  NV needs the row's largest magnitude first; its
 // elements stay in registers between the two passes where a warp's share is at most HOLD
 // steps (HOLD = 0: they are read again).  Bound by HBM: the row, its codes, scales and g once.
-template <int FMT, class T, bool VEC, int WPR, int HOLD>
-__global__ void __launch_bounds__(WARPS * 32) write_kernel(const WriteParams p) {
-    __shared__ __align__(16) T stage_all[VEC ? 1 : WARPS * STEP];
-    __shared__ float s_max[WARPS];
-    __shared__ float s_s2[WARPS];
+template <int FMT, class T, bool VEC, int W, int WPR, int HOLD>
+__global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
+    __shared__ __align__(16) T stage_all[VEC ? 1 : W * STEP];
+    __shared__ float s_max[W];
+    __shared__ float s_s2[W];
     griddep_launch();
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     T* stage = stage_all + (VEC ? 0 : warp * STEP);
-    const int64_t i = (int64_t)blockIdx.x * (WARPS / WPR) + warp / WPR;
+    const int64_t i = (int64_t)blockIdx.x * (W / WPR) + warp / WPR;
     const int mine = warp % WPR;               // of the row's warps
     const int base = warp - mine;
     if (i >= p.n) return;
@@ -430,13 +439,13 @@ __device__ __forceinline__ void store8(T* to, const T (&t)[8]) {
 
 // One warp per row.  Bound by HBM: the output once.
 template <int FMT, class T, bool VEC>
-__global__ void __launch_bounds__(WARPS * 32) read_kernel(const ReadParams p) {
-    __shared__ __align__(16) T stage_all[VEC ? 1 : WARPS * STEP];
+__global__ void __launch_bounds__(READ_WARPS * 32) read_kernel(const ReadParams p) {
+    __shared__ __align__(16) T stage_all[VEC ? 1 : READ_WARPS * STEP];
     griddep_launch();
     griddep_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     T* stage = stage_all + (VEC ? 0 : warp * STEP);
-    const int64_t i = (int64_t)blockIdx.x * WARPS + warp;
+    const int64_t i = (int64_t)blockIdx.x * READ_WARPS + warp;
     if (i >= p.n) return;
     const int64_t slot = p.slots ? __ldcg(p.slots + i) : p.start + i;
     if (slot < 0) return;
@@ -476,8 +485,10 @@ __global__ void __launch_bounds__(WARPS * 32) read_kernel(const ReadParams p) {
             // code * s has at most six significant bits: one rounding in the product with g
             // (and one to a 16-bit output, from a value already within 2^-24)
             alignas(16) T t[8];
+            mul8(v, v, s);
+            mul8(v, v, g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = from_float<T>(__fmul_rn(__fmul_rn(v[j], s), g));
+            for (int j = 0; j < 8; ++j) t[j] = from_float<T>(v[j]);
             if constexpr (VEC) {
                 if (c + 8 <= p.dim) {
                     store8(out + c, t);
@@ -508,29 +519,29 @@ static int write_v(const WriteParams& p, cudaStream_t st) {
     // Few rows: a CTA each; many: a warp each (1536 float32 NV elements a row, us: 148 rows 2.4
     // and 3.8, 1024 rows 4.9 and 5.8, 2048 rows 8.5 and 6.6).
     if (p.n <= FEW)
-        return launch_pdl(write_kernel<FMT, T, VEC, WARPS, 4>, dim3((unsigned)p.n), WARPS * 32, 0,
+        return launch_pdl(write_kernel<FMT, T, VEC, WARPS, WARPS, 4>, dim3((unsigned)p.n), WARPS * 32, 0,
                           st, p);
-    const dim3 grid((unsigned)((p.n + WARPS - 1) / WARPS));
+    const dim3 grid((unsigned)((p.n + NW - 1) / NW));
     if constexpr (FMT == kNV) {
         // A row stays in one warp's registers while it leaves room for enough warps, then in two
-        // warps' (float32 / bfloat16, us: 262144 x 1536 330 / 285 in one, 365 / 385 in two;
-        // 131072 x 2048 284 / 205 and 216 / 226; 65536 x 4096 348 / 266 read twice, 270 / 226 in
-        // two).
-        const dim3 pairs((unsigned)((p.n + WARPS / 2 - 1) / (WARPS / 2)));
+        // warps' (float32 / bfloat16, us, with eight warps a CTA: 262144 x 1536 330 / 285 in
+        // one, 365 / 385 in two; 131072 x 2048 284 / 205 and 216 / 226; 65536 x 4096 348 / 266
+        // read twice, 270 / 226 in two; with NW: 310 / 270, 207 / 181, 250 / 195).
+        const dim3 pairs((unsigned)((p.n + NW / 2 - 1) / (NW / 2)));
         if (p.dp <= 4 * STEP)
-            return launch_pdl(write_kernel<FMT, T, VEC, 1, 4>, grid, WARPS * 32, 0, st, p);
+            return launch_pdl(write_kernel<FMT, T, VEC, NW, 1, 4>, grid, NW * 32, 0, st, p);
         if (p.dp <= 6 * STEP)
-            return launch_pdl(write_kernel<FMT, T, VEC, 1, 6>, grid, WARPS * 32, 0, st, p);
+            return launch_pdl(write_kernel<FMT, T, VEC, NW, 1, 6>, grid, NW * 32, 0, st, p);
         if (p.dp <= 8 * STEP) {
             if constexpr (sizeof(T) == 4)
-                return launch_pdl(write_kernel<FMT, T, VEC, 2, 4>, pairs, WARPS * 32, 0, st, p);
+                return launch_pdl(write_kernel<FMT, T, VEC, NW, 2, 4>, pairs, NW * 32, 0, st, p);
             else
-                return launch_pdl(write_kernel<FMT, T, VEC, 1, 8>, grid, WARPS * 32, 0, st, p);
+                return launch_pdl(write_kernel<FMT, T, VEC, NW, 1, 8>, grid, NW * 32, 0, st, p);
         }
         if (p.dp <= 16 * STEP)
-            return launch_pdl(write_kernel<FMT, T, VEC, 2, 8>, pairs, WARPS * 32, 0, st, p);
+            return launch_pdl(write_kernel<FMT, T, VEC, NW, 2, 8>, pairs, NW * 32, 0, st, p);
     }
-    return launch_pdl(write_kernel<FMT, T, VEC, 1, 0>, grid, WARPS * 32, 0, st, p);
+    return launch_pdl(write_kernel<FMT, T, VEC, NW, 1, 0>, grid, NW * 32, 0, st, p);
 }
 
 template <int FMT, class T>
@@ -544,9 +555,9 @@ template <int FMT, class T>
 static int read_t(const ReadParams& p, cudaStream_t st) {
     constexpr size_t A = 8 * sizeof(T);
     const bool vec = reinterpret_cast<uintptr_t>(p.dst) % A == 0 && p.stride * sizeof(T) % A == 0;
-    const dim3 grid((unsigned)((p.n + WARPS - 1) / WARPS));
-    return vec ? launch_pdl(read_kernel<FMT, T, true>, grid, WARPS * 32, 0, st, p)
-               : launch_pdl(read_kernel<FMT, T, false>, grid, WARPS * 32, 0, st, p);
+    const dim3 grid((unsigned)((p.n + READ_WARPS - 1) / READ_WARPS));
+    return vec ? launch_pdl(read_kernel<FMT, T, true>, grid, READ_WARPS * 32, 0, st, p)
+               : launch_pdl(read_kernel<FMT, T, false>, grid, READ_WARPS * 32, 0, st, p);
 }
 
 }  // namespace fp4
