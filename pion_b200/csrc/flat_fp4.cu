@@ -237,24 +237,36 @@ __device__ __forceinline__ void store_chunk(const uint32_t (&r)[32], const TcPar
         store_columns<T, false>(r, out, p.ld, n, gq, g);
 }
 
-// Candidates that an epilogue warp has found and not yet appended: an append waits for its
-// place in the query's list about as long as the MMAs of a third of a tile take, so they are
-// made for up to 64 candidates at once.
+// Candidates that an epilogue warp has found and not yet appended.  Their places in the queries'
+// lists are asked for 32 at a time and used a tile later: the answer takes about as long as
+// the MMAs of a third of a tile, and a pair waits for the last of its 32 warps.
 struct Hits {
     uint64_t* entry;  // [HITS] score bits << 32 | row
     uint8_t* col;     // [HITS] query's column
     int n;            // warp-uniform
+    int at;           // this lane's place, where asked for
+    bool asked;       // for the first 32
 };
 
-__device__ __forceinline__ void append_hits(Hits& h, const TcParams& p, int qt_first, int lane) {
+__device__ __forceinline__ void ask_places(Hits& h, const TcParams& p, int qt_first, int lane) {
     __syncwarp();
-    for (int i = lane; i < h.n; i += 32) {
-        const int t = qt_first + h.col[i];
-        const int at = atomicAdd(&p.cand_n[t], 1);
-        if (at < CAP) p.cand[(int64_t)t * CAP + at] = h.entry[i];
+    if (lane < h.n) h.at = atomicAdd(&p.cand_n[qt_first + h.col[lane]], 1);
+    h.asked = true;
+}
+
+// The first 32 go to their places, the others move up.
+__device__ __forceinline__ void place_hits(Hits& h, const TcParams& p, int qt_first, int lane) {
+    __syncwarp();
+    if (lane < h.n && h.at < CAP)
+        p.cand[(int64_t)(qt_first + h.col[lane]) * CAP + h.at] = h.entry[lane];
+    __syncwarp();
+    if (lane + 32 < h.n) {
+        h.entry[lane] = h.entry[lane + 32];
+        h.col[lane] = h.col[lane + 32];
     }
     __syncwarp();
-    h.n = 0;
+    h.n = max(h.n - 32, 0);
+    h.asked = false;
 }
 
 // r[i], without an indexed access that would move r to local memory: a tree of selects.
@@ -309,7 +321,10 @@ __device__ __forceinline__ void collect_chunk(const uint32_t (&r)[32], const TcP
     }
     unsigned lanes = __ballot_sync(0xffffffffu, mine != 0);
     while (lanes) {
-        if (h.n > HITS - 32) append_hits(h, p, qt_first, lane);
+        if (h.n > HITS - 32) {  // no room for a round
+            if (!h.asked) ask_places(h, p, qt_first, lane);
+            place_hits(h, p, qt_first, lane);
+        }
         const int i = __clz((int)mine);
         const float v = pick(r, i) * g;
         if (mine) {
@@ -611,7 +626,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int half = (warp - 8) >> 2;      // of PER_QUARTER
         const int chunks = (nt + 31) / 32;     // of 32 columns; this warp takes every PER_QUARTER-th
         const int in_tile = (int)rank * HALF + quarter * 32 + lane;
-        Hits hits = {s_hits + (warp - 8) * HITS, s_hit_col + (warp - 8) * HITS, 0};
+        Hits hits = {s_hits + (warp - 8) * HITS, s_hit_col + (warp - 8) * HITS, 0, 0, false};
         int buf = 0;
         uint32_t buf_phase = 0;
         for (int j = first; j < p.n_tiles; j += stride) {
@@ -652,12 +667,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 else
                     store_chunk<__half>(r[c], p, t0, n, col, s_gq + at, g);
             }
+            if (hits.asked) place_hits(hits, p, qt * nt, lane);
+            if (hits.n >= 32) ask_places(hits, p, qt * nt, lane);
             if (++buf == bufs) {
                 buf = 0;
                 buf_phase ^= 1u;
             }
         }
-        if (mode == kCollect) append_hits(hits, p, qt * nt, lane);
+        while (hits.n > 0) {
+            if (!hits.asked) ask_places(hits, p, qt * nt, lane);
+            place_hits(hits, p, qt * nt, lane);
+        }
     }
     tc_fence_before();
     cluster_sync();
