@@ -328,7 +328,7 @@ int knn_chunk(pion_b200_ctx* ctx, const pion_b200_fp4_rows* r, int64_t n_rows, i
     f.parts = reinterpret_cast<uint64_t*>(base + s.parts);
     f.out_ids = ids;
     f.out_scores = scores;
-    ctx->launches += 2;
+    ctx->launches += dense ? 1 : 2;
     return launch_fp4_finish(f, st);
 }
 

@@ -1180,11 +1180,62 @@ __device__ __forceinline__ void write_best(const FinishParams& p, int t, const u
     }
 }
 
+// The k best of a stream of keys, by a CTA: offered keys above the k-th best so far are kept
+// until the list is nearly full, then the k best of them.
+template <int NT>
+struct BestKeys {
+    static constexpr int BATCH = 512;  // offered at most between two calls of settle()
+    uint64_t* key;                     // [LIST], shared
+    int* n;                            // shared, 0 at first
+    uint64_t floor;
+    __device__ __forceinline__ void offer(uint64_t x) {  // by any thread
+        if (x > floor) key[atomicAdd(n, 1)] = x;
+    }
+    __device__ __forceinline__ int settle(int k, bool last) {  // by all threads
+        __syncthreads();
+        int have = *n;
+        if (have > LIST - BATCH || last) {
+            sort_desc<NT>(key, have);
+            have = min(have, k);
+            floor = have == k ? key[k - 1] : 0;
+            __syncthreads();
+            if (threadIdx.x == 0) *n = have;
+        }
+        __syncthreads();
+        return have;
+    }
+};
+
+// The k best of rows [begin, end), all scored exactly, by a CTA -> key[0, found).  `n`: shared.
+template <int FMT, int NT>
+__device__ int scan_rows(const FinishParams& p, const QueryShared& q, float gq, int64_t begin,
+                         int64_t end, uint64_t* key, int* n) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int W = NT / 32, BATCH = BestKeys<NT>::BATCH;
+    __syncthreads();
+    if (threadIdx.x == 0) *n = 0;
+    __syncthreads();
+    BestKeys<NT> best = {key, n, 0};
+    int found = begin < end ? 0 : best.settle(p.k, true);
+    for (int64_t r0 = begin; r0 < end; r0 += BATCH) {
+        for (int i = 2 * warp; i < BATCH && r0 + i < end; i += 2 * W) {
+            const int64_t row = min(r0 + i + (lane >> 4), end - 1);
+            const float g = __ldcg(p.row_scale + row);
+            const double dot = half_warp_dot<FMT>(p, q, row, lane & 15);
+            if ((lane & 15) == 0 && row == r0 + i + (lane >> 4))
+                best.offer(row_key(dot, g, gq, row));
+        }
+        found = best.settle(p.k, r0 + BATCH >= end);
+    }
+    return found;
+}
+
 // The k best rows of one query per CTA: its candidates whose approximate score can be among
 // the k best are scored exactly and sorted.  A query with more than LIST of those, or whose
-// candidates overflowed, is left to rescue_kernel.
+// candidates overflowed, is left to rescue_kernel, or where all rows are few (dense) scored
+// here row by row.
 template <int FMT, int NT>
-__global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const FinishParams p) {
+__global__ void __launch_bounds__(NT, NT > 256 ? 1 : 4) finish_kernel(const FinishParams p) {
     __shared__ __align__(16) uint64_t key[LIST];
     __shared__ int s_warp[NT / 32];
     __shared__ int s_n;
@@ -1276,7 +1327,9 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const Fini
                 sort_desc<NT>(key, found);
             }
         }
-        if (whole) {
+        if (whole && p.dense) {
+            found = scan_rows<FMT, NT>(p, q, gq, 0, p.n_rows, key, &s_n);
+        } else if (whole) {
             if (threadIdx.x == 0) {
                 p.done[t] = 0;
                 p.flagged[atomicAdd(p.n_flagged, 1)] = t;
@@ -1307,34 +1360,8 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 6) finish_kernel(const Fini
     write_best<NT>(p, t, key, found);
 }
 
-// The k best of a stream of keys, by a CTA: offered keys above the k-th best so far are kept
-// until the list is nearly full, then the k best of them.
-template <int NT>
-struct BestKeys {
-    static constexpr int BATCH = 512;  // offered at most between two calls of settle()
-    uint64_t* key;                     // [LIST], shared
-    int* n;                            // shared, 0 at first
-    uint64_t floor;
-    __device__ __forceinline__ void offer(uint64_t x) {  // by any thread
-        if (x > floor) key[atomicAdd(n, 1)] = x;
-    }
-    __device__ __forceinline__ int settle(int k, bool last) {  // by all threads
-        __syncthreads();
-        int have = *n;
-        if (have > LIST - BATCH || last) {
-            sort_desc<NT>(key, have);
-            have = min(have, k);
-            floor = have == k ? key[k - 1] : 0;
-            __syncthreads();
-            if (threadIdx.x == 0) *n = have;
-        }
-        __syncthreads();
-        return have;
-    }
-};
-
 // Flagged queries (many rows that tie with the k-th best, a sample that missed the best rows, or
-// norms whose products leave float32): every row, exactly.  Each query's rows are split
+// norms whose products leave float32) of many rows: every row, exactly.  Each query's rows are split
 // between as many CTAs as the grid has to spare; the last one to finish merges the parts.
 constexpr int RESCUE_CTAS = 296;
 template <int FMT>
@@ -1347,8 +1374,6 @@ __global__ void __launch_bounds__(SEL) rescue_kernel(const FinishParams p) {
     griddep_wait();
     const int flagged = __ldcg(p.n_flagged);
     if (flagged == 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    constexpr int W = SEL / 32;
     QueryShared q;
     q.codes = reinterpret_cast<int8_t*>(dyn);
     q.scales = reinterpret_cast<float*>(dyn + p.dp);
@@ -1360,20 +1385,7 @@ __global__ void __launch_bounds__(SEL) rescue_kernel(const FinishParams p) {
         const float gq = __ldcg(p.q_scale + qs);
         const int64_t begin = p.n_rows * part / splits, end = p.n_rows * (part + 1) / splits;
         load_query<FMT, SEL>(p, q, qs, threadIdx.x);
-        if (threadIdx.x == 0) s_n = 0;
-        __syncthreads();
-        BestKeys<SEL> best = {key, &s_n, 0};
-        int found = begin < end ? 0 : best.settle(p.k, true);
-        for (int64_t r0 = begin; r0 < end; r0 += BestKeys<SEL>::BATCH) {
-            for (int i = 2 * warp; i < BestKeys<SEL>::BATCH && r0 + i < end; i += 2 * W) {
-                const int64_t row = min(r0 + i + (lane >> 4), end - 1);
-                const float g = __ldcg(p.row_scale + row);
-                const double dot = half_warp_dot<FMT>(p, q, row, lane & 15);
-                if ((lane & 15) == 0 && row == r0 + i + (lane >> 4))
-                    best.offer(row_key(dot, g, gq, row));
-            }
-            found = best.settle(p.k, r0 + BestKeys<SEL>::BATCH >= end);
-        }
+        int found = scan_rows<FMT, SEL>(p, q, gq, begin, end, key, &s_n);
         uint64_t* out = p.parts + (int64_t)item * p.k;
         for (int j = threadIdx.x; j < p.k; j += SEL) out[j] = j < found ? key[j] : 0;
         __threadfence();
@@ -1406,8 +1418,9 @@ static int round_up(int x, int a) { return (x + a - 1) / a * a; }
 // fit what was measured (1M x 1536, us a tile: NV nt 128 1.77, 192 2.00, 256 2.40; MX 1.75,
 // 1.83, 2.35); about 450 cycles more where one accumulator buffer has to be drained before
 // the next tile.  Taken is the nt whose query tiles, spread over the pairs, take the least:
-// 256 for a batch of 1024 (search 0.80 ms against 0.96 at 192), 16 for one query.
-static bool make_plan(int fmt, int dp, int nq, int64_t n_tiles, Plan* out) {
+// 256 for a batch of 1024 (main pass NV 549 us against 727 at 192 and 834 at 128, MX 525, 640
+// and 762), 16 for one query.
+static bool search_plan(int fmt, int dp, int nq, int64_t n_tiles, Plan* out) {
     const int aps = atoms_per_stage(fmt), steps = dp / 64;
     const int kchunks = (dp / 2 + KC - 1) / KC;
     const int stage = A_BYTES + aps * 512;
@@ -1454,6 +1467,22 @@ static bool make_plan(int fmt, int dp, int nq, int64_t n_tiles, Plan* out) {
         }
     }
     return any;
+}
+
+// A call asks for the same plan several times: for its workspace, its queries and each launch.
+static bool make_plan(int fmt, int dp, int nq, int64_t n_tiles, Plan* out) {
+    thread_local int64_t of[4] = {-1, 0, 0, 0};
+    thread_local Plan plan;
+    thread_local bool ok = false;
+    if (of[0] != fmt || of[1] != dp || of[2] != nq || of[3] != n_tiles) {
+        ok = search_plan(fmt, dp, nq, n_tiles, &plan);
+        of[0] = fmt;
+        of[1] = dp;
+        of[2] = nq;
+        of[3] = n_tiles;
+    }
+    *out = plan;
+    return ok;
 }
 
 }  // namespace fp4
@@ -1607,7 +1636,7 @@ int launch_fp4_finish(const Fp4Finish& L, cudaStream_t st) {
     else
         rc = mx ? launch_pdl(finish_kernel<kMX, SEL>, grid, SEL, smem, st, p)
                 : launch_pdl(finish_kernel<kNV, SEL>, grid, SEL, smem, st, p);
-    if (rc != 0) return rc;
+    if (rc != 0 || L.dense) return rc;
     return mx ? launch_pdl(rescue_kernel<kMX>, dim3(RESCUE_CTAS), SEL, smem, st, p)
               : launch_pdl(rescue_kernel<kNV>, dim3(RESCUE_CTAS), SEL, smem, st, p);
 }

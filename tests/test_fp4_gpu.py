@@ -407,7 +407,7 @@ def test_many_overflowing_queries(ctx):
     x[::2] = x[0]
     tx, ex = typed(x, "f32")
     rows = pion_b200.quantize_rows_fp4(ctx, tx, "nv")
-    for nq, same in ((700, 400), (90, 2)):
+    for nq, same in ((700, 400), (90, 2), (40, 30)):
         q = rng.standard_normal((nq, 48))
         q[nq - same:] = x[0] + 0.01 * rng.standard_normal((same, 48))
         tq, eq = typed(q, "f32")
