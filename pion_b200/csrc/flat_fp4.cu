@@ -10,7 +10,10 @@
 //                     scores leave the warp in row order, 128 bytes at a time, and one query
 //                     costs a 16-column MMA beside the stream.  Epilogues: write the scores,
 //                     or keep the rows that reach a query's threshold.
-//   theta_kernel      a query's threshold from its scores of a sample of the rows.
+//   theta_sample_kernel, theta_kernel
+//                     a query's threshold from its scores of a sample of the rows, and from
+//                     its candidates so far.
+//   split_kernel      few queries: the candidates from the scores of every row.
 //   finish_kernel     the k best of a query: its candidates scored exactly, sorted.
 //   rescue_kernel     queries with more candidates than are kept: every row, exactly.
 //

@@ -101,7 +101,10 @@ def _matrix(ctx: Context, x, what: str, dim: int):
 def _slots(ctx: Context, slots, mem: int):
     """The slots as an int64 tensor in the call's memory."""
     if not isinstance(slots, torch.Tensor):
-        slots = torch.from_numpy(np.array(slots, dtype=np.int64))
+        slots = np.asarray(slots)
+        if slots.size and slots.dtype.kind not in "iu":
+            raise TypeError("slots must be a list of integers")
+        slots = torch.from_numpy(slots.astype(np.int64))
     if slots.dim() != 1 or slots.dtype not in (torch.int64, torch.int32):
         raise TypeError("slots must be a list of integers")
     want = torch.device("cuda", _device_of(ctx)) if mem == MEM_DEVICE else torch.device("cpu")
@@ -227,6 +230,8 @@ class FP4Rows:
 def quantize_rows_fp4(ctx: Context, src, format: str = "nv") -> FP4Rows:
     """A new store holding the rows of ``src`` [n, dim], row i in slot i."""
     src = src if isinstance(src, torch.Tensor) else np.asarray(src)
+    if src.ndim != 2:
+        raise ValueError(f"src must be [n, dim], got {tuple(src.shape)}")
     rows = FP4Rows(src.shape[0], src.shape[1], format, torch.device("cuda", _device_of(ctx)))
     rows.write(ctx, src)
     return rows

@@ -104,3 +104,17 @@ def test_layout_round_trip():
     assert np.array_equal(plain.row_scales(flat, 300, 6), bits)
     r, b = 177, 13
     assert flat[((1 * 6 + 3) * 32 + r % 32) * 16 + (r % 128) // 32 * 4 + 1] == bits[r, b]
+
+
+def test_slots_and_shapes_are_refused_before_any_call():
+    import pion_b200
+    import torch
+    from pion_b200 import _lib, fp4
+    assert fp4._slots(None, [3, -1], _lib.MEM_HOST).tolist() == [3, -1]
+    assert fp4._slots(None, np.array([3, 1], np.uint8), _lib.MEM_HOST).dtype == torch.int64
+    assert fp4._slots(None, [], _lib.MEM_HOST).numel() == 0
+    for bad in ([1.5], [True], np.array([1.0, 2.0]), [[1]]):
+        with pytest.raises(TypeError):
+            fp4._slots(None, bad, _lib.MEM_HOST)
+    with pytest.raises(ValueError):
+        pion_b200.quantize_rows_fp4(None, np.zeros(8, np.float32))
