@@ -183,6 +183,29 @@ def test_slots_repeated_skipped_and_out_of_range(ctx):
 
 
 @pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("dim", [40, 1900, 4000, 5000])
+def test_many_rows_for_the_same_slots(ctx, fmt, dim):
+    """More rows than are written by a CTA each, most of them for a slot of a later row, one and
+    two warps a row; again into the same store, whose claims were left at zero."""
+    import pion_b200
+    rng = np.random.default_rng(dim)
+    rows = pion_b200.FP4Rows(700, dim, fmt)
+    x = rows_np(1500, dim, 77)
+    t, exact = typed(x, "f32")
+    for _ in range(2):
+        slots = rng.integers(-20, 600, 1500)
+        rows.clear(ctx)
+        rows.write(ctx, t, slots=torch.from_numpy(slots).cuda())
+        finish(ctx)
+        last = {s: i for i, s in enumerate(slots.tolist()) if s >= 0}
+        at = np.array(sorted(last))
+        check_store(rows, at, exact[[last[s] for s in at.tolist()]], fmt)
+        rest = np.setdiff1d(np.arange(700), at)
+        assert torch.isnan(rows.row_scale[torch.from_numpy(rest).cuda()]).all()
+        assert not rows.claim.any()
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
 @pytest.mark.parametrize("n,dim,nq,types", [
     (1, 1, 1, "f32 f32"), (5, 40, 3, "bf16 f16"), (127, 128, 16, "f32 bf16"),
     (129, 200, 17, "f16 f32"), (1000, 384, 208, "f32 f32"), (700, 1536, 209, "bf16 bf16"),
