@@ -105,13 +105,13 @@ struct alignas(16) Eight {
 
 // The eight elements from column c0 + 8 * lane of a row, zeros past dim.  VEC: rows start at
 // 16-byte boundaries; else the warp's 256 elements come in one by one, side by side, and pass
-// through shared memory.
-template <class T, bool VEC>
+// through shared memory.  FULL: all of them lie inside the row.
+template <class T, bool VEC, bool FULL = false>
 __device__ __forceinline__ Eight<T> load8(const T* row, int c0, int dim, int lane, T* stage) {
     const int c = c0 + 8 * lane;
     Eight<T> e;
     if constexpr (VEC) {
-        if (c + 8 <= dim) {
+        if (FULL || c + 8 <= dim) {
             constexpr int N = sizeof(Eight<T>) / 16;
             uint4* raw = reinterpret_cast<uint4*>(&e);
 #pragma unroll
@@ -245,8 +245,10 @@ __device__ __forceinline__ void row_sync(int base) {
 // WPR warps per row: one or two where rows are many, the CTA's eight where they are few and a
 // row's own latency counts.  An MX row is one pass.  NV needs the row's largest magnitude first; its
 // elements stay in registers between the two passes where a warp's share is at most HOLD
-// steps (HOLD = 0: they are read again).  Bound by HBM: the row, its codes, scales and g once.
-template <int FMT, class T, bool VEC, int W, int WPR, int HOLD>
+// steps (HOLD = 0: they are read again).  FULL: dim is a whole number of steps, in NV WPR HOLD of
+// them, and nothing is checked against the row's end.  Bound by HBM: the row, its codes, scales
+// and g once.
+template <int FMT, class T, bool VEC, int W, int WPR, int HOLD, bool FULL>
 __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
     __shared__ __align__(16) T stage_all[VEC ? 1 : W * STEP];
     __shared__ float s_max[W];
@@ -322,12 +324,12 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
             s2 = fmaf(s, s, s2);
             codes = codes8<FMT>(v, d, bits ? rcp_approx(d) : 0.0f);
         }
-        if (c < p.dp) codes_out[k * 32] = codes;
+        if (FULL || c < p.dp) codes_out[k * 32] = codes;
         // four blocks' bytes to the first lane of their atom
         uint32_t word = bits << (8 * ((lane / BL) & 3));
 #pragma unroll
         for (int o = BL; o < 4 * BL; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-        if (c < p.dp && lane % (4 * BL) == 0)
+        if ((FULL || c < p.dp) && lane % (4 * BL) == 0)
             *reinterpret_cast<uint32_t*>(scales_out + k * (STEP / (32 * BL)) * 512) = word;
     };
     if constexpr (FMT == kMX) {
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (k0 + u * WPR < steps)
-                    e[u] = load8<T, VEC>(row, (k0 + u * WPR) * STEP, p.dim, lane, stage);
+                    e[u] = load8<T, VEC, FULL>(row, (k0 + u * WPR) * STEP, p.dim, lane, stage);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (k0 + u * WPR < steps) {
@@ -357,14 +359,14 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
         if constexpr (HOLD > 0) {
 #pragma unroll
             for (int u = 0; u < H; ++u)
-                if (first + u * WPR < steps)
-                    e[u] = load8<T, VEC>(row, (first + u * WPR) * STEP, p.dim, lane, stage);
+                if (FULL || first + u * WPR < steps)
+                    e[u] = load8<T, VEC, FULL>(row, (first + u * WPR) * STEP, p.dim, lane, stage);
 #pragma unroll
             for (int u = 0; u < H; ++u)
-                if (first + u * WPR < steps) amax = max_abs(amax, top[u] = e[u].top());
+                if (FULL || first + u * WPR < steps) amax = max_abs(amax, top[u] = e[u].top());
         } else {
             for (int k = first; k < steps; k += WPR) {
-                amax = max_abs(amax, load8<T, VEC>(row, k * STEP, p.dim, lane, stage).top());
+                amax = max_abs(amax, load8<T, VEC, FULL>(row, k * STEP, p.dim, lane, stage).top());
             }
         }
         row_max();
@@ -375,13 +377,13 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
         if constexpr (HOLD > 0) {
 #pragma unroll
             for (int u = 0; u < H; ++u)
-                if (first + u * WPR < steps) {
+                if (FULL || first + u * WPR < steps) {
                     e[u].values(v);
                     quantise(first + u * WPR, v, top[u]);
                 }
         } else {
             for (int k = first; k < steps; k += WPR) {
-                e[0] = load8<T, VEC>(row, k * STEP, p.dim, lane, stage);
+                e[0] = load8<T, VEC, FULL>(row, k * STEP, p.dim, lane, stage);
                 e[0].values(v);
                 quantise(k, v, e[0].top());
             }
@@ -514,34 +516,49 @@ __global__ void __launch_bounds__(READ_WARPS * 32) read_kernel(const ReadParams 
     }
 }
 
+template <int FMT, class T, bool VEC, int WPR, int HOLD, bool FULL>
+static int write_many(const WriteParams& p, cudaStream_t st) {
+    constexpr int ROWS = NW / WPR;
+    return launch_pdl(write_kernel<FMT, T, VEC, NW, WPR, HOLD, FULL>,
+                      dim3((unsigned)((p.n + ROWS - 1) / ROWS)), NW * 32, 0, st, p);
+}
+
+// NV rows that fill WPR warps' HOLD steps, and others.
+template <class T, bool VEC, int WPR, int HOLD>
+static int write_held(const WriteParams& p, cudaStream_t st) {
+    return VEC && p.dim == WPR * HOLD * STEP ? write_many<kNV, T, VEC, WPR, HOLD, VEC>(p, st)
+                                             : write_many<kNV, T, VEC, WPR, HOLD, false>(p, st);
+}
+
 template <int FMT, class T, bool VEC>
 static int write_v(const WriteParams& p, cudaStream_t st) {
     // Few rows: a CTA each; many: a warp each (1536 float32 NV elements a row, us: 148 rows 2.4
     // and 3.8, 1024 rows 4.9 and 5.8, 2048 rows 8.5 and 6.6).
     if (p.n <= FEW)
-        return launch_pdl(write_kernel<FMT, T, VEC, WARPS, WARPS, 4>, dim3((unsigned)p.n), WARPS * 32, 0,
-                          st, p);
-    const dim3 grid((unsigned)((p.n + NW - 1) / NW));
+        return launch_pdl(write_kernel<FMT, T, VEC, WARPS, WARPS, 4, false>, dim3((unsigned)p.n),
+                          WARPS * 32, 0, st, p);
     if constexpr (FMT == kNV) {
         // A row stays in one warp's registers while it leaves room for enough warps, then in two
         // warps' (float32 / bfloat16, us, with eight warps a CTA: 262144 x 1536 330 / 285 in
         // one, 365 / 385 in two; 131072 x 2048 284 / 205 and 216 / 226; 65536 x 4096 348 / 266
-        // read twice, 270 / 226 in two; with NW: 310 / 270, 207 / 181, 250 / 195).
-        const dim3 pairs((unsigned)((p.n + NW / 2 - 1) / (NW / 2)));
-        if (p.dp <= 4 * STEP)
-            return launch_pdl(write_kernel<FMT, T, VEC, NW, 1, 4>, grid, NW * 32, 0, st, p);
-        if (p.dp <= 6 * STEP)
-            return launch_pdl(write_kernel<FMT, T, VEC, NW, 1, 6>, grid, NW * 32, 0, st, p);
+        // read twice, 270 / 226 in two; with NW: 310 / 272, 210 / 181, 259 / 195).  Rows that
+        // fill the registers are written without checks (310 / 272 -> 285 / 230, 210 / 181 -> 198 /
+        // 148, 259 / 195 -> 230 / 158).
+        if (p.dp <= 3 * STEP) return write_held<T, VEC, 1, 3>(p, st);
+        if (p.dp <= 4 * STEP) return write_held<T, VEC, 1, 4>(p, st);
+        if (p.dp <= 6 * STEP) return write_held<T, VEC, 1, 6>(p, st);
         if (p.dp <= 8 * STEP) {
             if constexpr (sizeof(T) == 4)
-                return launch_pdl(write_kernel<FMT, T, VEC, NW, 2, 4>, pairs, NW * 32, 0, st, p);
+                return write_held<T, VEC, 2, 4>(p, st);
             else
-                return launch_pdl(write_kernel<FMT, T, VEC, NW, 1, 8>, grid, NW * 32, 0, st, p);
+                return write_held<T, VEC, 1, 8>(p, st);
         }
-        if (p.dp <= 16 * STEP)
-            return launch_pdl(write_kernel<FMT, T, VEC, NW, 2, 8>, pairs, NW * 32, 0, st, p);
+        if (p.dp <= 16 * STEP) return write_held<T, VEC, 2, 8>(p, st);
+        return write_many<FMT, T, VEC, 1, 0, false>(p, st);
+    } else {
+        return VEC && p.dim % STEP == 0 ? write_many<FMT, T, VEC, 1, 0, VEC>(p, st)
+                                        : write_many<FMT, T, VEC, 1, 0, false>(p, st);
     }
-    return launch_pdl(write_kernel<FMT, T, VEC, NW, 1, 0>, grid, NW * 32, 0, st, p);
 }
 
 template <int FMT, class T>

@@ -69,7 +69,8 @@ def check_store(rows, slots, x, fmt):
                                        (64, 128, 8), (257, 384, 0), (20, 777, 7), (33, 1536, 0),
                                        (5, 2049, 0), (2, 8192, 0), (1100, 1536, 0),
                                        (1030, 1900, 0), (1027, 4096, 0), (1025, 5000, 3),
-                                       (1051, 600, 1)])
+                                       (1051, 600, 1), (1026, 768, 0),
+                                       (1029, 1024, 8), (1040, 2048, 0), (1033, 256, 0)])
 def test_write_and_read(ctx, fmt, dtype, n, dim, pad):
     import pion_b200
     x = rows_np(n, dim, n * dim + pad)
