@@ -125,7 +125,7 @@ __device__ __forceinline__ Eight<T> load8(const T* row, int c0, int dim, int lan
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int at = c0 + 32 * j + lane;
-            x[j] = at < dim ? row[at] : from_float<T>(0.0f);
+            x[j] = FULL || at < dim ? row[at] : from_float<T>(0.0f);
         }
         __syncwarp();
 #pragma unroll
@@ -245,10 +245,10 @@ __device__ __forceinline__ void row_sync(int base) {
 // WPR warps per row: one or two where rows are many, the CTA's eight where they are few and a
 // row's own latency counts.  An MX row is one pass.  NV needs the row's largest magnitude first; its
 // elements stay in registers between the two passes where a warp's share is at most HOLD
-// steps (HOLD = 0: they are read again).  FULL: dim is a whole number of steps, in NV WPR HOLD of
-// them, and nothing is checked against the row's end.  Bound by HBM: the row, its codes, scales
+// steps (HOLD = 0: they are read again).  The first OPEN steps of a warp (in MX all, if any) lie
+// inside the row and are not checked against its end.  Bound by HBM: the row, its codes, scales
 // and g once.
-template <int FMT, class T, bool VEC, int W, int WPR, int HOLD, bool FULL>
+template <int FMT, class T, bool VEC, int W, int WPR, int HOLD, int OPEN>
 __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
     __shared__ __align__(16) T stage_all[VEC ? 1 : W * STEP];
     __shared__ float s_max[W];
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
             for (int w = 0; w < WPR; ++w) amax = max_abs(amax, s_max[base + w]);
         }
     };
-    auto quantise = [&](int k, const float(&v)[8], float top) {
+    auto quantise = [&](int k, const float(&v)[8], float top, bool open) {
         const int c = k * STEP + lane * 8;
 #pragma unroll
         for (int o = 1; o < BL; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -324,12 +324,12 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
             s2 = fmaf(s, s, s2);
             codes = codes8<FMT>(v, d, bits ? rcp_approx(d) : 0.0f);
         }
-        if (FULL || c < p.dp) codes_out[k * 32] = codes;
+        if (open || c < p.dp) codes_out[k * 32] = codes;
         // four blocks' bytes to the first lane of their atom
         uint32_t word = bits << (8 * ((lane / BL) & 3));
 #pragma unroll
         for (int o = BL; o < 4 * BL; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-        if ((FULL || c < p.dp) && lane % (4 * BL) == 0)
+        if ((open || c < p.dp) && lane % (4 * BL) == 0)
             *reinterpret_cast<uint32_t*>(scales_out + k * (STEP / (32 * BL)) * 512) = word;
     };
     if constexpr (FMT == kMX) {
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (k0 + u * WPR < steps)
-                    e[u] = load8<T, VEC, FULL>(row, (k0 + u * WPR) * STEP, p.dim, lane, stage);
+                    e[u] = load8<T, VEC, (OPEN > 0)>(row, (k0 + u * WPR) * STEP, p.dim, lane, stage);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (k0 + u * WPR < steps) {
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
                     e[u].values(v);
                     const float top = e[u].top();
                     amax = max_abs(amax, top);
-                    quantise(k0 + u * WPR, v, top);
+                    quantise(k0 + u * WPR, v, top, OPEN > 0);
                 }
         }
         row_max();
@@ -359,14 +359,16 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
         if constexpr (HOLD > 0) {
 #pragma unroll
             for (int u = 0; u < H; ++u)
-                if (FULL || first + u * WPR < steps)
-                    e[u] = load8<T, VEC, FULL>(row, (first + u * WPR) * STEP, p.dim, lane, stage);
+                if (u < OPEN)
+                    e[u] = load8<T, VEC, true>(row, (first + u * WPR) * STEP, p.dim, lane, stage);
+                else if (first + u * WPR < steps)
+                    e[u] = load8<T, VEC>(row, (first + u * WPR) * STEP, p.dim, lane, stage);
 #pragma unroll
             for (int u = 0; u < H; ++u)
-                if (FULL || first + u * WPR < steps) amax = max_abs(amax, top[u] = e[u].top());
+                if (u < OPEN || first + u * WPR < steps) amax = max_abs(amax, top[u] = e[u].top());
         } else {
             for (int k = first; k < steps; k += WPR) {
-                amax = max_abs(amax, load8<T, VEC, FULL>(row, k * STEP, p.dim, lane, stage).top());
+                amax = max_abs(amax, load8<T, VEC>(row, k * STEP, p.dim, lane, stage).top());
             }
         }
         row_max();
@@ -377,15 +379,15 @@ __global__ void __launch_bounds__(W * 32) write_kernel(const WriteParams p) {
         if constexpr (HOLD > 0) {
 #pragma unroll
             for (int u = 0; u < H; ++u)
-                if (FULL || first + u * WPR < steps) {
+                if (u < OPEN || first + u * WPR < steps) {
                     e[u].values(v);
-                    quantise(first + u * WPR, v, top[u]);
+                    quantise(first + u * WPR, v, top[u], u < OPEN);
                 }
         } else {
             for (int k = first; k < steps; k += WPR) {
-                e[0] = load8<T, VEC, FULL>(row, k * STEP, p.dim, lane, stage);
+                e[0] = load8<T, VEC>(row, k * STEP, p.dim, lane, stage);
                 e[0].values(v);
-                quantise(k, v, e[0].top());
+                quantise(k, v, e[0].top(), false);
             }
         }
     }
@@ -516,18 +518,19 @@ __global__ void __launch_bounds__(READ_WARPS * 32) read_kernel(const ReadParams 
     }
 }
 
-template <int FMT, class T, bool VEC, int WPR, int HOLD, bool FULL>
+template <int FMT, class T, bool VEC, int WPR, int HOLD, int OPEN>
 static int write_many(const WriteParams& p, cudaStream_t st) {
     constexpr int ROWS = NW / WPR;
-    return launch_pdl(write_kernel<FMT, T, VEC, NW, WPR, HOLD, FULL>,
+    return launch_pdl(write_kernel<FMT, T, VEC, NW, WPR, HOLD, OPEN>,
                       dim3((unsigned)((p.n + ROWS - 1) / ROWS)), NW * 32, 0, st, p);
 }
 
-// NV rows that fill WPR warps' HOLD steps, and others.
+// NV rows that fill WPR warps' HOLD steps, all but the last, and others.
 template <class T, bool VEC, int WPR, int HOLD>
 static int write_held(const WriteParams& p, cudaStream_t st) {
-    return VEC && p.dim == WPR * HOLD * STEP ? write_many<kNV, T, VEC, WPR, HOLD, VEC>(p, st)
-                                             : write_many<kNV, T, VEC, WPR, HOLD, false>(p, st);
+    if (p.dim == WPR * HOLD * STEP) return write_many<kNV, T, VEC, WPR, HOLD, HOLD>(p, st);
+    if (p.dim >= WPR * (HOLD - 1) * STEP) return write_many<kNV, T, VEC, WPR, HOLD, HOLD - 1>(p, st);
+    return write_many<kNV, T, VEC, WPR, HOLD, 0>(p, st);
 }
 
 template <int FMT, class T, bool VEC>
@@ -535,7 +538,7 @@ static int write_v(const WriteParams& p, cudaStream_t st) {
     // Few rows: a CTA each; many: a warp each (1536 float32 NV elements a row, us: 148 rows 2.4
     // and 3.8, 1024 rows 4.9 and 5.8, 2048 rows 8.5 and 6.6).
     if (p.n <= FEW)
-        return launch_pdl(write_kernel<FMT, T, VEC, WARPS, WARPS, 4, false>, dim3((unsigned)p.n),
+        return launch_pdl(write_kernel<FMT, T, VEC, WARPS, WARPS, 4, 0>, dim3((unsigned)p.n),
                           WARPS * 32, 0, st, p);
     if constexpr (FMT == kNV) {
         // A row stays in one warp's registers while it leaves room for enough warps, then in two
@@ -543,7 +546,8 @@ static int write_v(const WriteParams& p, cudaStream_t st) {
         // one, 365 / 385 in two; 131072 x 2048 284 / 205 and 216 / 226; 65536 x 4096 348 / 266
         // read twice, 270 / 226 in two; with NW: 310 / 272, 210 / 181, 259 / 195).  Rows that
         // fill the registers are written without checks (310 / 272 -> 285 / 230, 210 / 181 -> 198 /
-        // 148, 259 / 195 -> 230 / 158).
+        // 148, 259 / 195 -> 230 / 158), and of others all steps but the last (float16, 100000 x
+        // 777: 78 -> 68, 60000 x 1900: 87 -> 71).
         if (p.dp <= 3 * STEP) return write_held<T, VEC, 1, 3>(p, st);
         if (p.dp <= 4 * STEP) return write_held<T, VEC, 1, 4>(p, st);
         if (p.dp <= 6 * STEP) return write_held<T, VEC, 1, 6>(p, st);
@@ -554,10 +558,10 @@ static int write_v(const WriteParams& p, cudaStream_t st) {
                 return write_held<T, VEC, 1, 8>(p, st);
         }
         if (p.dp <= 16 * STEP) return write_held<T, VEC, 2, 8>(p, st);
-        return write_many<FMT, T, VEC, 1, 0, false>(p, st);
+        return write_many<FMT, T, VEC, 1, 0, 0>(p, st);
     } else {
-        return VEC && p.dim % STEP == 0 ? write_many<FMT, T, VEC, 1, 0, VEC>(p, st)
-                                        : write_many<FMT, T, VEC, 1, 0, false>(p, st);
+        return p.dim % STEP == 0 ? write_many<FMT, T, VEC, 1, 0, 1>(p, st)
+                                 : write_many<FMT, T, VEC, 1, 0, 0>(p, st);
     }
 }
 
