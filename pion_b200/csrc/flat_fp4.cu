@@ -113,15 +113,44 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
                  "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrives on the first CTA's copy of a barrier.  Relaxed: what the arrival stands for (TMEM
-// stores that were waited for, copies that completed on an mbarrier, TMEM loads) is no memory
-// access of this thread, and a release at cluster scope costs a fence per arrival.
+// The address of a shared-memory object of a CTA of the pair, by rank.
+__device__ __forceinline__ uint32_t smem_of(const void* p, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+// Arrives on the first CTA's copy of a barrier.  Relaxed: what the arrival stands for is in TMEM
+// (stores and loads that were waited for, ordered by the tcgen05 fences around the arrival and the
+// wait for it) and no memory access that it would have to pass on; a release at cluster scope
+// costs a fence per arrival.
 __device__ __forceinline__ void mbar_arrive_leader(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(smem_of(bar, 0))
+                 : "memory");
+}
+// A copy into this CTA's shared memory that completes on the first CTA's copy of a barrier, so
+// that the thread which waits there may let the tensor cores read both CTAs' shares.
+__device__ __forceinline__ void tma_load_pair(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
+                                              int32_t x, int32_t y) {
     asm volatile(
-        "{\n\t.reg .b32 remote;\n\tmapa.shared::cluster.u32 remote, %0, 0;\n\t"
-        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [remote];\n\t}\n" ::"r"(
-            smem_u32(bar))
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_of(bar, 0))
         : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
+}
+// Counts bytes of a phase as arrived that no copy will bring.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "r"(bytes)
+                 : "memory");
+}
+// A value for both CTAs' copies of a word.
+__device__ __forceinline__ void tell_pair(int* word, int value) {
+#pragma unroll
+    for (uint32_t r = 0; r < 2; ++r)
+        asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(smem_of(word, r)), "r"(value) : "memory");
 }
 
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_slot, uint32_t ncols) {
@@ -348,10 +377,12 @@ __device__ __forceinline__ int tile_of(const TcParams& p, int j) {
 // ------------------------------------------------------------ the product --
 // A CTA pair works on tiles of 256 rows, 128 per CTA, against its tile of queries: each CTA
 // keeps the codes of half of them in shared memory and streams its rows' codes and scales
-// through a ring.  Scale warps move the scales into TMEM -- the rows' per stage into sets of
-// columns used in turn, the queries' once where they fit (tcgen05.cp was tried first: its
-// copies queue with the MMAs, about 90 ns each, and took longer than them) -- and tell the
-// issuing thread of the first CTA, in one arrival, that codes and scales are there.
+// through a ring.  The codes of both CTAs complete on a barrier of the first, the scales on each
+// CTA's own.  Scale warps move the scales into TMEM -- the rows' per stage into sets of columns used
+// in turn, the queries' once where they fit (tcgen05.cp was tried first: its copies queue with the
+// MMAs, about 90 ns each, and took longer than them) -- and arrive on the barrier of the codes, so
+// that the issuing warp waits once a stage (on a barrier each for codes and scales, a batch's main
+// pass took 3 % longer).
 template <int FMT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     fp4_tc_kernel(const __grid_constant__ CUtensorMap tmap_rows,
@@ -377,18 +408,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     float* s_th = s_gq + MAX_NT;
     uint64_t* s_hits = reinterpret_cast<uint64_t*>(s_th + MAX_NT);
     uint8_t* s_hit_col = reinterpret_cast<uint8_t*>(s_hits + EPI_WARPS * HITS);
-    uint64_t* full = reinterpret_cast<uint64_t*>(s_hit_col + EPI_WARPS * HITS);
-    uint64_t* empty = full + MAX_STAGES;
-    uint64_t* sready = empty + MAX_STAGES;   // per set, on the first CTA: both CTAs' stage is in
-    uint64_t* sfree = sready + MAX_STAGES;
+    uint64_t* full = reinterpret_cast<uint64_t*>(s_hit_col + EPI_WARPS * HITS);  // a stage's scales
+    uint64_t* ready = full + MAX_STAGES;     // on the first CTA: both CTAs' codes, and scales in TMEM
+    uint64_t* empty = ready + MAX_STAGES;
+    uint64_t* sfree = empty + MAX_STAGES;    // per set
     uint64_t* tfull = sfree + MAX_STAGES;
     uint64_t* tempty = tfull + 2;            // on the first CTA
-    uint64_t* bfull = tempty + 2;
-    uint64_t* qsf_done = bfull + 1;
+    uint64_t* bfull = tempty + 2;            // the queries' scales
+    uint64_t* bcodes = bfull + 1;            // on the first CTA: both CTAs' queries' codes
+    uint64_t* qsf_done = bcodes + 1;
     uint64_t* drain = qsf_done + 1;
     uint64_t* stall = drain + 1;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(stall + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    // at the end, alike in both CTAs: whether every MMA was issued, and the stages that each CTA has
+    // copied and each of its scale warps has put into TMEM
+    int* finished = const_cast<int*>(abort_flag) + 1;
+    int* copied = finished + 1;
+    int* scaled = copied + 2;
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);  // warp-uniform
     const int lane = threadIdx.x & 31;
@@ -405,8 +442,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < MAX_STAGES; ++s) {
             mbar_init(&full[s], 1);
+            mbar_init(&ready[s], 1 + 2 * SCALE_WARPS);
             mbar_init(&empty[s], 1 + SCALE_WARPS);
-            mbar_init(&sready[s], 2 * SCALE_WARPS);
             mbar_init(&sfree[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -414,10 +451,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             mbar_init(&tempty[b], 2 * EPI_WARPS);
         }
         mbar_init(bfull, 1);
+        mbar_init(bcodes, 1);
         mbar_init(qsf_done, SCALE_WARPS);
         mbar_init(drain, 1);
         mbar_init(stall, 1);
         *abort_flag = 0;
+        *finished = 0;
+        copied[0] = copied[1] = 0;
         fence_barrier_init();
     }
     if (warp == 5) tmem_alloc_pair(tmem_slot, TMEM_COLS);
@@ -470,7 +510,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(qsf_done);
-        int stage = 0, set = 0;
+        int stage = 0, set = 0, done = 0;
         uint32_t phase = 0, set_phase = 0;
         for (int j = first; j < p.n_tiles && ok; j += stride) {
             for (int kc = 0; kc < kchunks; ++kc) {
@@ -493,9 +533,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive_leader(&sready[set]);
+                    mbar_arrive_leader(&ready[stage]);
                     mbar_arrive(&empty[stage]);
                 }
+                ++done;
                 if (++stage == stages) {
                     stage = 0;
                     phase ^= 1u;
@@ -506,6 +547,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 }
             }
         }
+        if (lane == 0) tell_pair(&scaled[(int)rank * SCALE_WARPS + warp], done);
+        __syncwarp();
     } else if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
         if (warp == 4 && lane == 0) {
@@ -513,18 +556,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             tma_prefetch_desc(&tmap_rows);
             tma_prefetch_desc(&tmap_row_sf);
             const int half_nt = nt / 2;
-            mbar_arrive_expect_tx(bfull, (uint32_t)(kchunks * half_nt * KC +
-                                                    sf_tiles * kchunks * APS * 512));
+            mbar_arrive_expect_tx(bfull, (uint32_t)(sf_tiles * kchunks * APS * 512));
+            if (rank == 0) mbar_arrive_expect_tx(bcodes, (uint32_t)(2 * kchunks * half_nt * KC));
             for (int kc = 0; kc < kchunks; ++kc) {
-                tma_load_2d(sB + kc * half_nt * KC, &tmap_q, bfull, kc * KC,
-                            qt * p.plan.nt_pad + (int)rank * half_nt);
+                tma_load_pair(sB + kc * half_nt * KC, &tmap_q, bcodes, kc * KC,
+                              qt * p.plan.nt_pad + (int)rank * half_nt);
                 for (int h = 0; h < sf_tiles; ++h)
                     tma_load_2d(sSF + (h * kchunks + kc) * APS * 512, &tmap_q_sf, bfull, 0,
                                 (qt * sf_tiles + h) * p.atoms + kc * APS);
             }
             // The ring holds the queries' scales until they are in TMEM.
             bool ok = mbar_wait(qsf_done, 0, p.status, abort_flag, p.wait_ns);
-            int stage = 0;
+            int stage = 0, loads = 0;
             uint32_t phase = 0, issued = 0, parity = 0;  // bits by stage
             for (int j = first; j < p.n_tiles && ok; j += stride) {
                 const int half_tile = tile_of(p, j) * 2 + (int)rank;
@@ -534,10 +577,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         break;
                     }
                     uint8_t* dst = ring + stage * STAGE;
-                    mbar_arrive_expect_tx(&full[stage], STAGE);
-                    tma_load_2d(dst, &tmap_rows, &full[stage], kc * KC, half_tile * HALF);
+                    // (the other CTA's codes may land on the barrier before this arrival: its
+                    // phase ends with it)
+                    if (rank == 0) mbar_arrive_expect_tx(&ready[stage], 2 * A_BYTES);
+                    mbar_arrive_expect_tx(&full[stage], APS * 512);
+                    tma_load_pair(dst, &tmap_rows, &ready[stage], kc * KC, half_tile * HALF);
                     tma_load_2d(dst + A_BYTES, &tmap_row_sf, &full[stage], 0,
                                 half_tile * p.atoms + kc * APS);
+                    ++loads;
                     issued |= 1u << stage;
                     parity = (parity & ~(1u << stage)) | (phase << stage);
                     if (++stage == stages) {
@@ -547,11 +594,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 }
             }
             // Every copy this thread issued lands before the CTA may exit (a wait of its own
-            // length: the caller's budget may have run out).
+            // length: the caller's budget may have run out); the codes are waited for below.
             mbar_wait(bfull, 0, p.status, nullptr, kWaitBudgetNs);
+            if (rank == 0) mbar_wait(bcodes, 0, p.status, nullptr, kWaitBudgetNs);
             for (int s = 0; s < stages; ++s)
                 if ((issued >> s) & 1u)
                     mbar_wait(&full[s], (parity >> s) & 1u, p.status, nullptr, kWaitBudgetNs);
+            tell_pair(&copied[rank], loads);
         } else if (warp == 5 && rank == 0) {
             // --------------------------------------------------- MMA issuer
             // The whole warp runs the loop, so that every operand is in a uniform register; one
@@ -563,17 +612,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const uint32_t b_step = (uint32_t)(nt / 2) * KC >> 4;
             const bool one = elect_one();
             int stage = 0, set = 0, buf = 0;
-            uint32_t set_phase = 0, buf_phase = 0;
+            uint32_t phase = 0, buf_phase = 0;
             bool ok = !p.test_stall || blockIdx.x != 0;
             if (!ok) mbar_wait(stall, 0, p.status, abort_flag, p.wait_ns);
+            ok = ok && __all_sync(0xffffffffu,
+                                  mbar_wait(bcodes, 0, p.status, abort_flag, p.wait_ns));
             for (int j = first; j < p.n_tiles && ok; j += stride) {
-                if (!__all_sync(0xffffffffu, mbar_wait(&tempty[buf], buf_phase ^ 1u, p.status,
-                                                       abort_flag, p.wait_ns)))
-                    break;
+                ok = __all_sync(0xffffffffu, mbar_wait(&tempty[buf], buf_phase ^ 1u, p.status,
+                                                       abort_flag, p.wait_ns));
+                if (!ok) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(buf * nt);
                 for (int kc = 0; kc < kchunks; ++kc) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sready[set], set_phase, p.status,
+                    ok = __all_sync(0xffffffffu, mbar_wait(&ready[stage], phase, p.status,
                                                            abort_flag, p.wait_ns));
                     if (!ok) break;
                     tc_fence_after();
@@ -602,11 +653,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         if (kc == kchunks - 1) tc_commit_pair(&tfull[buf]);
                     }
                     __syncwarp();
-                    if (++stage == stages) stage = 0;
-                    if (++set == sets) {
-                        set = 0;
-                        set_phase ^= 1u;
+                    if (++stage == stages) {
+                        stage = 0;
+                        phase ^= 1u;
                     }
+                    if (++set == sets) set = 0;
                 }
                 if (++buf == bufs) {
                     buf = 0;
@@ -614,7 +665,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 }
             }
             // All MMAs issued above complete before TMEM is released.
-            if (one) tc_commit_pair(drain);
+            if (one) {
+                tc_commit_pair(drain);
+                tell_pair(finished, ok);
+            }
             __syncwarp();
             mbar_wait(drain, 0, p.status, nullptr, kWaitBudgetNs);
         } else if (warp == 5) {
@@ -684,6 +738,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     tc_fence_before();
     cluster_sync();
+    if (!*finished) {
+        // A wait ran out.  Codes may be on their way into either CTA, whose barriers lie in the
+        // first: what one CTA has not copied of the stages that the other has, and what scale
+        // warps have not put into TMEM, is made up for, then each stage's last phase waited for.
+        // (Phases before it are complete: a stage is copied again once it has been multiplied.)
+        if (rank == 0 && warp == 4 && lane == 0) {
+            const int most = max(copied[0], copied[1]);
+            for (int i = max(most - stages, 0); i < most; ++i) {
+                uint64_t* bar = &ready[i % stages];
+                if (i >= copied[0])
+                    mbar_arrive_expect_tx(bar, A_BYTES);
+                else if (i >= copied[1])
+                    mbar_complete_tx(bar, A_BYTES);
+                int missing = 0;
+                for (int w = 0; w < 2 * SCALE_WARPS; ++w) missing += scaled[w] <= i;
+                if (missing) mbar_arrive_n(bar, (uint32_t)missing);
+                mbar_wait(bar, (uint32_t)(i / stages) & 1u, p.status, nullptr, kWaitBudgetNs);
+            }
+        }
+        __syncwarp();
+        cluster_sync();
+    }
     if (warp == 5) {
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, TMEM_COLS);
