@@ -118,14 +118,14 @@ __device__ __forceinline__ Eight<T> load8(const T* row, int c0, int dim, int lan
             for (int j = 0; j < N; ++j) raw[j] = __ldcg(reinterpret_cast<const uint4*>(row + c) + j);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e.x[j] = c + j < dim ? row[c + j] : from_float<T>(0.0f);
+            for (int j = 0; j < 8; ++j) e.x[j] = c + j < dim ? __ldcg(row + c + j) : from_float<T>(0.0f);
         }
     } else {
         T x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int at = c0 + 32 * j + lane;
-            x[j] = FULL || at < dim ? row[at] : from_float<T>(0.0f);
+            x[j] = FULL || at < dim ? __ldcg(row + at) : from_float<T>(0.0f);
         }
         __syncwarp();
 #pragma unroll
@@ -231,7 +231,7 @@ __global__ void claim_kernel(const int64_t* slots, int64_t n, int64_t n_slots,
     griddep_wait();
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= n) return;
-    const int64_t s = slots[i];
+    const int64_t s = __ldcg(slots + i);
     if (s >= n_slots) record_error(status, PION_B200_EINVAL);
     if (s >= 0 && s < n_slots) atomicMax(&claim[s], (int32_t)(i + 1));
 }
