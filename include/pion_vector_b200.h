@@ -531,9 +531,11 @@ int pion_v_b200_fp4_scores(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, i
                            int out_type, int64_t out_stride, void *workspace,
                            int64_t workspace_bytes, int mem, void *cuda_stream);
 /* The k best of slots [0, n_rows) by (score desc, slot asc) -> out_ids (id_base + slot) and
- * out_scores [nq x k]; -1 / -inf past the rows that are not empty.  Here a score is
- * f32(((sum) g_r) g_t) of the sum in float64, so the ids do not depend on an order of
- * summation.  k <= 256.  A query whose candidates overflow (thousands of rows that tie with
+ * out_scores [nq x k]; -1 / -inf past the rows that are not empty.  Here a score is the exact
+ * ((sum) g_r) g_t, rounded once to float32, so the ids do not depend on an order of
+ * summation.  (Which rows are summed exactly goes by the tensor cores' float32 sums and a bound
+ * of their error, (dp / 64 + 8) 2^-22 of the norms' product, that rests on measurement: at
+ * least 15 times the largest error seen.)  k <= 256.  A query whose candidates overflow (thousands of rows that tie with
  * its k-th, or are as near to it as float32 sums with the longest row's norm can tell) is
  * answered by an exact scan of the rows: right, but about 1 ms a query and million rows. */
 int pion_v_b200_flat_fp4_knn(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, int64_t n_rows,

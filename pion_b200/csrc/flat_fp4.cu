@@ -17,11 +17,12 @@
 //   finish_kernel     the k best of a query: its candidates scored exactly, sorted.
 //   rescue_kernel     queries with more candidates than are kept: every row, exactly.
 //
-// Exactness: a product of two codes is a multiple of 1/4 up to 36, and a row's scales span a
-// few powers of two, so the sum in float64 is exact; it is rounded once to float32, and rows
-// with equal scores rank by id.  The tensor cores' float32 sums only choose which rows are
-// summed again: with |approximate - exact| <= eps, a row among the k best scores at least
-// the k-th best approximate score of any subset less 2 eps.
+// Exactness: a product of two codes is a multiple of 1/4 up to 36 and a scale one of few bits, so
+// sums are held as integers (or, in MX, in float64 where a row's exponents lie near enough to each
+// other for that to be the same); ((sum) g_r) g_t is rounded once to float32, and rows with equal
+// scores rank by id.  The tensor cores' float32 sums only choose which rows are summed again: with
+// |approximate - exact| <= eps, a row among the k best scores at least the k-th best approximate
+// score of any subset less 2 eps.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -1168,22 +1169,108 @@ struct FinishParams {
     float* out_scores;
 };
 
-// Query block scales as float, codes as bytes (twice their value).
+// The query's codes as bytes (twice their value); its block scales in units of 2^-9 (NV), or their
+// exponents (MX).
 struct QueryShared {
     int8_t* codes;
-    float* scales;
+    uint32_t* scales;
 };
 
-// sum_j q_j v_j in units of both g, by half a warp (`sub`: the lane's place in it): exact integer
-// sums per block, float64 over the blocks.  A lane's loads of 64 blocks of 32 elements are in
-// flight together.
+constexpr long long kMantissa = (1ll << 52) - 1;  // of a float64
+
+// 2^e as a float64, -1022 <= e <= 1023.
+__device__ __forceinline__ double power_of_two(int e) { return __hiloint2double((e + 1023) << 20, 0); }
+
+// A sum of products in units of both rows' g: m 2^e exactly, or where |m| has its highest bit at 61,
+// m 2^e towards zero with the last bit set for what is left out.
+struct Sum {
+    long long m;
+    int e;
+};
+
+// sum of q_j v_j over the block of 32 elements `raw`, four times over, in halves.
+__device__ __forceinline__ void block_dots(const uint4& w, const int8_t* q, int (&dot)[2]) {
+    const uint32_t raw[4] = {w.x, w.y, w.z, w.w};
+    const int4* qb = reinterpret_cast<const int4*>(q);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int4 qq = qb[h];
+        dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h]), qq.x, 0);
+        dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h] >> 16), qq.y, dot[h]);
+        dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h + 1]), qq.z, dot[h]);
+        dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h + 1] >> 16), qq.w, dot[h]);
+    }
+}
+
+// MX sums whose blocks' exponents lie far apart, by half a warp: an integer of 16 digits of 32 bits
+// (and a carry), a lane's digit the sum of those blocks' products that begin in it.
+__device__ __noinline__ Sum half_warp_far_dot(const uint4* codes, const uint8_t* scales,
+                                              const int8_t* q_codes, const uint32_t* q_scales,
+                                              int blocks, int sub) {
+    long long digit = 0;  // at most 256 blocks of 13 bits and 31: 53 bits
+    for (int b0 = 0; b0 < blocks; b0 += 16) {
+        const int b = b0 + sub;
+        int dot[2] = {0, 0}, e = 0;
+        if (b < blocks) {
+            block_dots(__ldcg(codes + b), q_codes + b * 32, dot);
+            e = (int)(q_scales[b] + __ldcg(scales + (b >> 2) * 512 + (b & 3)));  // 0 to 504
+        }
+        const int mine = dot[0] + dot[1];
+        for (int i = 0; i < 16; ++i) {
+            const int d = __shfl_sync(0xffffffffu, mine, i, 16);
+            const int at = __shfl_sync(0xffffffffu, e, i, 16);
+            if (at >> 5 == sub) digit += (long long)d << (at & 31);
+        }
+    }
+    // The sign, then the magnitude's digits, from the lowest.
+    bool negative = false;
+    uint32_t d = 0, top = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        long long carry = 0;
+        for (int i = 0; i < 16; ++i) {
+            const long long x = __shfl_sync(0xffffffffu, digit, i, 16) + carry;
+            if (i == sub) d = (uint32_t)x;
+            carry = x >> 32;
+        }
+        top = (uint32_t)carry;
+        if (pass == 0) {
+            negative = carry < 0;
+            if (negative) digit = -digit;
+        }
+    }
+    // The highest digit that is not zero (the carry is the 17th), and the two below it.
+    const unsigned half = (threadIdx.x & 16) ? 16 : 0;
+    const unsigned some = (__ballot_sync(0xffffffffu, d != 0) >> half) & 0xFFFFu;
+    const int h = top ? 16 : some ? 31 - __clz((int)some) : 0;
+    const uint32_t d0 = __shfl_sync(0xffffffffu, d, h & 15, 16);
+    const uint32_t d1 = __shfl_sync(0xffffffffu, d, (h - 1) & 15, 16);
+    const uint32_t d2 = __shfl_sync(0xffffffffu, d, (h - 2) & 15, 16);
+    const uint32_t a = h == 16 ? top : d0, b = h >= 1 ? d1 : 0u, c = h >= 2 ? d2 : 0u;
+    if (a == 0) return {0, 0};
+    const bool below = h >= 3 && (some & ((1u << (h - 2)) - 1u)) != 0;
+    const int z = __clz((int)a);
+    uint64_t m = ((uint64_t)a << 32 | b) << z;
+    if (z) m |= c >> (32 - z);
+    const bool rest = (uint32_t)(c << z) != 0 || below;  // (z < 32)
+    m = m >> 2 | ((m & 3u) != 0 || rest ? 1u : 0u);
+    // the digits' unit is 2^-256: a quarter of 2^-254
+    return {negative ? -(long long)m : (long long)m, 32 * (h - 1) - z + 2 - 256};
+}
+
+// sum_j q_j v_j by half a warp (`sub`: the lane's place in it), in all its lanes.  NV: in units of
+// 2^-20 a block's sum has at most 48 bits and a row's 57, an integer.  MX: a block's sum is an integer
+// of 13 bits times a power of two; where those of a row are at most 2^32 apart, any order of them adds
+// up in float64 without rounding.  A lane's loads of 64 blocks of 32 elements are in flight together.
 template <int FMT>
-__device__ __forceinline__ double half_warp_dot(const FinishParams& p, const QueryShared& q,
-                                                int64_t row, int sub) {
+__device__ __forceinline__ Sum half_warp_dot(const FinishParams& p, const QueryShared& q, int64_t row,
+                                             int sub) {
+    static_assert(kMaxDim / 32 * (36 * 4 * 32) <= 1 << 21, "53 bits");
     const uint4* codes = reinterpret_cast<const uint4*>(p.codes + row * (p.dp / 2));
     const uint8_t* scales = p.scales + scale_word(row, 0, p.atoms);
     const int blocks = p.dp / 32;
     double acc = 0.0;
+    uint32_t reach = 0;  // the highest exponent, and 511 less the lowest
+    long long sum = 0;
     for (int b0 = sub; b0 < blocks; b0 += 64) {
         uint4 w[4];
         uint32_t s[4];
@@ -1203,36 +1290,69 @@ __device__ __forceinline__ double half_warp_dot(const FinishParams& p, const Que
         for (int u = 0; u < 4; ++u) {
             const int b = b0 + 16 * u;
             if (b >= blocks) break;
-            const uint32_t raw[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-            const int4* qb = reinterpret_cast<const int4*>(q.codes + b * 32);
-            int dot[2] = {0, 0};
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int4 qq = qb[h];
-                dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h]), qq.x, dot[h]);
-                dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h] >> 16), qq.y, dot[h]);
-                dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h + 1]), qq.z, dot[h]);
-                dot[h] = __dp4a((int)e2m1x4_bytes(raw[2 * h + 1] >> 16), qq.w, dot[h]);
-            }
+            int dot[2];
+            block_dots(w[u], q.codes + b * 32, dot);
             if (FMT == kMX) {
-                acc += (double)(dot[0] + dot[1]) *
-                       ((double)q.scales[b] * (double)e8m0_value(s[u]));
+                const uint32_t e = q.scales[b] + s[u];
+                const int d = dot[0] + dot[1];
+                acc = fma((double)d, power_of_two((int)e - 254), acc);
+                if (d != 0) reach = __vmaxu2(reach, e << 16 | (511u - e));
             } else {
-                acc += (double)dot[0] *
-                       ((double)q.scales[2 * b] * (double)e4m3_value(s[u] & 255u));
-                acc += (double)dot[1] *
-                       ((double)q.scales[2 * b + 1] * (double)e4m3_value(s[u] >> 8));
+                sum += (long long)(dot[0] * (int)e4m3_units(s[u] & 255u)) * (int)q.scales[2 * b];
+                sum += (long long)(dot[1] * (int)e4m3_units(s[u] >> 8)) * (int)q.scales[2 * b + 1];
             }
         }
     }
+    if constexpr (FMT == kMX) {
 #pragma unroll
-    for (int o = 8; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    return 0.25 * acc;
+        for (int o = 8; o; o >>= 1) {
+            acc += __shfl_xor_sync(0xffffffffu, acc, o);
+            reach = __vmaxu2(reach, __shfl_xor_sync(0xffffffffu, reach, o));
+        }
+        const bool far = (int)(reach >> 16) + (int)(reach & 0xFFFFu) - 511 > 32;
+        if (__any_sync(0xffffffffu, far)) {
+            const Sum x = half_warp_far_dot(codes, scales, q.codes, q.scales, blocks, sub);
+            if (far) return x;
+        }
+        const long long bits = __double_as_longlong(acc);
+        const int exponent = (int)(bits >> 52) & 0x7FF;  // at least 1023 - 254 where acc is not 0
+        const long long m = exponent ? (bits & kMantissa) | 1ll << 52 : 0;
+        return {bits < 0 ? -m : m, exponent - 1075 - 2};
+    } else {
+#pragma unroll
+        for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        return {sum, -20};
+    }
+}
+
+// ((m 2^e) g_r) g_t, rounded once to float32.  The two scales' product has 48 bits: a float64.  The
+// whole is rounded to the 53 bits of one with its last bit set for what is left out, so that the
+// rounding to float32 is that of the exact product.
+__device__ __forceinline__ float exact_score(Sum x, float g, float gq) {
+    const double scale = (double)g * (double)gq;
+    if (x.m == 0 || !(fabs(scale) > 0.0)) return (float)(scale * 0.0);  // (NaN for a NaN)
+    const uint64_t a = (uint64_t)(x.m < 0 ? -x.m : x.m);
+    if (a <= 1ull << 53) {
+        const double v = (double)x.m * power_of_two(x.e);
+        const double y = v * scale, left = fma(v, scale, -y);
+        long long bits = __double_as_longlong(y);
+        if (left != 0.0) bits = (bits - ((left > 0.0) != (y > 0.0))) | 1;
+        return (float)__longlong_as_double(bits);
+    }
+    const long long bits = __double_as_longlong(scale);
+    const uint64_t f = (uint64_t)((bits & kMantissa) | 1ll << 52) >> 5;
+    const uint64_t hi = __umul64hi(a, f), lo = a * f;  // 2^100 to 2^110
+    const int n = 64 - __clzll((long long)hi);
+    const uint64_t top = hi << (64 - n) | lo >> n;
+    const bool rest = lo << (64 - n) != 0 || (top & 0x7FFu) != 0;
+    const double v = (double)(long long)(top >> 11 | (rest ? 1u : 0u)) *
+                     power_of_two(x.e + ((int)(bits >> 52) & 0x7FF) - 1075 + 5 + n + 11);
+    return (float)((x.m < 0) != (bits < 0) ? -v : v);
 }
 
 // Larger is better: (score desc, row asc); 0 for a row that cannot be found.
-__device__ __forceinline__ uint64_t row_key(double dot, float g, float gq, int64_t row) {
-    const float s = (float)((dot * (double)g) * (double)gq) + 0.0f;
+__device__ __forceinline__ uint64_t row_key(Sum dot, float g, float gq, int64_t row) {
+    const float s = exact_score(dot, g, gq) + 0.0f;
     if (!(s > -INFINITY)) return 0;
     return ((uint64_t)ordered(s) << 32) | (uint32_t)~(uint32_t)row;
 }
@@ -1244,8 +1364,10 @@ __device__ __forceinline__ void load_query(const FinishParams& p, const QuerySha
     const uint16_t* codes = reinterpret_cast<const uint16_t*>(p.q_codes + qs * (p.dp / 2));
     for (int i = at; i < p.dp / 4; i += NT)
         reinterpret_cast<uint32_t*>(q.codes)[i] = e2m1x4_bytes(__ldcg(codes + i));
-    for (int b = at; b < p.dp / block_of(FMT); b += NT)
-        q.scales[b] = scale_value<FMT>(__ldcg(p.q_scales + scale_word(qs, b >> 2, p.atoms) + (b & 3)));
+    for (int b = at; b < p.dp / block_of(FMT); b += NT) {
+        const uint32_t byte = __ldcg(p.q_scales + scale_word(qs, b >> 2, p.atoms) + (b & 3));
+        q.scales[b] = FMT == kMX ? byte : e4m3_units(byte);
+    }
 }
 
 template <int NT>
@@ -1300,7 +1422,7 @@ __device__ int scan_rows(const FinishParams& p, const QueryShared& q, float gq, 
         for (int i = 2 * warp; i < BATCH && r0 + i < end; i += 2 * W) {
             const int64_t row = min(r0 + i + (lane >> 4), end - 1);
             const float g = __ldcg(p.row_scale + row);
-            const double dot = half_warp_dot<FMT>(p, q, row, lane & 15);
+            const Sum dot = half_warp_dot<FMT>(p, q, row, lane & 15);
             if ((lane & 15) == 0 && row == r0 + i + (lane >> 4))
                 best.offer(row_key(dot, g, gq, row));
         }
@@ -1336,7 +1458,7 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 4) finish_kernel(const Fini
     const float two_eps = 2.0f * eps_of(p.dp, __ldcg(p.q_norm + t), gq, __ldcg(p.norm_max));
     QueryShared q;
     q.codes = reinterpret_cast<int8_t*>(dyn);
-    q.scales = reinterpret_cast<float*>(dyn + p.dp);
+    q.scales = reinterpret_cast<uint32_t*>(dyn + p.dp);
     if (warp > 0) load_query<FMT, NT - 32>(p, q, qs, threadIdx.x - 32);
     if (threadIdx.x == 0) s_n = 0;
 
@@ -1397,7 +1519,7 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 4) finish_kernel(const Fini
                     const int i = min(i0 + (lane >> 4), s_n - 1);
                     const int64_t row = (int64_t)key[i];
                     const float g = __ldcg(p.row_scale + row);
-                    const double dot = half_warp_dot<FMT>(p, q, row, lane & 15);
+                    const Sum dot = half_warp_dot<FMT>(p, q, row, lane & 15);
                     // (an odd one out is done by both halves, and written by the first)
                     if ((lane & 15) == 0 && i == i0 + (lane >> 4)) key[i] = row_key(dot, g, gq, row);
                 }
@@ -1455,7 +1577,7 @@ __global__ void __launch_bounds__(SEL) rescue_kernel(const FinishParams p) {
     if (flagged == 0) return;
     QueryShared q;
     q.codes = reinterpret_cast<int8_t*>(dyn);
-    q.scales = reinterpret_cast<float*>(dyn + p.dp);
+    q.scales = reinterpret_cast<uint32_t*>(dyn + p.dp);
     const int splits = max(1, RESCUE_CTAS / flagged);
     for (int item = blockIdx.x; item < flagged * splits; item += gridDim.x) {
         const int t = __ldcg(p.flagged + item / splits);

@@ -128,6 +128,12 @@ __device__ __forceinline__ float e4m3_value(uint32_t byte) {
     return v;
 }
 
+// In units of 2^-9, the least of them: an integer up to 448 * 512.
+__device__ __forceinline__ uint32_t e4m3_units(uint32_t byte) {
+    const uint32_t e = byte >> 3, m = byte & 7u;
+    return e ? (8u | m) << (e - 1u) : m;
+}
+
 // 2^(byte - 127), exact down to the subnormal 2^-127.
 __device__ __forceinline__ float e8m0_value(uint32_t byte) {
     return byte ? __uint_as_float(byte << 23) : __uint_as_float(0x00400000u);
