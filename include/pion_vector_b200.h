@@ -522,8 +522,9 @@ int pion_v_b200_fp4_read(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows,
 int64_t pion_v_b200_fp4_workspace(const pion_b200_fp4_rows *rows, int64_t n_rows, int64_t nq,
                                   int64_t k);
 /* Scores of every query with the rows of slots [0, n_rows): out[t * out_stride + r] =
- * ((sum_j q_j v_j) g_r) g_t, accumulated and multiplied in float32.  q: nq rows of q_type, quantised here
- * in the store's format.  With `mem` DEVICE the scratch is the caller's `workspace`
+ * ((sum_j q_j v_j) g_r) g_t, accumulated and multiplied in float32 (what leaves it is infinite, by
+ * the sign with which it did); -inf for an empty row or query.  q: nq rows of q_type, quantised
+ * here in the store's format.  With `mem` DEVICE the scratch is the caller's `workspace`
  * (16-byte aligned; pion_v_b200_fp4_workspace bytes), or the context's where both it and
  * cuda_stream are NULL. */
 int pion_v_b200_fp4_scores(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, int64_t n_rows,

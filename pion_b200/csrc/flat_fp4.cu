@@ -241,7 +241,8 @@ template <>
 __device__ __forceinline__ __half cast_out<__half>(float v) { return __float2half_rn(v); }
 
 // One 32-column chunk of one row's scores, the first n of them, to out[t][col], t from t0.  NaN,
-// which an empty row's or query's scale makes of a score, becomes -inf.
+// which an empty row's or query's scale makes of a score, becomes -inf.  (A live row has none: an
+// accumulator that has become infinite stays so, also where the other infinity is added.)
 template <class T, bool FULL>
 __device__ __forceinline__ void store_columns(const uint32_t (&r)[32], T* out, int64_t ld, int n,
                                               const float* gq, float g) {

@@ -150,3 +150,29 @@ def test_products_past_float32_that_cancel(ctx, n, copies):
         x[i, 1024 + rng.integers(0, 512)] = 2.0 ** -40 * (1 + i % 2)
         x[i, 1536 + rng.integers(0, 512)] = 2.0 ** 30 if i % 5 == 0 else 0
     check(ctx, q, x, "mx", 10, copies)
+
+
+def test_sums_that_leave_float32_are_no_empty_slots(ctx):
+    """-inf is an empty row's or query's score; a live one's sum past float32 is infinite by the sign
+    with which it left float32."""
+    import pion_b200
+    x = np.zeros((6, 256), np.float32)
+    q = np.zeros((4, 256), np.float32)
+    q[0, ::32] = 2.0 ** 100
+    q[1, ::32] = 1
+    q[3, 0] = np.nan
+    x[0, ::32] = 2.0 ** 100 * np.array([1, 1, -1, -1] * 2)
+    x[1, ::32] = 2.0 ** 100
+    x[2, ::32] = -2.0 ** 100
+    x[3, 0] = np.inf
+    x[4, ::32] = 1
+    rows = pion_b200.quantize_rows_fp4(ctx, torch.from_numpy(x).cuda(), "mx")
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        s = pion_b200.fp4_scores(ctx, rows, torch.from_numpy(q).cuda(), dtype=dtype)
+        torch.cuda.synchronize()
+        ctx.sync()
+        s = s.double().cpu().numpy()
+        assert s[0, 0] == np.inf and s[0, 1] == np.inf and s[0, 2] == -np.inf
+        assert np.isneginf(s[:, 3]).all() and np.isneginf(s[3]).all()
+        assert s[1, 0] == 0 and (s[2, [0, 1, 2, 4, 5]] == 0).all() and s[1, 4] == 8
+        assert (s[:3, 5] == 0).all()
