@@ -104,6 +104,8 @@ def _slots(ctx: Context, slots, mem: int):
         slots = np.asarray(slots)
         if slots.size and slots.dtype.kind not in "iu":
             raise TypeError("slots must be a list of integers")
+        if slots.dtype.kind == "u" and slots.size and int(slots.max()) > np.iinfo(np.int64).max:
+            raise ValueError("a slot is past 64 bits")
         slots = torch.from_numpy(slots.astype(np.int64))
     if slots.dim() != 1 or slots.dtype not in (torch.int64, torch.int32):
         raise TypeError("slots must be a list of integers")
