@@ -155,6 +155,8 @@ class FP4Rows:
                  scales=None, row_scale=None, norm_max=None, claim=None):
         cb, sb = _sizes(format, n_rows, dim)
         if codes is None and scales is None and row_scale is None and norm_max is None:
+            if claim is not None:
+                raise ValueError("claim is given with codes, scales, row_scale and norm_max only")
             device = torch.device("cuda" if device is None else device)
             codes = torch.zeros((n_rows, cb // max(n_rows, 1)), dtype=torch.uint8, device=device)
             scales = torch.zeros(sb, dtype=torch.uint8, device=device)

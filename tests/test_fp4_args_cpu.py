@@ -13,3 +13,12 @@ def test_slots_past_64_bits_are_refused():
     good = fp4._slots(None, np.array([1, 2 ** 63 - 1], np.uint64), _lib.MEM_HOST)
     assert good.tolist() == [1, 2 ** 63 - 1]
     assert fp4._slots(None, np.zeros(0, np.uint64), _lib.MEM_HOST).numel() == 0
+
+
+def test_a_lone_claim_buffer_is_refused():
+    """A store is made of no given tensors, or of all but the claims: given alone, they would be
+    dropped."""
+    import pion_b200
+    claim = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="claim"):
+        pion_b200.FP4Rows(4, 16, "nv", device="cpu", claim=claim)
