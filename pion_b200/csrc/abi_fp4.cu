@@ -416,7 +416,7 @@ int pion_v_b200_fp4_write(pion_b200_ctx* ctx, const pion_b200_fp4_rows* rows, co
             w.slots = ds;
         }
     }
-    ctx->launches += slots ? 2 : 1;
+    ctx->launches += fp4_write_launches(slots != nullptr, n);
     if (int rc = launch_fp4_write(w, ctx->stream))
         return set_error(ctx, rc, "%s: launch failed: %s", who, cudaGetErrorString(cudaGetLastError()));
     return mem == PION_B200_MEM_HOST ? finish_sync(ctx) : 0;

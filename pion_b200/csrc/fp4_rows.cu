@@ -583,10 +583,12 @@ static int read_t(const ReadParams& p, cudaStream_t st) {
 
 }  // namespace fp4
 
+int fp4_write_launches(bool slots, int64_t n) { return slots && n > fp4::FEW ? 2 : 1; }
+
 int launch_fp4_write(const Fp4Write& w, cudaStream_t st) {
     using namespace fp4;
     if (w.n <= 0) return 0;
-    if (w.slots && w.n > FEW) {
+    if (fp4_write_launches(w.slots != nullptr, w.n) > 1) {
         if (launch_pdl(claim_kernel, dim3((unsigned)((w.n + 255) / 256)), 256, 0, st, w.slots, w.n,
                        w.n_slots, w.claim, w.status) != 0)
             return PION_B200_ECUDA;

@@ -485,6 +485,7 @@ struct Fp4Write {
     int* status = nullptr;
 };
 int launch_fp4_write(const Fp4Write& w, cudaStream_t st);
+int fp4_write_launches(bool slots, int64_t n);  // kernels of such a write
 struct Fp4Read {
     int format = 0;
     int dim = 0;
