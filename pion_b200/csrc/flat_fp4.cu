@@ -1474,8 +1474,9 @@ __global__ void __launch_bounds__(NT, NT > 256 ? 1 : 4) finish_kernel(const Fini
                                : __uint_as_float((uint32_t)(__ldcg(cand + i) >> 32));
             };
             uint32_t* list = reinterpret_cast<uint32_t*>(key);
+            // (-inf is an empty slot's: where the margin is known, no score of a row left float32)
             auto take = [&](float a, float cut, uint64_t row) {
-                if (a >= cut || !known) {
+                if ((a >= cut && a > -INFINITY) || !known) {
                     const int at = atomicAdd(&s_n, 1);
                     if (at < LIST) key[at] = row;
                 }

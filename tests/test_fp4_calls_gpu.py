@@ -18,3 +18,47 @@ def test_launches_are_counted_as_they_are_made(ctx):
         assert ctx.launches - before == want
     torch.cuda.synchronize()
     ctx.sync()
+
+
+def best_time(f, runs=5, calls=10):
+    """The least of some mean times of a call, in us."""
+    times = []
+    for _ in range(runs + 1):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        torch.cuda.synchronize()
+        a.record()
+        for _ in range(calls):
+            f()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) / calls * 1e3)
+    return min(times[1:])
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("n", [2500, 16000])
+def test_few_rows_among_many_empty_slots(ctx, fmt, n):
+    """A store searched at its capacity while it holds fewer than k rows: they are found, and the
+    empty slots are not scored one by one (16000 of them took 37 times as long as as many rows)."""
+    import pion_b200
+    rng = np.random.default_rng(n)
+    x = torch.from_numpy(rng.standard_normal((n, 4096)).astype(np.float32)).cuda()
+    full = pion_b200.quantize_rows_fp4(ctx, x, fmt)
+    few = pion_b200.FP4Rows(n, 4096, fmt)
+    at = [7, n // 2, n - 1]
+    few.write(ctx, x[at], slots=at)
+    ix = pion_b200.FlatFP4Index(ctx, few)
+    q = x[at][:2] + 0.1
+    ids, sc = ix.search(q, 10)
+    all_ids, all_sc = pion_b200.FlatFP4Index(ctx, full).search(q, 10)
+    torch.cuda.synchronize()
+    ctx.sync()
+    assert ids[:, 0].tolist() == at[:2] == all_ids[:, 0].tolist()
+    assert torch.equal(sc[:, 0], all_sc[:, 0])
+    for row in ids.tolist():
+        assert sorted(row[:3]) == sorted(at) and row[3:] == [-1] * 7
+    assert torch.isneginf(sc[:, 3:]).all()
+    a = best_time(lambda: ix.search(q, 10))
+    b = best_time(lambda: pion_b200.FlatFP4Index(ctx, full).search(q, 10))
+    print(f"{fmt} {n} slots: 3 rows {a:.0f} us, full {b:.0f} us")
+    assert a < 4 * b
