@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 import torch
 
+import fp4_plain as plain
+
 pytestmark = pytest.mark.gpu
 
 
@@ -62,3 +64,37 @@ def test_few_rows_among_many_empty_slots(ctx, fmt, n):
     b = best_time(lambda: pion_b200.FlatFP4Index(ctx, full).search(q, 10))
     print(f"{fmt} {n} slots: 3 rows {a:.0f} us, full {b:.0f} us")
     assert a < 4 * b
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+def test_host_arrays_of_every_kind(ctx, fmt):
+    """float16, float64 and bfloat16 rows in host memory, inside wider buffers, read-only, and lists:
+    what the same rows on the GPU give."""
+    import pion_b200
+    rng = np.random.default_rng(31)
+    wide = rng.standard_normal((600, 90))
+    wide.flags.writeable = False
+
+    def answers(x, q):
+        rows = pion_b200.quantize_rows_fp4(ctx, x, fmt)
+        ids, sc = pion_b200.FlatFP4Index(ctx, rows).search(q, 7)
+        s = pion_b200.fp4_scores(ctx, rows, q)
+        torch.cuda.synchronize()
+        ctx.sync()
+        back = rows.read(ctx)
+        return [torch.as_tensor(np.asarray(a.cpu() if torch.is_tensor(a) else a))
+                for a in (ids, sc, s, back)]
+
+    for host, dev in ((wide.astype(np.float16), torch.float16), (wide, torch.float32),
+                      (torch.from_numpy(wide.copy()).bfloat16(), torch.bfloat16),
+                      (wide.astype(np.float32)[::2], torch.float32)):
+        x, q = host[:, 5:82], host[::31, 5:82]
+        tx = torch.as_tensor(np.ascontiguousarray(x)) if not torch.is_tensor(x) else x
+        want = answers(tx.to(dev).cuda(), tx[::31].to(dev).cuda())
+        for a, b in zip(answers(x, q), want):
+            assert torch.equal(a.float(), b.float())
+    rows = pion_b200.FP4Rows(3, 4, fmt)
+    rows.write(ctx, [[1.0, 2.0, -3.0, 0.5]], slots=[2])
+    codes, bits, g = plain.quantise([[1.0, 2.0, -3.0, 0.5]], fmt)
+    want = (plain.values(codes, bits, fmt)[:, :4] * g[:, None].astype(np.float64)).astype(np.float32)
+    assert np.array_equal(rows.read(ctx, slots=(2,)).cpu().numpy(), want)
