@@ -5,9 +5,9 @@
 // lower nibble first, padded with zeros to a multiple of 128 elements; one scale byte per block
 // (MX: 32 elements, e8m0; NV: 16 elements, e4m3); and one float g per row.
 //
-// Scale bytes lie as the tensor cores take them: tiles of 128 rows, atoms of 4 blocks, 512
-// bytes per (tile, atom) as [row % 32][row / 32 % 4][block % 4], so that one
-// tcgen05.cp.32x128b moves an atom into four TMEM columns.
+// Scale bytes lie as the tensor cores take them from TMEM: tiles of 128 rows, atoms of 4 blocks,
+// 512 bytes per (tile, atom) as [row % 32][row / 32 % 4][block % 4], so that an atom is a 16-byte
+// word of each of 32 lanes, four columns.
 #pragma once
 
 #include <cstdint>
@@ -19,8 +19,8 @@ namespace fp4 {
 
 constexpr int kMX = PION_B200_FP4_MX;
 constexpr int kNV = PION_B200_FP4_NV;
-// The query tile's codes and scale atoms stay in shared memory: at 8192 dimensions 32
-// queries of the NV format take 128 + 64 KB of the 227 KB.
+// The query tile's codes and, where TMEM has no room for them, scale atoms stay in shared memory: at
+// 8192 dimensions each CTA of a pair holds 64 + 64 KB of its 227 KB for 32 queries of the NV format.
 constexpr int kMaxDim = 8192;
 
 __host__ __device__ constexpr int pad_dim(int dim) { return (dim + 127) / 128 * 128; }
@@ -142,14 +142,6 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
 template <int FMT>
 __device__ __forceinline__ float scale_value(uint32_t byte) {
     return FMT == kMX ? e8m0_value(byte) : e4m3_value(byte);
-}
-
-__device__ __forceinline__ uint32_t e4m3_byte(float v) {  // nearest, ties to even, saturating
-    uint32_t r;
-    asm("{\n\t.reg .b16 t;\n\tcvt.rn.satfinite.e4m3x2.f32 t, %2, %1;\n\tcvt.u32.u16 %0, t;\n\t}"
-        : "=r"(r)
-        : "f"(v), "f"(0.0f));
-    return r & 0xFFu;
 }
 
 }  // namespace fp4

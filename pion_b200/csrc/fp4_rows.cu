@@ -24,9 +24,9 @@ namespace fp4 {
 
 constexpr int WARPS = 8;   // per CTA that writes one row
 constexpr int NW = 2;      // per CTA that writes several: its place is soon free for the next
-                           // (262144 x 1536, us with 8: NV float32 330 -> 313, MX bfloat16
-                           // 246 -> 201)
-constexpr int READ_WARPS = 4;  // (bfloat16 with 8: 173 us -> 165)
+                           // (262144 x 1536 float32, us with 8 and with 2: NV 344 and 321, MX 304
+                           // and 292)
+constexpr int READ_WARPS = 4;  // (262144 x 1536 bfloat16, us with 8 and with 4: 170 and 166)
 constexpr int FEW = 1024;  // rows written by a CTA each
 constexpr int STEP = 256;  // elements per warp step, eight consecutive ones per lane
 
@@ -535,19 +535,24 @@ static int write_held(const WriteParams& p, cudaStream_t st) {
 
 template <int FMT, class T, bool VEC>
 static int write_v(const WriteParams& p, cudaStream_t st) {
-    // Few rows: a CTA each; many: a warp each (1536 float32 NV elements a row, us: 148 rows 2.4
-    // and 3.8, 1024 rows 4.9 and 5.8, 2048 rows 8.5 and 6.6).
+    // Few rows: a CTA each; many: a warp each (NV float32, 1536 elements, us a write in a graph of
+    // them: 148 rows 2.3 and 2.6, 1024 rows 4.7 and 4.7, 2048 rows 8.2 and 5.1).
     if (p.n <= FEW)
         return launch_pdl(write_kernel<FMT, T, VEC, WARPS, WARPS, 4, 0>, dim3((unsigned)p.n),
                           WARPS * 32, 0, st, p);
     if constexpr (FMT == kNV) {
-        // A row stays in one warp's registers while it leaves room for enough warps, then in two
-        // warps' (float32 / bfloat16, us, with eight warps a CTA: 262144 x 1536 330 / 285 in
-        // one, 365 / 385 in two; 131072 x 2048 284 / 205 and 216 / 226; 65536 x 4096 348 / 266
-        // read twice, 270 / 226 in two; with NW: 310 / 272, 210 / 181, 259 / 195).  Rows that
-        // fill the registers are written without checks (310 / 272 -> 285 / 230, 210 / 181 -> 198 /
-        // 148, 259 / 195 -> 230 / 158), and of others all steps but the last (float16, 100000 x
-        // 777: 78 -> 68, 60000 x 1900: 87 -> 71).
+        // A row stays in one warp's registers while that leaves room for enough warps, else in two
+        // warps', and is read twice only where neither holds it.  Steps known to lie inside the row
+        // are not checked against its end.  Medians of writes in turn, us:
+        //                            one warp   two warps   read twice   the variant taken, checked
+        //   262144 x 1536  float32      321         330         431          349
+        //                  bfloat16     225         278         395          270
+        //   131072 x 2048  float32      247         222         296          243
+        //                  bfloat16     148         173         262          181
+        //   65536 x 4096   float32                  244         307          280
+        //                  bfloat16                 161         259          196
+        //   100000 x 777   float16       67                                   76
+        //   60000 x 1900   float16       76                                   90
         if (p.dp <= 3 * STEP) return write_held<T, VEC, 1, 3>(p, st);
         if (p.dp <= 4 * STEP) return write_held<T, VEC, 1, 4>(p, st);
         if (p.dp <= 6 * STEP) return write_held<T, VEC, 1, 6>(p, st);
