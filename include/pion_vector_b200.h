@@ -538,7 +538,9 @@ int pion_v_b200_fp4_scores(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, i
  * of their error, (dp / 64 + 8) 2^-22 of the norms' product, that rests on measurement: at
  * least 15 times the largest error seen.)  k <= 256.  A query whose candidates overflow (thousands of rows that tie with
  * its k-th, or are as near to it as float32 sums with the longest row's norm can tell) is
- * answered by an exact scan of the rows: right, but about 1 ms a query and million rows. */
+ * answered by an exact scan of the rows: right, but about 1 ms a query and million rows.  One
+ * row 10^4 times longer than the rest makes that every query's case, until fp4_clear; so do
+ * k near 256 and 70 million rows and more. */
 int pion_v_b200_flat_fp4_knn(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, int64_t n_rows,
                              int64_t id_base, const void *q, int q_type, int64_t q_stride,
                              int64_t nq, int64_t k, int32_t *out_ids, float *out_scores,
