@@ -535,8 +535,8 @@ int pion_v_b200_fp4_scores(pion_b200_ctx *ctx, const pion_b200_fp4_rows *rows, i
  * out_scores [nq x k]; -1 / -inf past the rows that are not empty.  Here a score is the exact
  * ((sum) g_r) g_t, rounded once to float32, so the ids do not depend on an order of
  * summation.  (Which rows are summed exactly goes by the tensor cores' float32 sums and a bound
- * of their error, (dp / 64 + 8) 2^-22 of the norms' product, that rests on measurement: at
- * least 15 times the largest error seen.)  k <= 256.  A query whose candidates overflow (thousands of rows that tie with
+ * of their error, (dp / 64 + 8) 2^-22 of the norms' product, that rests on measurement: 2.5
+ * times the largest error of products made to lose most, 15 times that of random ones.)  k <= 256.  A query whose candidates overflow (thousands of rows that tie with
  * its k-th, or are as near to it as float32 sums with the longest row's norm can tell) is
  * answered by an exact scan of the rows: right, but about 1 ms a query and million rows.  One
  * row 10^4 times longer than the rest makes that every query's case, until fp4_clear; so do

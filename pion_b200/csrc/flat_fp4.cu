@@ -63,8 +63,9 @@ __host__ __device__ constexpr int atoms_per_stage(int fmt) { return fmt == kMX ?
 // Error bound of an approximate score: eps = rel_eps(dp) * |q| * |v| (norms bounded from the
 // block scales): two float32 steps of the running sum for every 64 elements, and eight more.
 // Measured over blocks of many magnitudes and q near v, where partial sums are largest:
-// 2^-23.5 at 64 elements, 2^-21.0 at 1536 and 2^-18.8 at 8192 (the bound: 2^-18.8, 2^-17.0
-// and 2^-14.9).
+// 2^-23.5 at 64 elements, 2^-21.0 at 1536 and 2^-18.8 at 8192 (the bound: 2^-18.7, 2^-17.0
+// and 2^-14.9).  Where every step is cut off, one large product and all others just below its last
+// bits: 2^-22.7, 2^-18.6 and 2^-16.2, about one step of the sum for every 64 elements.
 __host__ __device__ constexpr float rel_eps(int dp) { return (float)(dp / 64 + 8) * 0x1p-22f; }
 
 enum Mode { kScores = 0, kCollect = 1 };

@@ -143,3 +143,42 @@ def test_scores_of_more_than_two_to_31(ctx, dtype):
     ctx.sync()
     assert torch.equal(out[:, n - 515:], last)
     assert torch.equal(out[-3:], some)
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("dim", [64, 128, 1536, 8192])
+def test_error_bound_where_products_are_cut_off(ctx, fmt, dim):
+    """The search's premise, |approximate - exact| <= (dp / 64 + 8) 2^-22 |q| |v|, where an adder that
+    cuts off at its largest term loses most: one large product, all others just below its last bits,
+    of one sign, in the same step and in later ones."""
+    import pion_b200
+    block = plain.BLOCK[fmt]
+    xs, qs = [], []
+    for gap in range(8, 17):                 # small products are 2^-2gap of the large one
+        for extra in (0, 1):
+            for big, small in ((6.0, 6.0), (4.0, 6.0), (4.0, 1.0), (6.0, 1.5), (4.0, 3.0), (1.0, 6.0)):
+                for sign in (1.0, -1.0):
+                    x = np.full(dim, small * 2.0 ** (-gap - extra))
+                    q = np.full(dim, small * 2.0 ** -gap)
+                    x[:block], q[:block] = 0, 0
+                    x[0], q[0] = big, sign * big
+                    xs.append(x), qs.append(q)
+                    x, q = x.copy(), q.copy()          # the large one in the last block
+                    x[[0, dim - 1]], q[[0, dim - 1]] = x[[dim - 1, 0]], q[[dim - 1, 0]]
+                    x[dim - block:dim - 1] = q[dim - block:dim - 1] = 0
+                    x[1:block], q[1:block] = x[0], q[0]
+                    xs.append(x), qs.append(q)
+    x, q = np.float32(xs), np.float32(qs)
+    rows = pion_b200.quantize_rows_fp4(ctx, torch.from_numpy(x).cuda(), fmt)
+    got = pion_b200.fp4_scores(ctx, rows, torch.from_numpy(q).cuda())
+    torch.cuda.synchronize()
+    ctx.sync()
+    want, _ = plain.products(q.astype(np.float64), x.astype(np.float64), fmt)
+
+    def norms(v):
+        c, b, g = plain.quantise(v.astype(np.float64), fmt)
+        return np.linalg.norm(plain.values(c, b, fmt), axis=1) * g
+
+    off = (np.abs(got.double().cpu().numpy() - want) / (norms(q)[:, None] * norms(x))).max()
+    print(f"{fmt} dim {dim}: largest error {off:.3g} |q||v| = 2^{np.log2(off + 1e-30):.1f}")
+    assert off <= (plain.pad_dim(dim) / 64 + 8) * 2.0 ** -22
