@@ -250,7 +250,8 @@ int pion_v_b200_sync(pion_b200_ctx *ctx);
  * PION_B200_ETIMEOUT; the kernel then drains its copies and MMAs, frees its tensor
  * memory and returns, so the context stays usable.  (For tests, the environment
  * variable PION_B200_TEST_STALL=1 makes one CTA of each main pass wait on a barrier that
- * nothing arrives on.) */
+ * nothing arrives on; 2 and 3, in 4-bit products, the copies of the second or the first CTA of
+ * a pair.) */
 int pion_v_b200_set_wait_budget(pion_b200_ctx *ctx, int64_t ns);
 /* Message of the last failing call on this context ("" if none). */
 const char *pion_v_b200_last_error(const pion_b200_ctx *ctx);

@@ -189,7 +189,8 @@ size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 // call reports PION_B200_ETIMEOUT (no fault, the GPU stays usable).
 int test_stall() {
     const char* e = getenv("PION_B200_TEST_STALL");
-    return e && atoi(e) == 1 ? 1 : 0;
+    const int at = e ? atoi(e) : 0;
+    return at >= 1 && at <= 3 ? at : 0;
 }
 
 int timing_begin(pion_b200_ctx* ctx, int tag) {
@@ -708,7 +709,7 @@ int pion_v_b200_flat_i8_knn(pion_b200_ctx* ctx, const pion_b200_index* ix, const
             L.thr0 = pre ? tv + (kk - 1) : nullptr;
             L.thr0_stride = kk;
             L.bound_mode = 0;
-            L.test_stall = test_stall();
+            L.test_stall = test_stall() == 1;
             rc = launch_flat_i8_tc(L, st);
             ctx->launches++;
             timing_end(ctx, t_main);

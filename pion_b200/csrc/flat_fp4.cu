@@ -102,7 +102,8 @@ struct TcParams {
     uint64_t* cand;           // [nq][CAP]: approximate score bits << 32 | row
     int* status;
     uint64_t wait_ns;
-    int test_stall;           // the first pair's issuer waits on a barrier nothing arrives on
+    int test_stall;           // in the first pair a wait for a barrier nothing arrives on: 1 the
+                              // issuer, 2 the second CTA's copies after a stage, 3 the first's
 };
 
 // ------------------------------------------------------------- PTX pieces --
@@ -575,6 +576,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             for (int j = first; j < p.n_tiles && ok; j += stride) {
                 const int half_tile = tile_of(p, j) * 2 + (int)rank;
                 for (int kc = 0; kc < kchunks; ++kc) {
+                    if (p.test_stall > 1 && pair == 0 && (int)rank == 3 - p.test_stall && loads == 1)
+                        ok = mbar_wait(stall, 0, p.status, abort_flag, p.wait_ns);
+                    if (!ok) break;
                     if (!mbar_wait(&empty[stage], phase ^ 1u, p.status, abort_flag, p.wait_ns)) {
                         ok = false;
                         break;
@@ -616,7 +620,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const bool one = elect_one();
             int stage = 0, set = 0, buf = 0;
             uint32_t phase = 0, buf_phase = 0;
-            bool ok = !p.test_stall || blockIdx.x != 0;
+            bool ok = p.test_stall != 1 || blockIdx.x != 0;
             if (!ok) mbar_wait(stall, 0, p.status, abort_flag, p.wait_ns);
             ok = ok && __all_sync(0xffffffffu,
                                   mbar_wait(bcodes, 0, p.status, abort_flag, p.wait_ns));

@@ -307,7 +307,7 @@ int* call_status(pion_b200_ctx* ctx, int mem);
 int finish_sync(pion_b200_ctx* ctx);
 bool valid_ctx(const pion_b200_ctx* ctx);
 bool stream_capturing(cudaStream_t st);
-int test_stall();  // PION_B200_TEST_STALL=1
+int test_stall();  // PION_B200_TEST_STALL: 1, or 2 and 3 (4-bit product), else 0
 int use_device(pion_b200_ctx* ctx);
 size_t align_up(size_t x, size_t a);
 int prepass_tiles(int k);

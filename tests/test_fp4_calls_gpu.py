@@ -98,3 +98,43 @@ def test_host_arrays_of_every_kind(ctx, fmt):
     codes, bits, g = plain.quantise([[1.0, 2.0, -3.0, 0.5]], fmt)
     want = (plain.values(codes, bits, fmt)[:, :4] * g[:, None].astype(np.float64)).astype(np.float32)
     assert np.array_equal(rows.read(ctx, slots=(2,)).cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+@pytest.mark.parametrize("stall", ["1", "2", "3"])
+def test_waits_that_run_out_in_either_cta(ctx, monkeypatch, fmt, stall):
+    """The issuing warp, or the copies of one CTA of a pair, wait for what never comes: the CTAs have
+    copied different numbers of stages when they give up; they settle what is in flight, the call
+    reports it, and the next is right."""
+    import time
+
+    import pion_b200
+    rng = np.random.default_rng(17)
+    x = torch.from_numpy(rng.standard_normal((30000, 1000)).astype(np.float32)).cuda()
+    rows = pion_b200.quantize_rows_fp4(ctx, x, fmt)
+    ix = pion_b200.FlatFP4Index(ctx, rows)
+    q = x[:600] + 0.1
+    for nq in (1, 600):
+        want = pion_b200.fp4_scores(ctx, rows, q[:nq])
+        ids, sc = ix.search(q[:nq], 10)
+        torch.cuda.synchronize()
+        ctx.sync()
+        ctx.set_wait_budget(1_000_000)
+        monkeypatch.setenv("PION_B200_TEST_STALL", stall)
+        try:
+            for call in (lambda: pion_b200.fp4_scores(ctx, rows, q[:nq]), lambda: ix.search(q[:nq], 10)):
+                t0 = time.perf_counter()
+                call()
+                torch.cuda.synchronize()
+                assert time.perf_counter() - t0 < 1.5      # no wait of the drain's own 2 s ran out
+                with pytest.raises(pion_b200.PionError) as e:
+                    ctx.sync()
+                assert e.value.code == -11
+        finally:
+            monkeypatch.delenv("PION_B200_TEST_STALL")
+            ctx.set_wait_budget(0)
+        assert torch.equal(pion_b200.fp4_scores(ctx, rows, q[:nq]), want)
+        again = ix.search(q[:nq], 10)
+        assert torch.equal(again[0], ids) and torch.equal(again[1], sc)
+        torch.cuda.synchronize()
+        ctx.sync()
