@@ -237,7 +237,8 @@ int pion_v_b200_ctx_device(const pion_b200_ctx *ctx);
  * framework's current stream; NULL restores the context's own stream (pass
  * cudaStreamLegacy for the legacy default stream).  Work queued after a switch waits
  * for the work already queued on the previous stream (the context's scratch is
- * shared), without blocking the host. */
+ * shared), without blocking the host; so a stream that is being captured is refused
+ * (PION_B200_EINVAL) while the previous one is not, and the capture goes on. */
 int pion_v_b200_set_stream(pion_b200_ctx *ctx, void *cuda_stream);
 /* Waits for the context's stream and returns the first error any device-side wait
  * recorded since the last call (PION_B200_ETIMEOUT), else 0.  A call with host buffers

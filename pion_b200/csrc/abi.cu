@@ -300,6 +300,9 @@ int pion_v_b200_set_stream(pion_b200_ctx* ctx, void* cuda_stream) {
         // The context's scratch is shared by both streams: work queued from now on waits
         // for everything already queued on the previous stream.
         if (int rc = use_device(ctx)) return rc;
+        // a capture cannot wait for work outside it, and trying to would end it
+        if (stream_capturing(next) && !stream_capturing(ctx->stream))
+            return set_error(ctx, PION_B200_EINVAL, "set_stream: the stream is being captured");
         if (!ctx->switch_ev &&
             cudaEventCreateWithFlags(&ctx->switch_ev, cudaEventDisableTiming) != cudaSuccess)
             return set_error(ctx, PION_B200_ECUDA, "set_stream: event create failed");

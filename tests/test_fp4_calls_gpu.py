@@ -138,3 +138,29 @@ def test_waits_that_run_out_in_either_cta(ctx, monkeypatch, fmt, stall):
         assert torch.equal(again[0], ids) and torch.equal(again[1], sc)
         torch.cuda.synchronize()
         ctx.sync()
+
+
+def test_host_memory_is_refused_while_capturing(ctx):
+    """The refusal leaves the capture, the context and torch as they were."""
+    import pion_b200
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((300, 64)).astype(np.float32)
+    rows = pion_b200.quantize_rows_fp4(ctx, x, "nv")
+    ix = pion_b200.FlatFP4Index(ctx, rows)
+    tq = torch.from_numpy(x[:4]).cuda()
+    want = [t.clone() for t in ix.search(tq, 5)]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for bad in (lambda: rows.write(ctx, x[:3], start=0), lambda: ix.search(x[:4], 5),
+                    lambda: pion_b200.fp4_scores(ctx, rows, x[:4])):
+            with pytest.raises(pion_b200.PionError) as e:
+                bad()
+            assert e.value.code == -1
+        out = ix.search(tq, 5)
+    g.replay()
+    torch.cuda.synchronize()
+    ctx.sync()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    ids, sc = ix.search(x[:4], 5)
+    assert np.array_equal(ids, want[0].cpu().numpy())
