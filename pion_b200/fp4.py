@@ -160,8 +160,8 @@ class FP4Rows:
             device = torch.device("cuda" if device is None else device)
             codes = torch.zeros((n_rows, cb // max(n_rows, 1)), dtype=torch.uint8, device=device)
             scales = torch.zeros(sb, dtype=torch.uint8, device=device)
-            row_scale = torch.full((n_rows,), float("nan"), device=device)
-            norm_max = torch.zeros(1, device=device)
+            row_scale = torch.full((n_rows,), float("nan"), dtype=torch.float32, device=device)
+            norm_max = torch.zeros(1, dtype=torch.float32, device=device)
             claim = torch.zeros(n_rows, dtype=torch.int32, device=device)
         elif codes is None or scales is None or row_scale is None or norm_max is None:
             raise ValueError("a store of given tensors needs codes, scales, row_scale and norm_max")

@@ -22,3 +22,18 @@ def test_a_lone_claim_buffer_is_refused():
     claim = torch.zeros(4, dtype=torch.int32)
     with pytest.raises(ValueError, match="claim"):
         pion_b200.FP4Rows(4, 16, "nv", device="cpu", claim=claim)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.bfloat16, torch.float16])
+def test_a_new_store_does_not_go_by_torchs_default_dtype(dtype):
+    """A model's program often sets one: the kernels read and write float32 scales and norms."""
+    import pion_b200
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(dtype)
+    try:
+        rows = pion_b200.FP4Rows(5, 16, "nv", device="cpu")
+    finally:
+        torch.set_default_dtype(before)
+    assert rows.row_scale.dtype == rows.norm_max.dtype == torch.float32
+    assert rows.codes.dtype == rows.scales.dtype == torch.uint8 and rows.claim.dtype == torch.int32
+    assert torch.isnan(rows.row_scale).all() and rows.norm_max.item() == 0
