@@ -178,13 +178,23 @@ class FP4Rows:
                     raise ValueError(f"{name} must be {size} contiguous {dtype} values")
                 if at < 0 or t.get_device() != at:
                     raise ValueError(f"{name} must be on the store's CUDA device")
-        self.n_rows, self.dim, self.format = n_rows, dim, format
-        self.codes, self.scales, self.row_scale = codes, scales, row_scale
-        self.norm_max, self.claim = norm_max, claim
+        self._n_rows, self._dim, self._format = n_rows, dim, format
+        self._codes, self._scales, self._row_scale = codes, scales, row_scale
+        self._norm_max, self._claim = norm_max, claim
         self._c = _lib.FP4RowsDesc(
             FORMATS[format], 0, n_rows, dim, codes.data_ptr(), scales.data_ptr(),
             row_scale.data_ptr(), norm_max.data_ptr(),
             claim.data_ptr() if claim is not None else None)
+
+    # What _c holds the addresses and sizes of stays as it is.
+    n_rows = property(lambda self: self._n_rows)
+    dim = property(lambda self: self._dim)
+    format = property(lambda self: self._format)
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    row_scale = property(lambda self: self._row_scale)
+    norm_max = property(lambda self: self._norm_max)
+    claim = property(lambda self: self._claim)
 
     @property
     def device(self):

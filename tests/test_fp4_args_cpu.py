@@ -37,3 +37,15 @@ def test_a_new_store_does_not_go_by_torchs_default_dtype(dtype):
     assert rows.row_scale.dtype == rows.norm_max.dtype == torch.float32
     assert rows.codes.dtype == rows.scales.dtype == torch.uint8 and rows.claim.dtype == torch.int32
     assert torch.isnan(rows.row_scale).all() and rows.norm_max.item() == 0
+
+
+def test_a_stores_tensors_and_sizes_stay():
+    """The calls pass their addresses and sizes as they were at first: another tensor or size put in
+    their place would not be seen, and the old memory freed."""
+    import pion_b200
+    rows = pion_b200.FP4Rows(5, 16, "nv", device="cpu")
+    for name in ("codes", "scales", "row_scale", "norm_max", "claim", "n_rows", "dim", "format"):
+        was = getattr(rows, name)
+        with pytest.raises(AttributeError):
+            setattr(rows, name, was)
+        assert getattr(rows, name) is was
