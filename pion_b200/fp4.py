@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 
 import numpy as np
 
@@ -68,6 +69,14 @@ def _call(ctx: Context, fn, *args, mem: int = MEM_DEVICE):
     finally:
         if before != _device_of(ctx):
             torch.cuda.set_device(before)
+
+
+def _int64(x, what: str) -> int:
+    """x as an int of 64 bits (ctypes would wrap a larger one)."""
+    x = operator.index(x)
+    if not -2 ** 63 <= x < 2 ** 63:
+        raise ValueError(f"{what} {x} is past 64 bits")
+    return x
 
 
 def _matrix(ctx: Context, x, what: str, dim: int):
@@ -153,6 +162,7 @@ class FP4Rows:
 
     def __init__(self, n_rows: int, dim: int, format: str = "nv", device=None, *, codes=None,
                  scales=None, row_scale=None, norm_max=None, claim=None):
+        n_rows, dim = _int64(n_rows, "n_rows"), _int64(dim, "dim")
         cb, sb = _sizes(format, n_rows, dim)
         if codes is None and scales is None and row_scale is None and norm_max is None:
             if claim is not None:
@@ -221,20 +231,20 @@ class FP4Rows:
             if len(slots) != n:
                 raise ValueError(f"{len(slots)} slots for {n} rows")
             ps = slots.data_ptr()
-        _call(ctx, ctx.lib.pion_v_b200_fp4_write, self._ref(ctx), p, typ, stride, n, ps, start,
-              mem=mem)
+        _call(ctx, ctx.lib.pion_v_b200_fp4_write, self._ref(ctx), p, typ, stride, n, ps,
+              _int64(start, "start"), mem=mem)
 
     def read(self, ctx: Context, slots=None, start: int = 0, count: int | None = None,
              dtype=None, out=None):
         """Slots ``slots``, or ``count`` slots from ``start`` (default: all), as rows [n, dim] of
         ``dtype`` (default float32) on the store's device, or into ``out``.  An empty slot
         reads as NaN; a negative one leaves its row of ``out`` as it was (undefined without)."""
-        ps = None
+        ps, start = None, _int64(start, "start")
         if slots is not None:
             slots = _slots(ctx, slots, MEM_DEVICE)
             n, ps = len(slots), slots.data_ptr()
         else:
-            n = self.n_rows - start if count is None else count
+            n = self.n_rows - start if count is None else _int64(count, "count")
         out, typ, stride = _output(out, (max(n, 0), self.dim), dtype, self.device)
         _call(ctx, ctx.lib.pion_v_b200_fp4_read, self._ref(ctx), ps, start, n, out.data_ptr(), typ,
               stride)
@@ -265,7 +275,7 @@ def fp4_scores(ctx: Context, rows: FP4Rows, q, n_rows: int | None = None, dtype=
     """Scores [nq, n_rows] of the queries ``q`` [nq, dim] (quantised in the store's format) with
     the rows of slots [0, n_rows), accumulated in float32; -inf for an empty slot.  Into ``out``
     (rows may be strided) or a new tensor of ``dtype`` (default float32), in q's memory."""
-    n = rows.n_rows if n_rows is None else n_rows
+    n = rows.n_rows if n_rows is None else _int64(n_rows, "n_rows")
     p, typ, stride, nq, mem, keep = _matrix(ctx, q, "q", rows.dim)
     out, otyp, ostride = _output(out, (nq, max(n, 0)), dtype,
                                  rows.device if mem == MEM_DEVICE else torch.device("cpu"))
@@ -284,7 +294,7 @@ class FlatFP4Index:
     def __init__(self, ctx: Context, rows, id_base: int = 0, format: str = "nv"):
         self.ctx = ctx
         self.rows = rows if isinstance(rows, FP4Rows) else quantize_rows_fp4(ctx, rows, format)
-        self.id_base = id_base
+        self.id_base = _int64(id_base, "id_base")
         self.dim = self.rows.dim
 
     @property
@@ -295,7 +305,7 @@ class FlatFP4Index:
         """Top-k of slots [0, n_rows) by (score desc, id asc) per query -> (ids int32 [nq, k],
         scores float32 [nq, k]), in q's memory; -1 / -inf past the rows that are not empty."""
         ctx, rows = self.ctx, self.rows
-        n = rows.n_rows if n_rows is None else n_rows
+        n, k = rows.n_rows if n_rows is None else _int64(n_rows, "n_rows"), _int64(k, "k")
         p, typ, stride, nq, mem, keep = _matrix(ctx, q, "q", rows.dim)
         device = rows.device if mem == MEM_DEVICE else torch.device("cpu")
         ids = torch.empty((nq, max(k, 0)), dtype=torch.int32, device=device)

@@ -49,3 +49,16 @@ def test_a_stores_tensors_and_sizes_stay():
         with pytest.raises(AttributeError):
             setattr(rows, name, was)
         assert getattr(rows, name) is was
+
+
+
+def test_numbers_past_64_bits_are_refused():
+    """ctypes would wrap them: a start of 2^64 is not slot 0."""
+    from pion_b200 import fp4
+    for bad in (2 ** 64, 2 ** 63, -2 ** 63 - 1):
+        with pytest.raises(ValueError):
+            fp4._int64(bad, "start")
+    for good in (0, -1, 2 ** 63 - 1, np.int64(7), np.uint32(9)):
+        assert fp4._int64(good, "start") == good and type(fp4._int64(good, "start")) is int
+    with pytest.raises(TypeError):
+        fp4._int64(1.5, "start")
