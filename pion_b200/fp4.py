@@ -144,6 +144,7 @@ def _sizes(format: str, n_rows: int, dim: int):
     """Bytes of a store's codes and scales."""
     if format not in FORMATS:
         raise ValueError(f"format must be one of {sorted(FORMATS)}, got {format!r}")
+    n_rows, dim = _int64(n_rows, "n_rows"), _int64(dim, "dim")
     cb, sb = ctypes.c_int64(), ctypes.c_int64()
     rc = _lib.load().pion_v_b200_fp4_sizes(FORMATS[format], n_rows, dim, ctypes.byref(cb),
                                            ctypes.byref(sb))
@@ -162,7 +163,6 @@ class FP4Rows:
 
     def __init__(self, n_rows: int, dim: int, format: str = "nv", device=None, *, codes=None,
                  scales=None, row_scale=None, norm_max=None, claim=None):
-        n_rows, dim = _int64(n_rows, "n_rows"), _int64(dim, "dim")
         cb, sb = _sizes(format, n_rows, dim)
         if codes is None and scales is None and row_scale is None and norm_max is None:
             if claim is not None:
@@ -197,21 +197,21 @@ class FP4Rows:
             claim.data_ptr() if claim is not None else None)
 
     # What _c holds the addresses and sizes of stays as it is.
-    n_rows = property(lambda self: self._n_rows)
-    dim = property(lambda self: self._dim)
-    format = property(lambda self: self._format)
-    codes = property(lambda self: self._codes)
-    scales = property(lambda self: self._scales)
-    row_scale = property(lambda self: self._row_scale)
-    norm_max = property(lambda self: self._norm_max)
-    claim = property(lambda self: self._claim)
+    n_rows = property(operator.attrgetter("_n_rows"))
+    dim = property(operator.attrgetter("_dim"))
+    format = property(operator.attrgetter("_format"))
+    codes = property(operator.attrgetter("_codes"))
+    scales = property(operator.attrgetter("_scales"))
+    row_scale = property(operator.attrgetter("_row_scale"))
+    norm_max = property(operator.attrgetter("_norm_max"))
+    claim = property(operator.attrgetter("_claim"))
 
     @property
     def device(self):
-        return self.codes.device
+        return self._codes.device
 
     def _ref(self, ctx: Context):
-        if self.codes.get_device() != _device_of(ctx):
+        if self._codes.get_device() != _device_of(ctx):
             raise ValueError(f"the store is on {self.device}, the context on device "
                              f"{_device_of(ctx)}")
         return ctypes.byref(self._c)
@@ -224,7 +224,7 @@ class FP4Rows:
     def write(self, ctx: Context, src, slots=None, start: int = 0):
         """Quantises the rows of ``src`` [n, dim] into slots ``slots[i]``, or ``start + i``.
         A negative slot skips its row; of several rows for one slot the last is kept."""
-        p, typ, stride, n, mem, keep = _matrix(ctx, src, "src", self.dim)
+        p, typ, stride, n, mem, keep = _matrix(ctx, src, "src", self._dim)
         ps = None
         if slots is not None:
             slots = _slots(ctx, slots, mem)
@@ -232,20 +232,20 @@ class FP4Rows:
                 raise ValueError(f"{len(slots)} slots for {n} rows")
             ps = slots.data_ptr()
         _call(ctx, ctx.lib.pion_v_b200_fp4_write, self._ref(ctx), p, typ, stride, n, ps,
-              _int64(start, "start"), mem=mem)
+              start and _int64(start, "start"), mem=mem)
 
     def read(self, ctx: Context, slots=None, start: int = 0, count: int | None = None,
              dtype=None, out=None):
         """Slots ``slots``, or ``count`` slots from ``start`` (default: all), as rows [n, dim] of
         ``dtype`` (default float32) on the store's device, or into ``out``.  An empty slot
         reads as NaN; a negative one leaves its row of ``out`` as it was (undefined without)."""
-        ps, start = None, _int64(start, "start")
+        ps, start = None, start and _int64(start, "start")
         if slots is not None:
             slots = _slots(ctx, slots, MEM_DEVICE)
             n, ps = len(slots), slots.data_ptr()
         else:
             n = self.n_rows - start if count is None else _int64(count, "count")
-        out, typ, stride = _output(out, (max(n, 0), self.dim), dtype, self.device)
+        out, typ, stride = _output(out, (max(n, 0), self._dim), dtype, self.device)
         _call(ctx, ctx.lib.pion_v_b200_fp4_read, self._ref(ctx), ps, start, n, out.data_ptr(), typ,
               stride)
         return out
@@ -267,7 +267,7 @@ def _workspace(ctx: Context, rows: FP4Rows, n_rows: int, nq: int, k: int, mem: i
         if mem == MEM_DEVICE else 0
     if need <= 0:
         return None, None, 0  # host memory, nothing to hold, or sizes that the call refuses
-    ws = rows.codes.new_empty(need)
+    ws = rows._codes.new_empty(need)
     return ws, ws.data_ptr(), need
 
 
@@ -294,7 +294,7 @@ class FlatFP4Index:
     def __init__(self, ctx: Context, rows, id_base: int = 0, format: str = "nv"):
         self.ctx = ctx
         self.rows = rows if isinstance(rows, FP4Rows) else quantize_rows_fp4(ctx, rows, format)
-        self.id_base = _int64(id_base, "id_base")
+        self.id_base = id_base and _int64(id_base, "id_base")
         self.dim = self.rows.dim
 
     @property
@@ -305,7 +305,7 @@ class FlatFP4Index:
         """Top-k of slots [0, n_rows) by (score desc, id asc) per query -> (ids int32 [nq, k],
         scores float32 [nq, k]), in q's memory; -1 / -inf past the rows that are not empty."""
         ctx, rows = self.ctx, self.rows
-        n, k = rows.n_rows if n_rows is None else _int64(n_rows, "n_rows"), _int64(k, "k")
+        n, k = rows.n_rows if n_rows is None else _int64(n_rows, "n_rows"), operator.index(k)
         p, typ, stride, nq, mem, keep = _matrix(ctx, q, "q", rows.dim)
         device = rows.device if mem == MEM_DEVICE else torch.device("cpu")
         ids = torch.empty((nq, max(k, 0)), dtype=torch.int32, device=device)

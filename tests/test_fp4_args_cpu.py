@@ -62,3 +62,8 @@ def test_numbers_past_64_bits_are_refused():
         assert fp4._int64(good, "start") == good and type(fp4._int64(good, "start")) is int
     with pytest.raises(TypeError):
         fp4._int64(1.5, "start")
+    import pion_b200
+    with pytest.raises(ValueError):
+        pion_b200.FP4Rows(2 ** 64 + 4, 16, "nv", device="cpu")
+    with pytest.raises(ValueError):
+        pion_b200.FP4Rows(4, 2 ** 64 + 16, "nv", device="cpu")
